@@ -144,6 +144,19 @@ PROTOTYPES = {
         [_p, _i64, _kvp, _i32, _i32, _p, _p, _p, _p, _p, _i64, _p, _i64, _p, _sz, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
          _f32, _i32, _i32, _i32, _i32, _i32, _i32, _p, _p],
     ),
+    "dgpt_fmha_packed": (
+        C.c_int,
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32,
+         _i32, _p, _p],
+    ),
+    "dgpt_tree_attn_splits": (_i32, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "dgpt_tree_attn_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "dgpt_tree_attn": (
+        C.c_int,
+        [_p, _i64, _kvp, _i64, _p, _p, _p, _i32, _p, _i64, _p, _sz, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _p, _p],
+    ),
+    "dgpt_token_logprobs": (C.c_int, [_p, _i64, _p, _f32, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _p]),
+    "dgpt_kv_keep": (C.c_int, [_kvp, _i64, _p, _p, _p, _p, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _p, _p]),
     "dgpt_silu_mul": (C.c_int, [_p, _p, _i64, _i32, _p]),
     "dgpt_embed_streams": (
         C.c_int, [_p, _p, _p, _p, _i32, _p, _i64, _i64, _i64, _p, _i32, _p, _f32, _p, _p, _i32, _i32, _i32, _i32, _p]
@@ -169,6 +182,7 @@ PROTOTYPES = {
     "dgpt_xielu": (C.c_int, [_p, _p, _i64, _f32, _f32, _i32, _p]),
 }
 _NOT_LAUNCHING = {
+    "dgpt_tree_attn_splits", "dgpt_tree_attn_workspace_bytes",
     "dgpt_last_error", "dgpt_version", "dgpt_decode_attn_workspace_bytes", "dgpt_decode_attn_static_capacity_bytes",
     "dgpt_small_gpt_supported", "dgpt_lmhead_workspace_bytes", "dgpt_latent_attn_workspace_bytes", "dgpt_retention_workspace_bytes",
 }

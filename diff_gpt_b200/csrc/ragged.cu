@@ -1,0 +1,125 @@
+// Entry points of attention over packed prompts and over trees of drafted tokens: checks, and which kernel takes a call.
+#include "ragged.cuh"
+
+using namespace dgpt;
+
+static bool head_dim_ok(int D) { return D == 8 || D == 16 || D == 32 || D == 64 || D == 128; }
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+extern "C" int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k, int64_t k_row_stride,
+                                int64_t k_head_stride, const void* v, int64_t v_row_stride, int64_t v_head_stride, void* o,
+                                int64_t o_row_stride, int64_t o_head_stride, float* lse, const int32_t* seq_starts,
+                                const int32_t* key_starts, int32_t n_seq, int32_t n_rows, int32_t n_keys, int32_t H, int32_t G, int32_t D,
+                                float scale, int32_t dtype, int32_t impl, int32_t* status, void* stream) {
+  DGPT_REQUIRE(n_seq >= 0 && n_rows >= 0 && n_keys >= 0 && H > 0 && G > 0 && H % G == 0, "fmha_packed: bad sizes");
+  DGPT_REQUIRE(key_starts || n_keys == n_rows, "fmha_packed: without starts of their own the keys are as many as the queries");
+  DGPT_REQUIRE(scale > 0.f, "fmha_packed: the scale must be positive");
+  DGPT_REQUIRE(impl >= 0 && impl <= 2, "fmha_packed: impl must be 0 (choose), 1 (CUDA cores) or 2 (tensor cores)");
+  if (dtype != DGPT_F32 && dtype != DGPT_BF16) {
+    set_error("fmha_packed: unknown dtype %d", dtype);
+    return DGPT_E_UNSUPPORTED;
+  }
+  if (!head_dim_ok(D)) {
+    set_error("fmha_packed: head_dim %d is not built", D);
+    return DGPT_E_UNSUPPORTED;
+  }
+  if (n_seq == 0 || n_rows == 0) return DGPT_OK;
+  DGPT_REQUIRE(q && o && seq_starts && (n_keys == 0 || (k && v)), "fmha_packed: NULL pointer");
+  DGPT_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "fmha_packed: pointers must be 16-byte aligned");
+  const int64_t strides[8] = {q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride, o_row_stride, o_head_stride};
+  for (int64_t s : strides) DGPT_REQUIRE(s >= D && s % 8 == 0, "fmha_packed: strides must be multiples of 8 elements, and rows and heads apart");
+  PackedProblem p;
+  p.q = q; p.k = k; p.v = v; p.o = o;
+  p.q_rs = q_row_stride; p.q_hs = q_head_stride;
+  p.k_rs = k_row_stride; p.k_hs = k_head_stride;
+  p.v_rs = v_row_stride; p.v_hs = v_head_stride;
+  p.o_rs = o_row_stride; p.o_hs = o_head_stride;
+  p.lse = lse;
+  p.q_starts = seq_starts;
+  p.k_starts = key_starts ? key_starts : seq_starts;
+  p.n_seq = n_seq; p.n_rows = n_rows; p.n_keys = n_keys; p.H = H; p.G = G;
+  p.scale_log2 = scale * kLog2e;
+  p.status = status;
+  if (impl == 2) {
+    set_error("fmha_packed: the tensor-core kernel does not cover dtype %d, head_dim %d", dtype, D);
+    return DGPT_E_UNSUPPORTED;
+  }
+  return packed_simt(p, D, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int32_t dgpt_tree_attn_splits(int32_t B, int32_t T, int32_t H, int32_t G, int32_t D, int32_t max_keys, int32_t dtype) {
+  (void)D;
+  (void)dtype;
+  if (B <= 0 || T <= 0 || H <= 0 || G <= 0 || H % G != 0 || max_keys <= 0) return 1;
+  const long long rows = (long long)T * (H / G), tiles = rows <= 16 ? 1 : (rows + 63) / 64;
+  const long long items = (long long)B * G * tiles;
+  const long long want = (2 * 148 + items - 1) / items, most = (max_keys + 255) / 256;
+  const long long n = want < most ? want : most;
+  return (int32_t)(n < 1 ? 1 : n > 256 ? 256 : n);
+}
+
+extern "C" size_t dgpt_tree_attn_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t D, int32_t n_splits) {
+  if (B <= 0 || T <= 0 || H <= 0 || D <= 0 || n_splits <= 1) return 0;
+  return ((size_t)B * T * H * n_splits * (D + 1) * sizeof(float) + 15) / 16 * 16;
+}
+
+extern "C" int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv_layout* kv, int64_t kv_token_stride, const int32_t* ctx_len,
+                              const int32_t* n_nodes, const uint64_t* ancestors, int32_t words, void* out, int64_t out_row_stride,
+                              void* workspace, size_t workspace_bytes, int32_t n_splits, int32_t B, int32_t T, int32_t H, int32_t G, int32_t D,
+                              float scale, int32_t dtype, int32_t impl, int32_t* status, void* stream) {
+  DGPT_REQUIRE(B >= 0 && T >= 0 && H > 0 && G > 0 && H % G == 0, "tree_attn: bad sizes");
+  DGPT_REQUIRE(T <= 256, "tree_attn: at most 256 drafted tokens per sequence, got %d", T);
+  DGPT_REQUIRE((long long)words * 64 >= T && words <= 4, "tree_attn: %d words of ancestors do not hold %d nodes", words, T);
+  DGPT_REQUIRE(scale > 0.f, "tree_attn: the scale must be positive");
+  DGPT_REQUIRE(impl >= 0 && impl <= 2, "tree_attn: impl must be 0 (choose), 1 (CUDA cores) or 2 (tensor cores)");
+  DGPT_REQUIRE(n_splits >= 1 && n_splits <= 256, "tree_attn: n_splits must be 1 to 256");
+  if (dtype != DGPT_F32 && dtype != DGPT_BF16) {
+    set_error("tree_attn: unknown dtype %d", dtype);
+    return DGPT_E_UNSUPPORTED;
+  }
+  if (!head_dim_ok(D)) {
+    set_error("tree_attn: head_dim %d is not built", D);
+    return DGPT_E_UNSUPPORTED;
+  }
+  if (B == 0 || T == 0) return DGPT_OK;
+  DGPT_REQUIRE(q && ctx_len && ancestors && out, "tree_attn: NULL pointer");
+  if (int e = validate_kv(kv, D)) return e;
+  DGPT_REQUIRE(aligned16(q) && aligned16(out), "tree_attn: pointers must be 16-byte aligned");
+  DGPT_REQUIRE(q_row_stride >= (int64_t)H * D && out_row_stride >= (int64_t)H * D && q_row_stride % 8 == 0 && out_row_stride % 8 == 0,
+               "tree_attn: row strides must be multiples of 8 elements that hold a row");
+  DGPT_REQUIRE(kv_token_stride >= D && kv_token_stride % 8 == 0, "tree_attn: the token stride must be a multiple of 8 elements that holds a head");
+  DGPT_REQUIRE(kv->head_stride >= 0 && kv->page_stride >= 0 && kv->n_pages >= 0, "tree_attn: strides and pages must not be negative");
+  const size_t need = dgpt_tree_attn_workspace_bytes(B, T, H, D, n_splits);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
+    set_error("tree_attn: workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    return DGPT_E_WORKSPACE;
+  }
+  DGPT_REQUIRE(aligned16(workspace), "tree_attn: the workspace must be 16-byte aligned");
+  TreeProblem p;
+  p.q = q;
+  p.q_rs = q_row_stride;
+  p.kv = make_view(kv);
+  p.kv.token_stride = kv_token_stride;
+  p.ctx = ctx_len;
+  p.n_nodes = n_nodes;
+  p.ancestors = reinterpret_cast<const unsigned long long*>(ancestors);
+  p.words = words;
+  p.o = out;
+  p.o_rs = out_row_stride;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_lse = n_splits > 1 ? p.part_o + (size_t)B * T * H * n_splits * D : nullptr;
+  p.n_splits = n_splits;
+  p.B = B; p.T = T; p.H = H; p.G = G; p.D = D;
+  p.group = H / G;
+  p.rows_per_tile = p.tiles = 0;
+  p.scale_log2 = scale * kLog2e;
+  p.status = status;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (impl == 2) {
+    set_error("tree_attn: the tensor-core kernel does not cover dtype %d, head_dim %d with this layout", dtype, D);
+    return DGPT_E_UNSUPPORTED;
+  }
+  const int rc = tree_simt(p, dtype, st);
+  if (rc != DGPT_OK || n_splits == 1) return rc;
+  return tree_merge(p, dtype, st);
+}

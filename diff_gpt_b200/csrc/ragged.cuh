@@ -1,0 +1,190 @@
+// Attention over sequences whose lengths lie on the device: packed prompts and trees of drafted tokens.
+//
+// Both are rows of queries against the keys of one sequence and one key/value head,
+//   o_r = sum_j p_rj v_j,   p_r = softmax_j(q_r . k_j * scale) over the keys that row r sees,
+// and differ in which rows lie side by side, where keys lie and which of them a row sees.  A problem struct answers these for the
+// kernels (ragged_simt.cu on the CUDA cores, ragged_tc.cu on the tensor cores): `item` turns a work item's number into the rows
+// and keys of one tile, `q_row`, `k_row`, `v_row` give addresses, `sees` the mask, `o_row` where a row's result goes.
+#pragma once
+
+#include "common.cuh"
+
+namespace dgpt {
+
+// One tile of up to BM rows against keys [key0, key1) of a sequence.
+struct RaggedItem {
+  int rows;        // rows of the tile that exist
+  int seq, g, h;   // sequence, key/value head, query head of the tile (packed) or first query head of its group (tree)
+  int row0;        // first row: token (packed), node * group + head in group (tree)
+  int key0, key1;  // keys of this item; the sequence's first `clear` keys are seen by every row
+  int clear;
+  int last0;       // packed: the last key that the tile's first row sees (negative: none); row r sees r more
+  int split;       // tree: which share of the keys
+  long long kbase; // packed: row of the sequence's key 0
+};
+
+// ---- packed prompts ---------------------------------------------------------------------------------------------
+// Sequence s owns query rows [q_starts[s], q_starts[s + 1]) and key rows [k_starts[s], k_starts[s + 1]); its last query sees all of
+// its keys, the one before all but the last, and so on.
+//
+// Tiles of BM rows start at a sequence's first row, so their number follows from all lengths, which the host does not know.
+// Without a pass that counts them: sequence s takes the tile slots from base(s) = q_starts[s] / BM + s on.  A sequence of n rows has
+// ceil(n / BM) tiles, and base(s + 1) - base(s) is never less than that, so no two tiles share a slot; at most one slot a sequence stays
+// empty, and a binary search over base() finds a slot's sequence.
+struct PackedProblem {
+  const void *q, *k, *v;
+  long long q_rs, q_hs, k_rs, k_hs, v_rs, v_hs, o_rs, o_hs;
+  void* o;
+  float* lse;  // [n_rows, H] or NULL
+  const int *q_starts, *k_starts;
+  int n_seq, n_rows, n_keys, H, G;
+  float scale_log2;
+  int* status;
+
+  __host__ __device__ long long slots(int bm) const { return (long long)n_rows / bm + n_seq; }
+  // A start is taken into the tensor's rows: wrong numbers give wrong rows, never an access outside.
+  __device__ int q_start(int s) const { return min(max(q_starts[s], 0), n_rows); }
+  __device__ int k_start(int s) const { return min(max(k_starts[s], 0), n_keys); }
+  __device__ bool item(long long slot, int h, int bm, RaggedItem& it) const {
+    int lo = 0, hi = n_seq - 1;
+    while (lo < hi) {  // the last sequence whose base is not behind the slot
+      const int mid = (lo + hi + 1) >> 1;
+      if ((long long)(q_start(mid) / bm) + mid <= slot) lo = mid;
+      else hi = mid - 1;
+    }
+    const int first = q_start(lo), end = q_start(lo + 1);
+    const long long row0 = first + (slot - first / bm - lo) * bm;
+    if (row0 < first || row0 >= end) return false;
+    it.seq = lo;
+    it.h = h;
+    it.g = h / (H / G);
+    it.row0 = (int)row0;
+    it.rows = min(bm, end - (int)row0);
+    const int kb = k_start(lo), nk = max(0, k_start(lo + 1) - kb);
+    const long long behind = (long long)nk - (end - first) + (row0 - first);  // keys before the one of the tile's first row
+    it.key0 = 0;
+    it.last0 = (int)behind;
+    it.key1 = (int)max(0ll, min((long long)nk, behind + it.rows));
+    it.clear = (int)max(0ll, min((long long)nk, behind + 1));
+    it.split = 0;
+    it.kbase = kb;
+    return true;
+  }
+  __device__ bool sees(const RaggedItem& it, int r, int j) const { return j < it.key1 && j <= it.last0 + r; }
+  template <typename T>
+  __device__ const T* q_row(const RaggedItem& it, int r) const {
+    return static_cast<const T*>(q) + (long long)(it.row0 + r) * q_rs + (long long)it.h * q_hs;
+  }
+  template <typename T>
+  __device__ const T* k_row(const RaggedItem& it, int j) const {
+    return static_cast<const T*>(k) + (it.kbase + j) * k_rs + (long long)it.g * k_hs;
+  }
+  template <typename T>
+  __device__ const T* v_row(const RaggedItem& it, int j) const {
+    return static_cast<const T*>(v) + (it.kbase + j) * v_rs + (long long)it.g * v_hs;
+  }
+  // The first CTA looks at all starts.
+  __device__ void check(int block, int thread, int threads) const {
+    if (block != 0 || status == nullptr) return;
+    bool bad = false;
+    for (int s = thread; s <= n_seq; s += threads) {
+      const int a = q_starts[s], b = k_starts[s];
+      bad |= a < 0 || a > n_rows || b < 0 || b > n_keys;
+      if (s > 0) bad |= a < q_starts[s - 1] || b < k_starts[s - 1];
+    }
+    if (bad) atomicOr(status, 1);
+  }
+};
+
+// ---- trees of drafted tokens ------------------------------------------------------------------------------------
+// Node t < n_nodes[s] of sequence s sits in cache slot ctx[s] + t and sees slots [0, ctx[s]) and those nodes j of its own sequence
+// whose bit is set: word j / 64, bit j % 64 of ancestors[s][t].  The rows of one key/value head are its T * (H / G) pairs of node and
+// query head, node-major, so that K and V are read once for all of them.
+struct TreeProblem {
+  const void* q;
+  long long q_rs;
+  KvView kv;
+  const int* ctx;
+  const int* n_nodes;                  // NULL: T everywhere
+  const unsigned long long* ancestors; // [B][T][words]
+  int words;
+  void* o;
+  long long o_rs;
+  float* part_o;    // [n_splits][B * T * H][D] and their sums' logarithms (base 2) [n_splits][B * T * H]; n_splits == 1: unused
+  float* part_lse;
+  int n_splits, B, T, H, G, D, group, rows_per_tile, tiles;  // group = H / G
+  float scale_log2;
+  int* status;
+
+  __host__ __device__ long long items() const { return (long long)B * G * tiles * n_splits; }
+  // Keys [0, keys) of a sequence, of which the last `nodes` are drafts.  What does not fit the layout is left out.
+  __device__ void lengths(int s, int& context, int& nodes) const {
+    const long long room = (long long)(kv.page_table ? kv.max_pages : 1) * kv.page_tokens;
+    context = (int)min((long long)max(ctx[s], 0), room);
+    nodes = n_nodes ? min(max(n_nodes[s], 0), T) : T;
+    nodes = (int)min((long long)nodes, room - context);
+  }
+  // Splits share the key tiles of `bn` keys evenly; the ones behind may get none.
+  __device__ bool item(long long i, int bn, RaggedItem& it) const {
+    it.split = (int)(i % n_splits);
+    i /= n_splits;
+    const int tile = (int)(i % tiles);
+    i /= tiles;
+    it.g = (int)(i % G);
+    it.seq = (int)(i / G);
+    it.h = it.g * group;
+    int context, nodes;
+    lengths(it.seq, context, nodes);
+    const int n = n_nodes ? min(max(n_nodes[it.seq], 0), T) : T;
+    it.row0 = tile * rows_per_tile;
+    it.rows = min(rows_per_tile, n * group - it.row0);
+    if (it.rows <= 0) return false;
+    const int keys = context + nodes, n_tiles = (keys + bn - 1) / bn;
+    const int per = n_tiles / n_splits, more = n_tiles - per * n_splits;  // the first `more` splits take one tile more
+    const int t0 = it.split * per + min(it.split, more), t1 = t0 + per + (it.split < more ? 1 : 0);
+    it.key0 = min(keys, t0 * bn);
+    it.key1 = min(keys, t1 * bn);
+    it.clear = context;
+    it.last0 = 0;
+    it.kbase = 0;
+    return true;
+  }
+  __device__ const unsigned long long* mask_row(const RaggedItem& it, int r) const {
+    return ancestors + ((long long)it.seq * T + (it.row0 + r) / group) * words;
+  }
+  __device__ bool sees(const RaggedItem& it, int r, int j) const {
+    if (j < it.clear) return true;
+    const int d = j - it.clear;
+    return (mask_row(it, r)[d >> 6] >> (d & 63)) & 1ull;
+  }
+  __device__ long long out_row(const RaggedItem& it, int r) const { return (long long)it.seq * T + (it.row0 + r) / group; }
+  __device__ int head(const RaggedItem& it, int r) const { return it.h + (it.row0 + r) % group; }
+  template <typename E>
+  __device__ const E* q_row(const RaggedItem& it, int r) const {
+    return static_cast<const E*>(q) + out_row(it, r) * q_rs + (long long)head(it, r) * D;
+  }
+  // Offset of key j, or -1 where the page table names no page: its key and value count as zeros, as they do in the tensor-core kernel.
+  __device__ long long key_offset(const RaggedItem& it, int j) const {
+    const int lp = j / kv.page_tokens, in = j - lp * kv.page_tokens;
+    const long long pg = kv.page_table ? (long long)kv.page_table[(long long)it.seq * kv.max_pages + lp] : it.seq;
+    if (pg < 0 || (kv.n_pages > 0 && pg >= kv.n_pages)) return -1;
+    return pg * kv.page_stride + (long long)it.g * kv.head_stride + (long long)in * kv.token_stride;
+  }
+  // The first CTA looks at all lengths.
+  __device__ void check(int block, int thread, int threads) const {
+    if (block != 0 || status == nullptr) return;
+    const long long room = (long long)(kv.page_table ? kv.max_pages : 1) * kv.page_tokens;
+    for (int s = thread; s < B; s += threads) {
+      const int n = n_nodes ? n_nodes[s] : T;
+      if (ctx[s] < 0 || n < 0 || n > T || (long long)ctx[s] + n > room) atomicOr(status, 1);
+    }
+  }
+};
+
+// ragged_simt.cu: any dtype, head_dim 8, 16, 32, 64 or 128
+int packed_simt(const PackedProblem& p, int D, int dtype, cudaStream_t st);
+int tree_simt(const TreeProblem& p, int dtype, cudaStream_t st);
+// n_splits partials of every row into one (ragged_simt.cu)
+int tree_merge(const TreeProblem& p, int dtype, cudaStream_t st);
+
+}  // namespace dgpt

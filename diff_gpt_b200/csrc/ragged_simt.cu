@@ -1,0 +1,296 @@
+// Attention of packed prompts and of trees of drafted tokens on the CUDA cores: fp32, heads of 8 and 16, and layouts whose pages the
+// tensor-core kernel cannot tile.
+//
+// A CTA of 256 threads owns a tile of BM rows and walks through its keys 64 at a time with the running maximum and sum of a softmax.
+// Q, K, V and the probabilities of a step lie in shared memory as fp32; the threads form a 16 x 16 grid over (rows, keys) of the scores
+// and over (rows, columns) of the output, each with BM / 16 rows, so that a number fetched from shared memory feeds several products.
+// fp32 products have no tensor-core form that keeps 24 bits; the floor is the FMA rate.
+#include "ragged.cuh"
+
+namespace dgpt {
+
+constexpr int kRgThreads = 256;
+constexpr int kRgBN = 64;
+
+template <typename T, int D, int BM, class P, bool TREE>
+__global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
+  constexpr int RM = BM / 16;                  // rows per thread
+  constexpr int KC = kRgBN / 16;               // score columns per thread
+  constexpr int CO = D >= 16 ? D / 16 : 1;     // output columns per thread
+  constexpr int VEC = Io<T>::kVec16, VPR = D / VEC;
+  constexpr int PITCH = D + 4, PPITCH = kRgBN + 4;
+  extern __shared__ __align__(16) float sm[];
+  float* Qs = sm;                      // [BM][PITCH]
+  float* Ks = Qs + BM * PITCH;         // [64][PITCH]
+  float* Vs = Ks + kRgBN * PITCH;      // [64][PITCH]
+  float* Ps = Vs + kRgBN * PITCH;      // [BM][PPITCH]
+
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  p.check((int)blockIdx.x, tid, kRgThreads);
+  RaggedItem it;
+  if constexpr (TREE) {
+    if (!p.item((long long)blockIdx.x, kRgBN, it)) return;
+  } else {
+    if (!p.item((long long)blockIdx.x / p.H, (int)(blockIdx.x % p.H), BM, it)) return;
+  }
+  for (int i = tid; i < BM * VPR; i += kRgThreads) {
+    const int r = i / VPR, c = i - r * VPR;
+    float t[VEC];
+    if (r < it.rows) {
+      ld16<T>(p.template q_row<T>(it, r) + c * VEC, t);
+#pragma unroll
+      for (int x = 0; x < VEC; ++x) t[x] *= p.scale_log2;
+    } else {
+#pragma unroll
+      for (int x = 0; x < VEC; ++x) t[x] = 0.f;
+    }
+#pragma unroll
+    for (int x = 0; x < VEC; x += 4) *reinterpret_cast<float4*>(&Qs[r * PITCH + c * VEC + x]) = make_float4(t[x], t[x + 1], t[x + 2], t[x + 3]);
+  }
+  float m[RM], l[RM], acc[RM][CO];
+#pragma unroll
+  for (int i = 0; i < RM; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < CO; ++c) acc[i][c] = 0.f;
+  }
+  for (int j0 = it.key0; j0 < it.key1; j0 += kRgBN) {
+    __syncthreads();  // Q is in place; the last step's K, V and P have been read
+    for (int i = tid; i < kRgBN * VPR; i += kRgThreads) {
+      const int jj = i / VPR, c = i - jj * VPR, j = j0 + jj;
+      float kf[VEC], vf[VEC];
+#pragma unroll
+      for (int x = 0; x < VEC; ++x) kf[x] = vf[x] = 0.f;
+      if (j < it.key1) {
+        if constexpr (TREE) {
+          const long long off = p.key_offset(it, j);
+          if (off >= 0) {
+            ld16<T>(static_cast<const T*>(p.kv.k) + off + c * VEC, kf);
+            ld16<T>(static_cast<const T*>(p.kv.v) + off + c * VEC, vf);
+          }
+        } else {
+          ld16<T>(p.template k_row<T>(it, j) + c * VEC, kf);
+          ld16<T>(p.template v_row<T>(it, j) + c * VEC, vf);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < VEC; x += 4) {
+        *reinterpret_cast<float4*>(&Ks[jj * PITCH + c * VEC + x]) = make_float4(kf[x], kf[x + 1], kf[x + 2], kf[x + 3]);
+        *reinterpret_cast<float4*>(&Vs[jj * PITCH + c * VEC + x]) = make_float4(vf[x], vf[x + 1], vf[x + 2], vf[x + 3]);
+      }
+    }
+    __syncthreads();
+    // scores: rows ty * RM + i, keys tx + 16 j
+    float s[RM][KC];
+#pragma unroll
+    for (int i = 0; i < RM; ++i)
+#pragma unroll
+      for (int j = 0; j < KC; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < D; d += 4) {
+      float4 a[RM], b[KC];
+#pragma unroll
+      for (int i = 0; i < RM; ++i) a[i] = *reinterpret_cast<const float4*>(&Qs[(ty * RM + i) * PITCH + d]);
+#pragma unroll
+      for (int j = 0; j < KC; ++j) b[j] = *reinterpret_cast<const float4*>(&Ks[(tx + 16 * j) * PITCH + d]);
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int j = 0; j < KC; ++j) s[i][j] = fmaf(a[i].w, b[j].w, fmaf(a[i].z, b[j].z, fmaf(a[i].y, b[j].y, fmaf(a[i].x, b[j].x, s[i][j]))));
+    }
+    const bool masked = j0 + kRgBN > it.clear || j0 + kRgBN > it.key1;
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      const int r = ty * RM + i;
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < KC; ++j) {
+          const int key = j0 + tx + 16 * j;
+          if (r >= it.rows || key >= it.key1 || !p.sees(it, r, key)) s[i][j] = -INFINITY;
+        }
+      }
+      float top = s[i][0];
+#pragma unroll
+      for (int j = 1; j < KC; ++j) top = fmaxf(top, s[i][j]);
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float mn = fmaxf(m[i], top), ref = mn == -INFINITY ? 0.f : mn;
+      const float f = exp2f(m[i] - ref);  // m = -inf: 0
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < KC; ++j) {
+        const float e = exp2f(s[i][j] - ref);
+        sum += e;
+        Ps[r * PPITCH + tx + 16 * j] = e;
+      }
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      m[i] = mn;
+      l[i] = l[i] * f + sum;
+#pragma unroll
+      for (int c = 0; c < CO; ++c) acc[i][c] *= f;
+    }
+    __syncthreads();
+    // output: rows ty * RM + i, columns tx * CO + c
+    if (D >= 16 || tx * CO < D) {
+#pragma unroll 4
+      for (int j = 0; j < kRgBN; j += 4) {
+        float4 a[RM];
+#pragma unroll
+        for (int i = 0; i < RM; ++i) a[i] = *reinterpret_cast<const float4*>(&Ps[(ty * RM + i) * PPITCH + j]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float b[CO];
+#pragma unroll
+          for (int c = 0; c < CO; ++c) b[c] = Vs[(j + x) * PITCH + tx * CO + c];
+#pragma unroll
+          for (int i = 0; i < RM; ++i) {
+            const float w = x == 0 ? a[i].x : x == 1 ? a[i].y : x == 2 ? a[i].z : a[i].w;
+#pragma unroll
+            for (int c = 0; c < CO; ++c) acc[i][c] = fmaf(w, b[c], acc[i][c]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RM; ++i) {
+    const int r = ty * RM + i;
+    if (r >= it.rows) continue;
+    // !(l <= 0): a row with a key that is not a number keeps saying so
+    const bool any = !(l[i] <= 0.f);
+    const float inv = any ? 1.f / l[i] : 0.f;
+    if constexpr (TREE) {
+      const long long row = p.out_row(it, r);
+      const int h = p.head(it, r);
+      if (p.n_splits > 1) {
+        const long long at = ((long long)it.split * p.B * p.T + row) * p.H + h;
+        if (D >= 16 || tx * CO < D) {
+#pragma unroll
+          for (int c = 0; c < CO; ++c) p.part_o[at * D + tx * CO + c] = any ? acc[i][c] * inv : 0.f;
+        }
+        if (tx == 0) p.part_lse[at] = any ? m[i] + log2f(l[i]) : -INFINITY;
+        continue;
+      }
+      if (D >= 16 || tx * CO < D) {
+        T* o = static_cast<T*>(p.o) + row * p.o_rs + (long long)h * D + tx * CO;
+#pragma unroll
+        for (int c = 0; c < CO; ++c) Io<T>::st(o + c, any ? acc[i][c] * inv : 0.f);
+      }
+    } else {
+      if (D >= 16 || tx * CO < D) {
+        T* o = static_cast<T*>(p.o) + (long long)(it.row0 + r) * p.o_rs + (long long)it.h * p.o_hs + tx * CO;
+#pragma unroll
+        for (int c = 0; c < CO; ++c) Io<T>::st(o + c, any ? acc[i][c] * inv : 0.f);
+      }
+      if (tx == 0 && p.lse) p.lse[(long long)(it.row0 + r) * p.H + it.h] = any ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
+    }
+  }
+}
+
+template <typename T, int D, int BM, class P, bool TREE>
+static int ragged_simt_go(const P& p, long long ctas, cudaStream_t st) {
+  constexpr size_t smem = ((size_t)(BM + 2 * kRgBN) * (D + 4) + (size_t)BM * (kRgBN + 4)) * sizeof(float);
+  auto kernel = ragged_simt_kernel<T, D, BM, P, TREE>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) {
+    set_error("ragged attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    return DGPT_E_CUDA;
+  }
+  kernel<<<(unsigned)ctas, kRgThreads, smem, st>>>(p);
+  return launch_status("ragged attention");
+}
+
+#define DGPT_BY_TYPE(GO)                                        \
+  do {                                                          \
+    if (dtype == DGPT_F32) {                                    \
+      switch (D) {                                              \
+        case 8: GO(float, 8);                                   \
+        case 16: GO(float, 16);                                 \
+        case 32: GO(float, 32);                                 \
+        case 64: GO(float, 64);                                 \
+        case 128: GO(float, 128);                               \
+      }                                                         \
+    } else if (dtype == DGPT_BF16) {                            \
+      switch (D) {                                              \
+        case 8: GO(__nv_bfloat16, 8);                           \
+        case 16: GO(__nv_bfloat16, 16);                         \
+        case 32: GO(__nv_bfloat16, 32);                         \
+        case 64: GO(__nv_bfloat16, 64);                         \
+        case 128: GO(__nv_bfloat16, 128);                       \
+      }                                                         \
+    }                                                           \
+    set_error("ragged attention: dtype %d with head_dim %d is not built", dtype, D); \
+    return DGPT_E_UNSUPPORTED;                                  \
+  } while (0)
+
+int packed_simt(const PackedProblem& p, int D, int dtype, cudaStream_t st) {
+  const long long ctas = p.slots(64) * p.H;
+  DGPT_REQUIRE(ctas <= 0x7fffffffll, "fmha_packed: too many rows");
+#define DGPT_GO(T, DD) return ragged_simt_go<T, DD, 64, PackedProblem, false>(p, ctas, st)
+  DGPT_BY_TYPE(DGPT_GO);
+#undef DGPT_GO
+}
+
+int tree_simt(const TreeProblem& full, int dtype, cudaStream_t st) {
+  TreeProblem p = full;
+  const int D = p.D, rows = p.T * p.group, bm = rows <= 16 ? 16 : 64;
+  p.rows_per_tile = bm;
+  p.tiles = (rows + bm - 1) / bm;
+  const long long ctas = p.items();
+  DGPT_REQUIRE(ctas <= 0x7fffffffll, "tree_attn: too many rows");
+#define DGPT_GO(T, DD)                                                                   \
+  return bm == 16 ? ragged_simt_go<T, DD, 16, TreeProblem, true>(p, ctas, st)           \
+                  : ragged_simt_go<T, DD, 64, TreeProblem, true>(p, ctas, st)
+  DGPT_BY_TYPE(DGPT_GO);
+#undef DGPT_GO
+}
+
+// ---- partials of a tree's rows into one -------------------------------------------------------------------------
+// One warp per (row, head): y = sum_s 2^(lse_s - m) o_s / sum_s 2^(lse_s - m).
+template <typename T>
+__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeProblem p) {
+  dep_wait();
+  const long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), n = (long long)p.B * p.T * p.H;
+  if (at >= n) return;
+  const int lane = threadIdx.x & 31, h = (int)(at % p.H);
+  const long long row = at / p.H;
+  const int s = (int)(row / p.T), t = (int)(row - (long long)s * p.T);
+  if (p.n_nodes && t >= p.n_nodes[s]) return;
+  float m = -INFINITY;
+  for (int i = lane; i < p.n_splits; i += 32) m = fmaxf(m, p.part_lse[i * n + at]);
+  m = warp_max(m);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f;  // columns lane * 4 .. (D <= 128)
+  const bool mine = lane * 4 < p.D;
+  for (int i = 0; i < p.n_splits; ++i) {
+    const float lse = p.part_lse[i * n + at];
+    if (lse == -INFINITY) continue;  // no key of this share is seen
+    const float w = exp2f(lse - ref);
+    total += w;
+    if (mine) {
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (i * n + at) * p.D + lane * 4);
+      acc[0] = fmaf(w, v.x, acc[0]);
+      acc[1] = fmaf(w, v.y, acc[1]);
+      acc[2] = fmaf(w, v.z, acc[2]);
+      acc[3] = fmaf(w, v.w, acc[3]);
+    }
+  }
+  if (!mine) return;
+  const bool any = !(total <= 0.f);
+  const float inv = any ? 1.f / total : 0.f;
+  T* o = static_cast<T*>(p.o) + row * p.o_rs + (long long)h * p.D + lane * 4;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) Io<T>::st(o + c, any ? acc[c] * inv : 0.f);
+}
+
+int tree_merge(const TreeProblem& p, int dtype, cudaStream_t st) {
+  const long long rows = (long long)p.B * p.T * p.H;
+  const dim3 grid((unsigned)((rows + 7) / 8));
+  if (dtype == DGPT_F32) launch_few(true, tree_merge_kernel<float>, grid, dim3(256), 0, st, p);
+  else launch_few(true, tree_merge_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p);
+  return launch_status("tree_attn");
+}
+
+}  // namespace dgpt

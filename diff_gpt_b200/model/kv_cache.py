@@ -176,6 +176,13 @@ class PagedKVCache:
         """Sequence index = row (append and per-trajectory attention)."""
         return self._layout(layer, self.row_table)
 
+    def keep_drafts(self, src_start: torch.Tensor, dst_start: torch.Tensor, path: torch.Tensor, count: torch.Tensor,
+                    status: torch.Tensor | None = None) -> None:
+        """What drafts path[r, :count[r]] of every row hold in slots from src_start[r] on moves to the slots from dst_start[r] on, in all
+        layers.  Slots are a row's own (those of its table); the shared prompt's are not written."""
+        ops.kv_keep(self.row_layout(0), src_start, dst_start, path, count, n_layer=self.n_layer, layer_stride=self.pool.stride(0),
+                    H=self.n_head, D=self.head_dim, dtype=self.pool.dtype, status=status)
+
 
 @dataclass(frozen=True)
 class StateSpec:

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -1122,5 +1123,212 @@ def streams_final(
         lib.dgpt_streams_final(
             x.data_ptr(), stride, y.data_ptr(), mix.data_ptr(), out.data_ptr(), out.numel(), w.data_ptr(), eps, _ptr(rows),
             h.data_ptr(), h.shape[0], n, Cdim, dtype_code(y), _stream(),
+        )
+    )
+
+
+# ---- serving with drafted tokens ----------------------------------------------------------------
+def _here(*ts: torch.Tensor | None) -> None:
+    """The calls below run on the current device's stream, so that is where their tensors have to be."""
+    _cuda(*ts)
+    at = torch._C._cuda_getDevice()
+    for t in ts:
+        if t is not None and t.device.index != at:
+            raise RuntimeError(f"tensors must be on the current device (cuda:{at}), got one on {t.device}")
+
+
+def _i32(name: str, t: torch.Tensor | None, *shape: int) -> None:
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _stride(t: torch.Tensor, dim: int, least: int) -> int:
+    """The stride of a dimension; of one with a single entry, any that the kernels take."""
+    return t.stride(dim) if t.shape[dim] > 1 else least
+
+
+def fmha_packed(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    seq_starts: torch.Tensor,
+    o: torch.Tensor,
+    *,
+    key_starts: torch.Tensor | None = None,
+    scale: float | None = None,
+    lse: torch.Tensor | None = None,
+    impl: int = 0,
+    status: torch.Tensor | None = None,
+) -> None:
+    """Causal attention over prompts of different lengths that lie one behind another (see `dgpt_fmha_packed`).
+
+    q, o: [rows, H, D]; k, v: [key rows, G, D], H a multiple of G (views with unit inner stride, other strides multiples of 8).
+    seq_starts: int32 [S + 1], prompt s is rows seq_starts[s] .. seq_starts[s + 1] - 1; key_starts: the same for its keys, of which
+    its last query sees all (None: the query rows').  lse: fp32 [rows, H] or None.  Rows of no prompt are left as they are.
+    """
+    _here(q, k, v, seq_starts, o, key_starts, lse, status)
+    if q.dim() != 3 or k.dim() != 3 or q.shape != o.shape or k.shape != v.shape or q.shape[2] != k.shape[2]:
+        raise ValueError(f"fmha_packed: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, o {tuple(o.shape)} do not fit")
+    if not q.dtype == k.dtype == v.dtype == o.dtype:
+        raise TypeError("fmha_packed: q, k, v and o must have one dtype")
+    if any(t.shape[2] > 1 and t.stride(2) != 1 for t in (q, k, v, o)):
+        raise ValueError("fmha_packed: the elements of a head must lie side by side")
+    (N, H, D), (M, G, _) = q.shape, k.shape
+    if seq_starts.dim() != 1 or seq_starts.numel() < 1:
+        raise ValueError("fmha_packed: seq_starts must hold one number more than there are prompts")
+    S = seq_starts.numel() - 1
+    _i32("seq_starts", seq_starts, S + 1)
+    _i32("key_starts", key_starts, S + 1)
+    _i32("status", status, 1)
+    if key_starts is None and M != N:
+        raise ValueError(f"fmha_packed: {M} key rows for {N} queries need key_starts")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (N, H) or not lse.is_contiguous()):
+        raise ValueError(f"fmha_packed: lse must be a contiguous float32 tensor of shape {(N, H)}")
+
+    def at(t: torch.Tensor, heads: int) -> tuple[int, int, int]:
+        return t.data_ptr(), _stride(t, 0, heads * D), _stride(t, 1, D)
+
+    check(
+        lib.dgpt_fmha_packed(
+            *at(q, H), *at(k, G), *at(v, G), *at(o, H), _ptr(lse), seq_starts.data_ptr(), _ptr(key_starts), S, N, M, H, G, D,
+            attn_scale(D) if scale is None else scale, dtype_code(q), impl, _ptr(status), _stream(),
+        )
+    )
+
+
+def tree_attn_splits(B: int, T: int, H: int, G: int, D: int, max_keys: int, dtype: torch.dtype) -> int:
+    """Shares of the keys that `tree_attn` would choose for sequences of about `max_keys` keys."""
+    return int(lib.dgpt_tree_attn_splits(B, T, H, G, D, max_keys, _DT[dtype]))
+
+
+def tree_attn_workspace_bytes(B: int, T: int, H: int, D: int, n_splits: int) -> int:
+    return int(lib.dgpt_tree_attn_workspace_bytes(B, T, H, D, n_splits))
+
+
+def tree_attn(
+    q: torch.Tensor,
+    kv: KvLayout,
+    ctx_len: torch.Tensor,
+    ancestors: torch.Tensor,
+    out: torch.Tensor,
+    *,
+    H: int,
+    G: int,
+    D: int,
+    max_keys: int = 0,
+    n_nodes: torch.Tensor | None = None,
+    token_stride: int = 0,
+    scale: float | None = None,
+    n_splits: int = 0,
+    workspace: torch.Tensor | None = None,
+    impl: int = 0,
+    status: torch.Tensor | None = None,
+) -> None:
+    """Attention of a tree of drafted tokens over a cache that already holds their keys and values (see `dgpt_tree_attn`).
+
+    q, out: [B * T, H * D], draft t of sequence s in row s * T + t; ctx_len: int32 [B], cached tokens before the drafts, which lie in the
+    slots behind them; ancestors: int64 [B, T, W] (or [B, T] for W = 1), bit j % 64 of word j / 64 says that the draft sees draft j;
+    n_nodes: int32 [B], drafts of each sequence (None: T; the rows behind are left as they are).  token_stride: elements between a
+    head's consecutive tokens (0: D).  n_splits 0: chosen for about `max_keys` keys a sequence (0: what the layout holds).  workspace: at
+    least `tree_attn_workspace_bytes` (None: allocated here).
+    """
+    _here(q, ctx_len, ancestors, out, n_nodes, workspace, status)
+    if ancestors.dim() == 2:
+        ancestors = ancestors.unsqueeze(2)
+    if ancestors.dim() != 3 or ancestors.dtype != torch.int64 or not ancestors.is_contiguous():
+        raise ValueError("tree_attn: ancestors must be a contiguous int64 tensor [B, T, W]")
+    B, T, words = ancestors.shape
+    if tuple(q.shape) != (B * T, H * D) or q.shape != out.shape or q.dtype != out.dtype:
+        raise ValueError(f"tree_attn: q {tuple(q.shape)} and out {tuple(out.shape)} must be {(B * T, H * D)} of one dtype")
+    if B * T > 0 and H * D > 1 and (q.stride(1) != 1 or out.stride(1) != 1):
+        raise ValueError("tree_attn: the elements of a row must lie side by side")
+    _i32("ctx_len", ctx_len, B)
+    _i32("n_nodes", n_nodes, B)
+    _i32("status", status, 1)
+    if n_splits == 0:
+        held = (kv.max_pages if kv.page_table else 1) * kv.page_tokens
+        n_splits = tree_attn_splits(B, T, H, G, D, min(max_keys, held) if max_keys > 0 else held, q.dtype) if q.dtype in _DT else 1
+    need = tree_attn_workspace_bytes(B, T, H, D, n_splits)
+    if workspace is None and need > 0:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace is not None and not workspace.is_contiguous():
+        raise ValueError("tree_attn: the workspace must be contiguous")
+    check(
+        lib.dgpt_tree_attn(
+            q.data_ptr(), _stride(q, 0, H * D), C.byref(kv), token_stride or D, ctx_len.data_ptr(), _ptr(n_nodes), ancestors.data_ptr(), words,
+            out.data_ptr(), _stride(out, 0, H * D), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+            n_splits, B, T, H, G, D, attn_scale(D) if scale is None else scale, dtype_code(q), impl, _ptr(status), _stream(),
+        )
+    )
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor  # fp32 [R]
+    entropy: torch.Tensor  # fp32 [R]
+    top_ids: torch.Tensor  # int32 [R, top_k]
+    top_logprobs: torch.Tensor  # fp32 [R, top_k]
+
+
+def token_logprobs(
+    logits: torch.Tensor,
+    targets: torch.Tensor,
+    *,
+    top_k: int = 0,
+    temperature: float = 1.0,
+    status: torch.Tensor | None = None,
+) -> TokenLogprobs:
+    """log softmax(logits / temperature)[r, targets[r]] per row, the entropy of the row's distribution, and its `top_k` (up to 32) most
+    probable tokens in descending order, equal ones by index.  logits: [R, V] (last dim contiguous), targets: int32 [R].
+    (See `dgpt_token_logprobs`; `token_nll` gives the first of these alone, rounded to the logits' type.)"""
+    _here(logits, targets, status)
+    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("token_logprobs: logits must be [R, V] with the elements of a row side by side")
+    R, V = logits.shape
+    _i32("targets", targets, R)
+    _i32("status", status, 1)
+    new = dict(device=logits.device)
+    r = TokenLogprobs(torch.empty(R, **new), torch.empty(R, **new), torch.empty((R, max(top_k, 0)), dtype=torch.int32, **new),
+                      torch.empty((R, max(top_k, 0)), **new))
+    check(
+        lib.dgpt_token_logprobs(
+            logits.data_ptr(), _stride(logits, 0, V), targets.data_ptr(), temperature, r.logprob.data_ptr(), r.entropy.data_ptr(),
+            r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), top_k, R, V, dtype_code(logits), _ptr(status), _stream(),
+        )
+    )
+    return r
+
+
+def kv_keep(
+    kv: KvLayout,
+    src_start: torch.Tensor,
+    dst_start: torch.Tensor,
+    path: torch.Tensor,
+    count: torch.Tensor,
+    *,
+    n_layer: int,
+    layer_stride: int,
+    H: int,
+    D: int,
+    dtype: torch.dtype,
+    token_stride: int = 0,
+    status: torch.Tensor | None = None,
+) -> None:
+    """Rows of accepted drafts move within a cache, in every layer (see `dgpt_kv_keep`): slot dst_start[s] + i takes what slot
+    src_start[s] + path[s, i] held before the call, i < count[s].  kv: layer 0's storage; path: int32 [B, T], T up to 256; src_start, dst_start,
+    count: int32 [B]; layer_stride, token_stride (0: D): elements."""
+    _here(src_start, dst_start, path, count, status)
+    if path.dim() != 2:
+        raise ValueError("kv_keep: path must be [B, T]")
+    B, T = path.shape
+    _i32("path", path, B, T)
+    for name, t in (("src_start", src_start), ("dst_start", dst_start), ("count", count)):
+        _i32(name, t, B)
+    _i32("status", status, 1)
+    if dtype not in _DT:
+        raise TypeError(f"unsupported dtype {dtype}: float32 and bfloat16 are built")
+    check(
+        lib.dgpt_kv_keep(
+            C.byref(kv), token_stride or D, src_start.data_ptr(), dst_start.data_ptr(), path.data_ptr(), count.data_ptr(), n_layer,
+            layer_stride, B, T, H, D, _DT[dtype], _ptr(status), _stream(),
         )
     )

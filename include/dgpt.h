@@ -588,6 +588,68 @@ int dgpt_retention(const void* in, int64_t in_row_stride, int32_t q_col, int32_t
                    void* y, int64_t y_row_stride, float* workspace, size_t workspace_bytes, int32_t n_seq, int32_t T, int32_t H,
                    int32_t dim, int32_t vdim, int32_t dtype, int32_t impl, int32_t* status, void* stream);
 
+/* ---- serving with drafted tokens: packed prompts, trees of drafts, probabilities of given tokens, accepted rows -----
+ * (No counterpart in the reference project, whose prompts come one length at a time and whose tokens one by one.) */
+
+/* Causal attention over prompts of different lengths that lie one behind another, grouped-query heads:
+ *   o[i,h,:] = sum_j p_j v[j,g,:],  p = softmax_j(q[i,h,:] . k[j,g,:] * scale),  g = h / (H / G)
+ * Sequence s has query rows seq_starts[s] .. seq_starts[s + 1] - 1 and key rows key_starts[s] .. key_starts[s + 1] - 1 (key_starts
+ * NULL: the query rows').  Its last query sees all of its keys, each query before it one key less; a query that sees none gets
+ * zeros.  Rows that belong to no sequence are neither read nor written, and no sequence's numbers reach another's output; within
+ * a sequence every key and value is a finite number.
+ * q, o: element (i,h,d) at i*row_stride + h*head_stride + d; k, v likewise over G heads; pointers 16-byte aligned, strides multiples
+ * of 8 elements.  lse: fp32 [n_rows, H], the scores' log-sum-exp (-inf where no key is seen), or NULL.
+ * seq_starts, key_starts: device int32 [n_seq + 1], not decreasing, within 0 .. n_rows (n_keys); status bit 0 is set where
+ * they are not (rows are then wrong, but nothing outside the tensors is touched).
+ * D: 8, 16, 32, 64, 128.  impl: 0 = choose, 1 = CUDA cores, 2 = tcgen05 (bf16, D = 32, 64, 128) or fail.
+ * status: device int32 or NULL; set to another value than 1 if a bounded wait ran out. */
+int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k, int64_t k_row_stride,
+                     int64_t k_head_stride, const void* v, int64_t v_row_stride, int64_t v_head_stride, void* o,
+                     int64_t o_row_stride, int64_t o_head_stride, float* lse, const int32_t* seq_starts,
+                     const int32_t* key_starts, int32_t n_seq, int32_t n_rows, int32_t n_keys, int32_t H, int32_t G, int32_t D,
+                     float scale, int32_t dtype, int32_t impl, int32_t* status, void* stream);
+
+/* Attention of a tree of drafted tokens over a cache.  Sequence s has ctx_len[s] cached tokens in slots 0 .. ctx_len[s] - 1 and
+ * n_nodes[s] drafts (NULL: T) in the slots behind them.  Draft t sees every cached token, and draft j of its own sequence where
+ * bit j % 64 of ancestors[s][t][j / 64] is set (its ancestors' and its own, for a tree; any mask is allowed).  Bits of drafts from n_nodes[s] on count
+ * for nothing.  A draft that sees nothing gets zeros; rows from n_nodes[s] on are left as they are.
+ * q, out: device [B * T, H * D], row s * T + t, with row strides that are multiples of 8; kv: keys and values of G heads, query head h
+ * reads h / (H / G), consecutive tokens of a head kv_token_stride elements apart; slots behind a sequence's last draft may
+ * hold anything, those before it finite numbers; a page number outside the pool stands for zeros.
+ * ancestors: device [B][T][words] with 64 * words >= T; T <= 256.  ctx_len, n_nodes: device int32 [B]; status bit 0 is set
+ * where they do not fit T or the layout (what does not fit is left out).
+ * n_splits (1 to 256) splits each sequence's keys; workspace from the _bytes call (not needed for 1), 16-byte aligned.  _splits chooses a
+ * number for sequences of about max_keys keys; any number gives the same rows but for the order of their sums.
+ * D, impl, status as in dgpt_fmha_packed. */
+int32_t dgpt_tree_attn_splits(int32_t B, int32_t T, int32_t H, int32_t G, int32_t D, int32_t max_keys, int32_t dtype);
+size_t dgpt_tree_attn_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t D, int32_t n_splits);
+int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv_layout* kv, int64_t kv_token_stride,
+                   const int32_t* ctx_len, const int32_t* n_nodes, const uint64_t* ancestors, int32_t words, void* out,
+                   int64_t out_row_stride, void* workspace, size_t workspace_bytes, int32_t n_splits, int32_t B, int32_t T, int32_t H,
+                   int32_t G, int32_t D, float scale, int32_t dtype, int32_t impl, int32_t* status, void* stream);
+
+/* Log probability of one given token per row under p = softmax(logits / temperature), the entropy of p (natural logarithms), and the
+ * top_k (0 to 32) most probable tokens with their log probabilities, in descending order of the logits, equal ones by index:
+ *   logprob[r] = log p[r][targets[r]],  entropy[r] = - sum_j p_j log p_j,  top_ids [R, top_k],  top_logprobs [R, top_k]
+ * A logit of -inf is a token that cannot come (probability 0, log probability -inf).  A row that holds a NaN or +inf, or nothing but -inf, has no
+ * distribution: its numbers are NaN (its top ids are those of its largest logits, NaN behind all others).
+ * logits: device [R, V] with row stride, rows on any boundary of their type; targets: device
+ * int32 [R]; outputs: fp32 and int32.  A target outside [0, V) gives NaN for its logprob and sets bit 2 of *status (status may be NULL). */
+int dgpt_token_logprobs(const void* logits, int64_t logits_row_stride, const int32_t* targets, float temperature, float* logprob,
+                        float* entropy, int32_t* top_ids, float* top_logprobs, int32_t top_k, int32_t R, int32_t V, int32_t dtype,
+                        int32_t* status, void* stream);
+
+/* Rows of accepted drafts move within a cache, in every layer, head, and for keys and values alike:
+ *   slot dst_start[s] + i  <-  slot src_start[s] + path[s][i],   i < count[s]
+ * All rows of a sequence are read before the first is written, so source and target may overlap; sequences must not write
+ * slots that others read or write.  kv: layer 0's storage (layer l's lies l * layer_stride elements behind it, through the same page
+ * table); consecutive tokens of a head kv_token_stride elements apart; k_base == v_base: one storage, moved once.
+ * path: device int32 [B, T], T <= 256; src_start, dst_start, count: device int32 [B].  A head's row is a multiple of 16 bytes.  A row whose
+ * slots do not exist, or lie in a page outside the pool, is not moved and sets bit 0 of *status, as does a count outside 0 .. T. */
+int dgpt_kv_keep(const dgpt_kv_layout* kv, int64_t kv_token_stride, const int32_t* src_start, const int32_t* dst_start,
+                 const int32_t* path, const int32_t* count, int32_t n_layer, int64_t layer_stride, int32_t B, int32_t T, int32_t H,
+                 int32_t D, int32_t dtype, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
