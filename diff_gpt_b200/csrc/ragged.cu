@@ -40,6 +40,8 @@ extern "C" int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_h
   p.n_seq = n_seq; p.n_rows = n_rows; p.n_keys = n_keys; p.H = H; p.G = G;
   p.scale_log2 = scale * kLog2e;
   p.status = status;
+  const bool tensor = packed_tc_supported(p, D, dtype);
+  if (tensor && impl != 1) return packed_tc(p, D, static_cast<cudaStream_t>(stream));
   if (impl == 2) {
     set_error("fmha_packed: the tensor-core kernel does not cover dtype %d, head_dim %d", dtype, D);
     return DGPT_E_UNSUPPORTED;
@@ -115,11 +117,12 @@ extern "C" int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv
   p.scale_log2 = scale * kLog2e;
   p.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (impl == 2) {
+  const bool tensor = tree_tc_supported(p, dtype);
+  if (impl == 2 && !tensor) {
     set_error("tree_attn: the tensor-core kernel does not cover dtype %d, head_dim %d with this layout", dtype, D);
     return DGPT_E_UNSUPPORTED;
   }
-  const int rc = tree_simt(p, dtype, st);
+  const int rc = tensor && impl != 1 ? tree_tc(p, st) : tree_simt(p, dtype, st);
   if (rc != DGPT_OK || n_splits == 1) return rc;
   return tree_merge(p, dtype, st);
 }

@@ -184,6 +184,11 @@ struct TreeProblem {
 // ragged_simt.cu: any dtype, head_dim 8, 16, 32, 64 or 128
 int packed_simt(const PackedProblem& p, int D, int dtype, cudaStream_t st);
 int tree_simt(const TreeProblem& p, int dtype, cudaStream_t st);
+// ragged_tc.cu: bf16, head_dim 32, 64 or 128
+bool packed_tc_supported(const PackedProblem& p, int D, int dtype);
+int packed_tc(const PackedProblem& p, int D, cudaStream_t st);
+bool tree_tc_supported(const TreeProblem& p, int dtype);
+int tree_tc(const TreeProblem& p, cudaStream_t st);
 // n_splits partials of every row into one (ragged_simt.cu)
 int tree_merge(const TreeProblem& p, int dtype, cudaStream_t st);
 

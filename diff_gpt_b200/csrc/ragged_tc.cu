@@ -1,0 +1,641 @@
+// Attention of packed prompts and of trees of drafted tokens on the tcgen05 tensor cores (sm_100a, bf16, head_dim 64 or 128; 32 rides on
+// the 64-wide kernel: TMA boxes reach past the tensor and arrive as zeros).
+//
+// A persistent CTA of 512 threads per SM walks through work items: 128 query rows against a run of key tiles of 128.  Lengths lie on the
+// device, so every role works an item's rows and keys out for itself (ragged.cuh).  Sequences are short as often as long, which is why
+// nothing stops between items: score products run two key tiles ahead of the probabilities whatever item they belong to, loads run ahead
+// of those, and a warpgroup of its own takes a finished item's output out of TMEM while the softmax threads are at the next one.
+//   warp 13          loader: TMA loads of Q, and of K and V tiles into rings of 3 and 2 slots (128-byte swizzle, one box per page and 64-wide
+//                    half of the head); page numbers are fetched 32 at a time
+//   warp 12, lane 0  issuer: S_g = Q K_g^T into one of two score buffers, O += P_g V_g with P from TMEM.  P V of tile g goes before S of tile
+//                    g + 2, so that the arrival of those scores also says that P_g has been read
+//   warps 0-7        softmax, two threads per row with 64 of a tile's scores each: probabilities against the running maximum in one sweep that
+//                    finds the tile's own maximum too; the two swap that through shared memory, and only where it exceeds the running one by more than 2^8
+//                    is O rescaled and the tile redone
+//   warps 8-11       output: row sums from shared memory, O from TMEM, one row per thread
+// TMEM columns: S0 [0,128)  S1 [128,256)  P0 [256,320)  P1 [320,384)  O [384, 384 + D).
+// No cluster launch and no multicast.  Every wait is bounded in clock cycles; one that runs out raises the CTA's abort flag, on which the other
+// roles stop too, sets bit 1 of the status word, and the CTA drains its copies, frees its TMEM and returns.
+#include "ragged.cuh"
+#include "tcgen05.cuh"
+
+namespace dgpt {
+namespace tc {
+
+constexpr int kRtThreads = 512;
+constexpr int kRtSoftmaxRegs = 160, kRtOutputRegs = 112, kRtHelperRegs = 80;  // 2 x 160 + 112 + 80 = 4 x 128, the launch's share
+constexpr int kRtStaged = 1024;  // prompts whose starts are kept in shared memory
+
+struct RtItem {
+  RaggedItem it;
+  int tile0, n;  // key tiles tile0 .. tile0 + n - 1
+};
+
+// The items of a CTA, one by one; false at the end.  Items without rows are passed over.
+template <class P, bool TREE>
+struct RtWalk {
+  const P& p;
+  long long i, total;
+  __device__ RtWalk(const P& q) : p(q), i(blockIdx.x) {
+    if constexpr (TREE) total = q.items();
+    else total = q.slots(kBM) * q.H;
+  }
+  __device__ bool next(RtItem& x) {
+    for (; i < total; i += gridDim.x) {
+      bool there;
+      if constexpr (TREE) {
+        there = p.item(i, kBN, x.it);
+      } else {
+        const long long slot = i / p.H;  // from the end: a prompt's last rows see the most keys
+        there = p.item(total / p.H - 1 - slot, (int)(i - slot * p.H), kBM, x.it);
+      }
+      if (!there) continue;
+      x.tile0 = x.it.key0 / kBN;
+      x.n = (x.it.key1 - x.it.key0 + kBN - 1) / kBN;
+      i += gridDim.x;
+      return true;
+    }
+    return false;
+  }
+  __device__ bool next_with_keys(RtItem& x) {
+    while (next(x))
+      if (x.n > 0) return true;
+    return false;
+  }
+};
+
+template <int D, class P, bool TREE>
+__global__ void __launch_bounds__(kRtThreads, 1)
+ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                 const P given, const int d_head) {
+  constexpr int kSub = D / 64;
+  constexpr uint32_t kSubBytes = kBN * 128;
+  constexpr uint32_t kTileBytes = kSub * kSubBytes;
+  constexpr uint32_t kIdescS = instr_desc(kBN, false);
+  constexpr uint32_t kIdescPV = instr_desc(D, true);
+  constexpr uint32_t kPCol = 256, kOCol = 384;
+  constexpr uint32_t kTmem = 512;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sV = smem + 4 * kTileBytes;  // Q | K0 K1 K2 | V0 V1 | barriers | hand-over words | row sums | starts
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * kTileBytes);
+  constexpr int iQ = 0, iQF = 1, iK = 2, iKF = 5, iV = 8, iS = 10, iP = 12, iO = 14, iOF = 16, iL = 17, iLF = 19, nBars = 21;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + nBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile unsigned long long* xch = reinterpret_cast<volatile unsigned long long*>(bars + 32);  // [2 turns][2 halves][128 rows]
+  float* sums = reinterpret_cast<float*>(bars + 32 + 4 * kBM);                                   // [2 items][l of half 0 | of half 1 | m][128 rows]
+  int* staged = reinterpret_cast<int*>(sums + 2 * 3 * kBM);                                      // packed: query starts, then key starts
+  const uint32_t aQ = smem_u32(smem), aK = aQ + kTileBytes, aV = aQ + 4 * kTileBytes, bar0 = smem_u32(bars);
+  auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  P p = given;
+  if constexpr (!TREE) {
+    if (given.n_seq < kRtStaged) {
+      for (int s = tid; s <= given.n_seq; s += kRtThreads) {
+        staged[s] = given.q_starts[s];
+        staged[kRtStaged + s] = given.k_starts[s];
+      }
+      p.q_starts = staged;
+      p.k_starts = staged + kRtStaged;
+    }
+  }
+  if (tid == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < nBars; ++i)
+      mbar_init(bar(i), (i == iP || i == iP + 1 || i == iL || i == iL + 1) ? 2 * kBM : (i == iOF || i == iLF || i == iLF + 1) ? kBM : 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  for (int i = tid; i < 4 * kBM; i += kRtThreads) xch[i] = 0ull;  // turn numbers of an earlier CTA must not be taken for this one's
+  if (warp == 0) {
+    tmem_alloc(smem_u32(tmem_slot), kTmem);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  RtWalk<P, TREE> walk(p);
+  RtItem x;
+
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRtHelperRegs));
+    if (warp == 13) {
+      // ================= loader =================
+      if (lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mq)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mk)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mv)) : "memory");
+      }
+      unsigned items = 0u, kn = 0u, vn = 0u;  // loads issued: Q, K tiles, V tiles
+      bool ok = true;
+      auto wait = [&](int b, unsigned parity) { return __all_sync(0xffffffffu, wait_or_abort(bar(b), parity, abort_flag)) != 0; };
+      int page0 = 0, page_seq = -1, page_id = 0;  // tree: this lane's page number is that of page page0 + lane of sequence page_seq
+      auto load_tile = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, const RtItem& w, int t) {
+        const int t0 = t * kBN;
+        if constexpr (!TREE) {
+          if (lane == 0) {
+            mbar_expect_tx(full, kTileBytes);
+#pragma unroll
+            for (int s = 0; s < kSub; ++s) tma_load_4d(dst + s * kSubBytes, map, full, s * 64, w.it.g, (int)(w.it.kbase + t0), 0);
+          }
+        } else {
+          const int pt = p.kv.page_tokens;
+          const bool dense = p.kv.page_table == nullptr;
+          const int per = dense || pt >= kBN ? 1 : kBN / pt;
+          const int first = dense ? 0 : t0 / pt;
+          const int valid = per == 1 ? 1 : min(per, (w.it.key1 - t0 + pt - 1) / pt);
+          if (!dense && (page_seq != w.it.seq || first < page0 || first + valid > page0 + 32)) {
+            page_seq = w.it.seq;
+            page0 = first;
+            const int at = min(first + lane, p.kv.max_pages - 1);
+            page_id = p.kv.page_table[(long long)w.it.seq * p.kv.max_pages + at];
+          }
+          if (lane == 0) mbar_expect_tx(full, per == 1 ? kTileBytes : (uint32_t)valid * pt * 128u * kSub);
+          for (int q = 0; q < valid; ++q) {
+            const int pg = dense ? w.it.seq : __shfl_sync(0xffffffffu, page_id, first + q - page0);
+            if (lane == 0) {
+#pragma unroll
+              for (int s = 0; s < kSub; ++s)
+                tma_load_4d(dst + s * kSubBytes + q * pt * 128, map, full, s * 64, per == 1 ? t0 - first * pt : 0, w.it.g, pg);
+            }
+          }
+        }
+      };
+      // K runs one tile ahead of V, across items too
+      RtWalk<P, TREE> ahead(p);
+      RtItem y;  // item of the K cursor
+      int kj = 0;
+      bool more = ahead.next_with_keys(y);
+      auto load_k = [&]() {
+        if (kj == 0) {
+          if (items > 0) ok = wait(iQF, (items - 1) & 1u);  // the last S of the item before is done
+          if (!ok) return;
+          if (lane == 0) {
+            if constexpr (TREE) {
+              mbar_expect_tx(bar(iQ), (uint32_t)(p.rows_per_tile * 128 * kSub));
+#pragma unroll
+              for (int s = 0; s < kSub; ++s) tma_load_4d(aQ + s * kSubBytes, &mq, bar(iQ), s * 64, y.it.h, y.it.row0 / p.group, y.it.seq);
+            } else {
+              mbar_expect_tx(bar(iQ), kTileBytes);
+#pragma unroll
+              for (int s = 0; s < kSub; ++s) tma_load_4d(aQ + s * kSubBytes, &mq, bar(iQ), s * 64, y.it.h, y.it.row0, 0);
+            }
+          }
+          ++items;
+        }
+        const unsigned ks = kn % 3u, ku = kn / 3u;
+        if (ku > 0) ok = wait(iKF + (int)ks, (ku - 1) & 1u);
+        if (!ok) return;
+        load_tile(&mk, aK + ks * kTileBytes, bar(iK + (int)ks), y, y.tile0 + kj);
+        ++kn;
+        if (++kj == y.n) {
+          kj = 0;
+          more = ahead.next_with_keys(y);
+        }
+      };
+      if (more) load_k();
+      while (ok && walk.next_with_keys(x)) {
+        for (int j = 0; ok && j < x.n; ++j) {
+          if (more) load_k();
+          if (!ok) break;
+          const unsigned vs = vn & 1u;
+          if (vn >= 2) ok = wait(iO + (int)vs, ((vn - 2) >> 1) & 1u);
+          if (!ok) break;
+          load_tile(&mv, aV + vs * kTileBytes, bar(iV + (int)vs), x, x.tile0 + j);
+          ++vn;
+        }
+      }
+      if (!ok || *abort_flag) {  // something ran out of time: give the copies still in flight a bounded chance to land
+        if (lane == 0 && p.status) atomicOr(p.status, 2);
+        if (items > 0) mbar_wait(bar(iQ), (items - 1) & 1u);
+        for (unsigned i = 0; i < 3u && i < kn; ++i) mbar_wait(bar(iK + (int)((kn - 1 - i) % 3u)), ((kn - 1 - i) / 3u) & 1u);
+        for (unsigned i = 0; i < 2u && i < vn; ++i) mbar_wait(bar(iV + (int)((vn - 1 - i) & 1u)), ((vn - 1 - i) >> 1) & 1u);
+      }
+    } else if (warp == 12) {
+      // ================= MMA issuer (one lane) =================
+      if (lane == 0) {
+        const uint64_t dQK = smem_desc(0, 16, 1024), dV = smem_desc(0, kSubBytes, 1024);
+        RtWalk<P, TREE> ahead(p);
+        RtItem y;  // item of the score cursor
+        int sj = 0;
+        unsigned items = 0u, sg = 0u, g = 0u;
+        bool ok = true, more = ahead.next_with_keys(y);
+        auto issue_s = [&]() {  // S(sg & 1) = Q K(sg % 3)^T
+          if (sj == 0) {
+            ok = wait_or_abort(bar(iQ), items & 1u, abort_flag);
+            ++items;
+          }
+          const unsigned ks = sg % 3u, buf = sg & 1u;
+          ok = ok && wait_or_abort(bar(iK + (int)ks), (sg / 3u) & 1u, abort_flag);
+          if (!ok) return;
+          tc_fence_after();
+          umma_ss_chain<D / 16>(tmem + buf * 128, dQK + (aQ >> 4), dQK + ((aK + ks * kTileBytes) >> 4), kIdescS, kSubBytes >> 4);
+          umma_commit(bar(iS + (int)buf));
+          umma_commit(bar(iKF + (int)ks));
+          ++sg;
+          if (++sj == y.n) {
+            umma_commit(bar(iQF));  // Q may be overwritten
+            sj = 0;
+            more = ahead.next_with_keys(y);
+          }
+        };
+        for (int i = 0; i < 2 && ok && more; ++i) issue_s();
+        unsigned outs = 0u;  // items whose first P V has been issued
+        while (ok && walk.next_with_keys(x)) {
+          for (int j = 0; ok && j < x.n; ++j, ++g) {
+            const unsigned buf = g & 1u, ph = (g >> 1) & 1u;
+            // P_g is complete when every row has arrived; by then every row has also consumed S_g
+            ok = wait_or_abort(bar(iP + (int)buf), ph, abort_flag) && wait_or_abort(bar(iV + (int)buf), ph, abort_flag);
+            if (ok && j == 0) {
+              if (outs > 0) ok = wait_or_abort(bar(iOF), (outs - 1) & 1u, abort_flag);  // O of the item before has been read
+              ++outs;
+            }
+            if (!ok) break;
+            tc_fence_after();
+            umma_ts_chain<kBN / 16>(tmem + kOCol, tmem + kPCol + buf * 64, dV + ((aV + buf * kTileBytes) >> 4), kIdescPV, j > 0 ? 1u : 0u);
+            umma_commit(bar(iO + (int)buf));
+            if (more) issue_s();
+          }
+        }
+        if (!ok) {
+          if (!*abort_flag) *abort_flag = 2;
+          if (p.status) atomicOr(p.status, 2);
+        }
+      }
+    } else if (warp == 14) {
+      p.check((int)blockIdx.x, lane, 32);
+    }
+  } else if (warp >= 8) {
+    // ================= output: one thread per row =================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRtOutputRegs));
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t o_addr = tmem + ((uint32_t)(quarter * 32) << 16) + kOCol;
+    unsigned items = 0u, g = 0u;
+    bool ok = true;
+    while (ok && walk.next(x)) {
+      const bool row_ok = row < x.it.rows;
+      float l = 0.f, m = -INFINITY;
+      uint32_t packed[D / 2];
+      float* part = nullptr;
+      long long at = 0;
+      if constexpr (TREE) {
+        if (p.n_splits > 1) {
+          if (row_ok) at = ((long long)x.it.split * p.B * p.T + p.out_row(x.it, row)) * p.H + p.head(x.it, row);
+          part = p.part_o + at * d_head;
+        }
+      }
+      if (x.n > 0) {
+        const int slot = (int)(items & 1u);
+        ok = __all_sync(0xffffffffu, wait_or_abort(bar(iL + slot), (items >> 1) & 1u, abort_flag)) != 0;
+        if (!ok) break;
+        const float* sum = sums + slot * 3 * kBM;
+        l = sum[row] + sum[kBM + row];
+        m = sum[2 * kBM + row];
+        mbar_arrive(bar(iLF + slot));
+        const unsigned last = g + (unsigned)x.n - 1u;
+        ok = __all_sync(0xffffffffu, wait_or_abort(bar(iO + (int)(last & 1u)), (last >> 1) & 1u, abort_flag)) != 0;
+        if (!ok) break;
+        tc_fence_after();
+        g += (unsigned)x.n;
+        ++items;
+      }
+      const bool any = !(l <= 0.f);  // a row with a score that is not a number keeps saying so
+      const float inv = any ? 1.f / l : 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        float v[32];
+        if (x.n > 0) {  // warp-uniform
+          tmem_ld32(o_addr + c * 32, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        }
+        if (!any) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        }
+        if constexpr (TREE) {
+          if (part) {
+            if (row_ok && c * 32 < d_head) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>(part + c * 32 + i) = make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
+            }
+            continue;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i] * inv, v[2 * i + 1] * inv);
+          packed[c * 16 + i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      if (x.n > 0) {
+        tc_fence_before();
+        mbar_arrive(bar(iOF));
+      }
+      if (!row_ok) continue;
+      if constexpr (TREE) {
+        if (part) {
+          p.part_lse[at] = any ? m + log2f(l) : -INFINITY;
+          continue;
+        }
+      }
+      __nv_bfloat16* dst;
+      if constexpr (TREE) {
+        dst = static_cast<__nv_bfloat16*>(p.o) + p.out_row(x.it, row) * p.o_rs + (long long)p.head(x.it, row) * d_head;
+      } else {
+        dst = static_cast<__nv_bfloat16*>(p.o) + (long long)(x.it.row0 + row) * p.o_rs + (long long)x.it.h * p.o_hs;
+        if (p.lse) p.lse[(long long)(x.it.row0 + row) * p.H + x.it.h] = any ? (m + log2f(l)) * kLn2 : -INFINITY;
+      }
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c)
+        if (c * 8 < d_head)
+          *reinterpret_cast<uint4*>(dst + c * 8) = make_uint4(packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
+    }
+    if (!ok && lane == 0 && p.status) atomicOr(p.status, 2);
+  } else {
+    // ================= softmax: two threads per row, one for each half of the key tile =================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRtSoftmaxRegs));
+    constexpr int kHalf = kBN / 2;
+    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    const float scale_log2 = p.scale_log2;
+    unsigned g = 0u, turn = 0u, items = 0u;
+    bool fail = false;
+    // Hand-over of one float between the two threads of a row: value and turn number travel in one 8-byte word (a single store, so no
+    // fence is needed), slots alternate, and the reader polls with a clock limit.
+    auto exchange = [&](float mine, bool& ok) -> float {
+      const unsigned xb = turn & 1u;
+      const unsigned long long want = (unsigned long long)(turn + 1u) << 32;
+      xch[(xb * 2 + half) * kBM + row] = want | __float_as_uint(mine);
+      const volatile unsigned long long* partner = xch + (xb * 2 + (half ^ 1)) * kBM + row;
+      ++turn;
+      const long long t_begin = clock64();
+      for (int spin = 0;; ++spin) {
+        const unsigned long long got = *partner;
+        if ((got >> 32) == (want >> 32)) return __uint_as_float((uint32_t)got);
+        if ((spin & 63) == 63 && (*abort_flag || clock64() - t_begin > kWaitLimitCycles)) {
+          if (!*abort_flag) *abort_flag = 2;
+          ok = false;
+          return 0.f;
+        }
+      }
+    };
+    while (!fail && walk.next_with_keys(x)) {
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < x.n; ++j, ++g) {
+        const unsigned buf = g & 1u, ph = (g >> 1) & 1u;
+        const int t0 = (x.tile0 + j) * kBN;
+        // exits are taken by whole warps (the vote makes the decision uniform), never by single lanes
+        if (!__all_sync(0xffffffffu, wait_or_abort(bar(iS + (int)buf), ph, abort_flag))) {
+          fail = true;
+          break;
+        }
+        tc_fence_after();
+        int held;  // key rows of this tile that belong to the sequence
+        if constexpr (TREE) held = x.it.key1 - t0;
+        else held = p.k_start(x.it.seq + 1) - (int)x.it.kbase - t0;
+        if (held < kBN) {  // value rows past them may hold anything: clear them so that 0 * x stays 0
+          if (!__all_sync(0xffffffffu, wait_or_abort(bar(iV + (int)buf), ph, abort_flag))) {
+            fail = true;
+            break;
+          }
+          if (half == 0 && row >= held) {
+#pragma unroll
+            for (int s = 0; s < kSub; ++s) {
+              uint4* vrow = reinterpret_cast<uint4*>(sV + buf * kTileBytes + s * kSubBytes + row * 128);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) vrow[c] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_async_smem();
+          }
+        }
+        if (quarter * 32 >= x.it.rows) {  // none of this warp's rows exists: what it leaves in P reaches no other row
+          tc_fence_before();
+          mbar_arrive(bar(iP + (int)buf));
+          continue;
+        }
+        const int c0 = t0 + half * kHalf;  // key of this thread's first column
+        float sv[kHalf];
+#pragma unroll
+        for (int c = 0; c < kHalf / 32; ++c) tmem_ld32_nowait(lane_addr + buf * 128 + half * kHalf + c * 32, &sv[c * 32]);
+        tc_wait_ld();
+        if (quarter * 32 + 32 > x.it.rows && row >= x.it.rows) {  // what Q holds there is anything: level scores keep the warp on the short path
+#pragma unroll
+          for (int i = 0; i < kHalf; ++i) sv[i] = 0.f;
+        }
+        if (t0 + kBN > x.it.clear && row < x.it.rows) {
+          if constexpr (TREE) {
+            // bit i: column i is seen
+            unsigned long long seen = ~0ull;
+            const int d0 = c0 - x.it.clear;
+            if (d0 > -kHalf) {
+              const unsigned long long* words = p.mask_row(x.it, row);
+              auto word = [&](int w) { return w < p.words ? words[w] : 0ull; };
+              if (d0 < 0) {
+                seen = (word(0) << -d0) | ((1ull << -d0) - 1ull);
+              } else {
+                const int w = d0 >> 6, s = d0 & 63;
+                seen = word(w) >> s;
+                if (s) seen |= word(w + 1) << (64 - s);
+              }
+            }
+            const int left = x.it.key1 - c0;
+            if (left < kHalf) seen = left > 0 ? seen & ((1ull << left) - 1ull) : 0ull;
+            const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              sv[i] = (lo >> i) & 1u ? sv[i] : -INFINITY;
+              sv[32 + i] = (hi >> i) & 1u ? sv[32 + i] : -INFINITY;
+            }
+          } else {
+            const int last = min(x.it.last0 + row, x.it.key1 - 1) - c0;
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) sv[i] = i <= last ? sv[i] : -INFINITY;
+          }
+        }
+        // One sweep turns this thread's scores into probabilities against a reference (log2 domain), writes them as packed bf16 and
+        // returns their sum, and the largest exponent met.
+        auto sweep = [&](float ref, float& top) -> float {
+          const uint64_t scale2 = pack2(scale_log2, scale_log2), negm2 = pack2(-ref, -ref);
+          uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
+          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < kHalf / 32; ++c) {
+            uint32_t packed[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float x0, x1;
+              unpack2(fma2(pack2(sv[c * 32 + i], sv[c * 32 + i + 1]), scale2, negm2), x0, x1);
+              tops[(i >> 1) & 3] = max3(tops[(i >> 1) & 3], x0, x1);
+              const float p0 = ex2(x0), p1 = ex2(x1);  // -inf -> 0
+              rs2[(i >> 1) & 3] = add2(rs2[(i >> 1) & 3], pack2(p0, p1));
+              const __nv_bfloat162 pk = __floats2bfloat162_rn(p0, p1);
+              packed[i >> 1] = *reinterpret_cast<const uint32_t*>(&pk);
+            }
+            tmem_st16(lane_addr + kPCol + buf * 64 + half * (kHalf / 2) + c * 16, packed);
+          }
+          float ra, rb, rc, rd;
+          unpack2(add2(rs2[0], rs2[1]), ra, rb);
+          unpack2(add2(rs2[2], rs2[3]), rc, rd);
+          top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+          return (ra + rb) + (rc + rd);
+        };
+        // From an item's second tile on the running maximum is almost always still good (it has to be within 2^8 of the true one), so the
+        // probabilities are taken against it at once and the tile's maximum is found on the way; m is the same in both threads of a row and
+        // so is the decision, and the votes are the same in both of its warps.
+        bool xok = true, settled = false;
+        float mx2, sum = 0.f, top;
+        const bool fast = __all_sync(0xffffffffu, m != -INFINITY);
+        if (fast) {
+          sum = sweep(m, top);
+          mx2 = fmaxf(top, exchange(top, xok)) + m;  // exponents were taken against m
+        } else {
+          float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < kHalf; i += 8) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mxs[c] = max3(mxs[c], sv[i + 2 * c], sv[i + 2 * c + 1]);
+          }
+          const float mine = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
+          mx2 = fmaxf(mine, exchange(mine, xok)) * scale_log2;
+        }
+        if (!__all_sync(0xffffffffu, xok)) {
+          fail = true;
+          break;
+        }
+        if (fast && !__any_sync(0xffffffffu, mx2 > m + 8.f)) {
+          l += sum;
+          settled = true;
+        }
+        if (!settled) {
+          float alpha = 1.f;
+          if (mx2 > m + 8.f || m == -INFINITY) {
+            alpha = m == -INFINITY ? 0.f : ex2(m - mx2);
+            m = mx2;
+          }
+          if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+            // O may only be touched when no product into it is in flight: that of the tile before must be done (this tile's waits for this row)
+            if (!__all_sync(0xffffffffu, wait_or_abort(bar(iO + (int)(buf ^ 1u)), ((g - 1) >> 1) & 1u, abort_flag))) {
+              fail = true;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              float v[32];
+              tmem_ld32(lane_addr + kOCol + half * (D / 2) + c * 32, v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] *= alpha;
+              tmem_st32(lane_addr + kOCol + half * (D / 2) + c * 32, v);
+            }
+          }
+          l = l * alpha + sweep(m == -INFINITY ? 0.f : m, top);
+        }
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar(iP + (int)buf));
+      }
+      if (fail) break;
+      // the item's sums go to the output threads
+      const int slot = (int)(items & 1u);
+      if (items >= 2 && !__all_sync(0xffffffffu, wait_or_abort(bar(iLF + slot), ((items - 2) >> 1) & 1u, abort_flag))) {
+        fail = true;
+        break;
+      }
+      sums[(slot * 3 + half) * kBM + row] = l;
+      if (half == 0) sums[(slot * 3 + 2) * kBM + row] = m;
+      mbar_arrive(bar(iL + slot));
+      ++items;
+    }
+    if (fail && p.status) atomicOr(p.status, 2);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, kTmem);
+}
+
+}  // namespace tc
+
+template <int D, class P, bool TREE>
+static int ragged_tc_go(const TcMaps& maps, const P& p, long long items, int d_head, cudaStream_t st) {
+  using namespace tc;
+  static int n_sm[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    set_error("ragged attention: cannot identify the current device");
+    return DGPT_E_CUDA;
+  }
+  if (n_sm[dev] == 0) cudaDeviceGetAttribute(&n_sm[dev], cudaDevAttrMultiProcessorCount, dev);
+  const long long ctas = items < n_sm[dev] ? items : n_sm[dev];
+  size_t smem = (size_t)6 * (D / 64) * kBN * 128 + 32 * 8 + 4 * kBM * 8 + 6 * kBM * 4 + (TREE ? 0 : 2 * kRtStaged * 4) + 1024;
+  if (smem < 120 * 1024) smem = 120 * 1024;  // one CTA owns an SM: it takes all 512 TMEM columns
+  auto kernel = ragged_tc_kernel<D, P, TREE>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) {
+    set_error("ragged attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    return DGPT_E_CUDA;
+  }
+  kernel<<<(unsigned)ctas, kRtThreads, smem, st>>>(maps.q, maps.k, maps.v, p, d_head);
+  return launch_status("ragged attention");
+}
+
+static bool tc_type(int D, int dtype) {
+  return dtype == DGPT_BF16 && (D == 32 || D == 64 || D == 128) && tc::device_is_sm100() && tc::encode_fn() != nullptr;
+}
+
+bool packed_tc_supported(const PackedProblem& p, int D, int dtype) { return p.n_keys > 0 && tc_type(D, dtype); }
+
+int packed_tc(const PackedProblem& p, int D, cudaStream_t st) {
+  using namespace tc;
+  TcMaps maps;
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)kBM, 1};
+  auto map = [&](CUtensorMap* m, const void* base, int heads, int rows, long long rs, long long hs) {
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows, 1};
+    const cuuint64_t strides[3] = {(cuuint64_t)hs * 2, (cuuint64_t)rs * 2, (cuuint64_t)rs * 2};
+    return encode_map(m, base, dims, strides, box);
+  };
+  if (!map(&maps.q, p.q, p.H, p.n_rows, p.q_rs, p.q_hs) || !map(&maps.k, p.k, p.G, p.n_keys, p.k_rs, p.k_hs) ||
+      !map(&maps.v, p.v, p.G, p.n_keys, p.v_rs, p.v_hs))
+    return DGPT_E_CUDA;
+  const long long items = p.slots(kBM) * p.H;
+  return D == 128 ? ragged_tc_go<128, PackedProblem, false>(maps, p, items, D, st) : ragged_tc_go<64, PackedProblem, false>(maps, p, items, D, st);
+}
+
+// Pages must make up whole key tiles, or be made up by them; one dense run per sequence may have any length: a tile never leaves the
+// run's tensor, and what the box covers past its end arrives as zeros.
+bool tree_tc_supported(const TreeProblem& p, int dtype) {
+  const int pt = p.kv.page_tokens;
+  if (!tc_type(p.D, dtype) || p.group > tc::kBM) return false;
+  if (p.kv.head_stride <= 0 || p.kv.page_stride <= 0) return false;
+  return p.kv.page_table == nullptr || (pt >= tc::kBN ? pt % tc::kBN == 0 : pt >= 8 && tc::kBN % pt == 0);
+}
+
+int tree_tc(const TreeProblem& full, cudaStream_t st) {
+  using namespace tc;
+  TreeProblem p = full;
+  const int nodes = kBM / p.group < p.T ? kBM / p.group : p.T;  // drafts of a tile, with all heads of a group
+  p.rows_per_tile = nodes * p.group;
+  p.tiles = (p.T + nodes - 1) / nodes;
+  const int D = p.D, pt = p.kv.page_tokens;
+  TcMaps maps;
+  {
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)p.H, (cuuint64_t)p.T, (cuuint64_t)p.B};
+    const cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)p.q_rs * 2, (cuuint64_t)p.q_rs * p.T * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)p.group, (cuuint32_t)nodes, 1};
+    if (!encode_map(&maps.q, p.q, dims, strides, box)) return DGPT_E_CUDA;
+  }
+  const bool dense = p.kv.page_table == nullptr;
+  const cuuint64_t n_pages = dense ? (cuuint64_t)p.B : p.kv.n_pages > 0 ? (cuuint64_t)p.kv.n_pages : (cuuint64_t)1 << 24;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)pt, (cuuint64_t)p.G, n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)p.kv.token_stride * 2, (cuuint64_t)p.kv.head_stride * 2, (cuuint64_t)p.kv.page_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)(!dense && pt < kBN ? pt : kBN), 1, 1};
+  if (!encode_map(&maps.k, p.kv.k, dims, strides, box) || !encode_map(&maps.v, p.kv.v, dims, strides, box)) return DGPT_E_CUDA;
+  return D == 128 ? ragged_tc_go<128, TreeProblem, true>(maps, p, p.items(), D, st) : ragged_tc_go<64, TreeProblem, true>(maps, p, p.items(), D, st);
+}
+
+}  // namespace dgpt

@@ -602,7 +602,7 @@ int dgpt_retention(const void* in, int64_t in_row_stride, int32_t q_col, int32_t
  * seq_starts, key_starts: device int32 [n_seq + 1], not decreasing, within 0 .. n_rows (n_keys); status bit 0 is set where
  * they are not (rows are then wrong, but nothing outside the tensors is touched).
  * D: 8, 16, 32, 64, 128.  impl: 0 = choose, 1 = CUDA cores, 2 = tcgen05 (bf16, D = 32, 64, 128) or fail.
- * status: device int32 or NULL; set to another value than 1 if a bounded wait ran out. */
+ * status: device int32 or NULL; bit 1 is set if a bounded wait ran out. */
 int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k, int64_t k_row_stride,
                      int64_t k_head_stride, const void* v, int64_t v_row_stride, int64_t v_head_stride, void* o,
                      int64_t o_row_stride, int64_t o_head_stride, float* lse, const int32_t* seq_starts,
