@@ -49,14 +49,23 @@ extern "C" int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_h
   return packed_simt(p, D, dtype, static_cast<cudaStream_t>(stream));
 }
 
+// One round of CTAs: a share is as long as its sequences allow.  The tensor-core kernel takes 128 rows an item and one CTA an SM, the other
+// 16 or 64 rows and two CTAs or more; a share below two tiles would wait for the second pass longer than it saves.
 extern "C" int32_t dgpt_tree_attn_splits(int32_t B, int32_t T, int32_t H, int32_t G, int32_t D, int32_t max_keys, int32_t dtype) {
-  (void)D;
-  (void)dtype;
   if (B <= 0 || T <= 0 || H <= 0 || G <= 0 || H % G != 0 || max_keys <= 0) return 1;
-  const long long rows = (long long)T * (H / G), tiles = rows <= 16 ? 1 : (rows + 63) / 64;
-  const long long items = (long long)B * G * tiles;
-  const long long want = (2 * 148 + items - 1) / items, most = (max_keys + 255) / 256;
-  const long long n = want < most ? want : most;
+  const bool tensor = dtype == DGPT_BF16 && D >= 32;
+  const long long group = H / G, rows = T * group;
+  long long tiles, ctas;
+  if (tensor) {
+    const long long nodes = group < 128 ? 128 / group : 1;
+    tiles = (T + nodes - 1) / nodes;
+    ctas = 148;
+  } else {
+    tiles = rows <= 16 ? 1 : (rows + 63) / 64;
+    ctas = 2 * 148;
+  }
+  const long long items = (long long)B * G * tiles, fit = ctas / items, most = (max_keys + 255) / 256;
+  const long long n = fit < most ? fit : most;
   return (int32_t)(n < 1 ? 1 : n > 256 ? 256 : n);
 }
 

@@ -20,7 +20,8 @@ struct RaggedItem {
   int clear;
   int last0;       // packed: the last key that the tile's first row sees (negative: none); row r sees r more
   int split;       // tree: which share of the keys
-  long long kbase; // packed: row of the sequence's key 0
+  int kbase;       // packed: row of the sequence's key 0
+  int held;        // packed: the sequence's keys
 };
 
 // ---- packed prompts ---------------------------------------------------------------------------------------------
@@ -45,22 +46,55 @@ struct PackedProblem {
   // A start is taken into the tensor's rows: wrong numbers give wrong rows, never an access outside.
   __device__ int q_start(int s) const { return min(max(q_starts[s], 0), n_rows); }
   __device__ int k_start(int s) const { return min(max(k_starts[s], 0), n_keys); }
-  __device__ bool item(long long slot, int h, int bm, RaggedItem& it) const {
+  // The last sequence whose base is not behind the slot: 32 at a time, for a whole warp.
+  __device__ int find(int slot, int bm, int lane) const {
+    int lo = 0, n = n_seq;
+    while (n > 1) {
+      const int step = (n + 31) >> 5, s = lo + lane * step;
+      const bool before = lane * step < n && q_start(s) / bm + s <= slot;
+      const int last = 31 - __clz(__ballot_sync(0xffffffffu, before) | 1u);
+      lo += last * step;
+      n = min(step, n - last * step);
+    }
+    return lo;
+  }
+  // The same by halves, for a thread.
+  __device__ int find(int slot, int bm) const {
     int lo = 0, hi = n_seq - 1;
-    while (lo < hi) {  // the last sequence whose base is not behind the slot
+    while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if ((long long)(q_start(mid) / bm) + mid <= slot) lo = mid;
+      if (q_start(mid) / bm + mid <= slot) lo = mid;
       else hi = mid - 1;
     }
-    const int first = q_start(lo), end = q_start(lo + 1);
-    const long long row0 = first + (slot - first / bm - lo) * bm;
-    if (row0 < first || row0 >= end) return false;
+    return lo;
+  }
+  // A sequence and what is known of it.
+  struct Cursor {
+    int seq = 0, first = 0, end = 0, kb = 0, nk = 0, slot0 = 0, slot1 = 0;  // it has slots [slot0, slot1)
+  };
+  __device__ void load(int s, int bm, Cursor& c) const {
+    c.seq = s;
+    c.first = q_start(s);
+    c.end = q_start(s + 1);
+    c.kb = k_start(s);
+    c.nk = max(0, k_start(s + 1) - c.kb);
+    c.slot0 = c.first / bm + s;
+    c.slot1 = c.end / bm + s + 1;
+  }
+  __device__ void seek(int slot, int bm, int lane, Cursor& c) const {
+    if (slot < c.slot0 || slot >= c.slot1) load(find(slot, bm, lane), bm, c);
+  }
+  __device__ bool item(int slot, const Cursor& c, int h, int bm, RaggedItem& it) const {
+    const int first = c.first, end = c.end, lo = c.seq;
+    const int tile = slot - first / bm - lo;
+    if (tile < 0 || (long long)first + (long long)tile * bm >= end) return false;
+    const int row0 = first + tile * bm;
     it.seq = lo;
     it.h = h;
     it.g = h / (H / G);
-    it.row0 = (int)row0;
-    it.rows = min(bm, end - (int)row0);
-    const int kb = k_start(lo), nk = max(0, k_start(lo + 1) - kb);
+    it.row0 = row0;
+    it.rows = min(bm, end - row0);
+    const int kb = c.kb, nk = c.nk;
     const long long behind = (long long)nk - (end - first) + (row0 - first);  // keys before the one of the tile's first row
     it.key0 = 0;
     it.last0 = (int)behind;
@@ -68,6 +102,7 @@ struct PackedProblem {
     it.clear = (int)max(0ll, min((long long)nk, behind + 1));
     it.split = 0;
     it.kbase = kb;
+    it.held = nk;
     return true;
   }
   __device__ bool sees(const RaggedItem& it, int r, int j) const { return j < it.key1 && j <= it.last0 + r; }
@@ -77,11 +112,11 @@ struct PackedProblem {
   }
   template <typename T>
   __device__ const T* k_row(const RaggedItem& it, int j) const {
-    return static_cast<const T*>(k) + (it.kbase + j) * k_rs + (long long)it.g * k_hs;
+    return static_cast<const T*>(k) + (long long)(it.kbase + j) * k_rs + (long long)it.g * k_hs;
   }
   template <typename T>
   __device__ const T* v_row(const RaggedItem& it, int j) const {
-    return static_cast<const T*>(v) + (it.kbase + j) * v_rs + (long long)it.g * v_hs;
+    return static_cast<const T*>(v) + (long long)(it.kbase + j) * v_rs + (long long)it.g * v_hs;
   }
   // The first CTA looks at all starts.
   __device__ void check(int block, int thread, int threads) const {
@@ -101,6 +136,7 @@ struct PackedProblem {
 // whose bit is set: word j / 64, bit j % 64 of ancestors[s][t].  The rows of one key/value head are its T * (H / G) pairs of node and
 // query head, node-major, so that K and V are read once for all of them.
 struct TreeProblem {
+  struct Cursor {};
   const void* q;
   long long q_rs;
   KvView kv;
@@ -116,7 +152,7 @@ struct TreeProblem {
   float scale_log2;
   int* status;
 
-  __host__ __device__ long long items() const { return (long long)B * G * tiles * n_splits; }
+  __host__ __device__ long long items() const { return (long long)B * G * tiles * n_splits; }  // below 2^31 (the entry point sees to it)
   // Keys [0, keys) of a sequence, of which the last `nodes` are drafts.  What does not fit the layout is left out.
   __device__ void lengths(int s, int& context, int& nodes) const {
     const long long room = (long long)(kv.page_table ? kv.max_pages : 1) * kv.page_tokens;
@@ -125,13 +161,12 @@ struct TreeProblem {
     nodes = (int)min((long long)nodes, room - context);
   }
   // Splits share the key tiles of `bn` keys evenly; the ones behind may get none.
-  __device__ bool item(long long i, int bn, RaggedItem& it) const {
-    it.split = (int)(i % n_splits);
-    i /= n_splits;
-    const int tile = (int)(i % tiles);
-    i /= tiles;
-    it.g = (int)(i % G);
-    it.seq = (int)(i / G);
+  __device__ bool item(unsigned i, int bn, RaggedItem& it) const {
+    const unsigned a = i / (unsigned)n_splits, b = a / (unsigned)tiles, c = b / (unsigned)G;
+    it.split = (int)(i - a * (unsigned)n_splits);
+    const int tile = (int)(a - b * (unsigned)tiles);
+    it.g = (int)(b - c * (unsigned)G);
+    it.seq = (int)c;
     it.h = it.g * group;
     int context, nodes;
     lengths(it.seq, context, nodes);
@@ -146,7 +181,7 @@ struct TreeProblem {
     it.key1 = min(keys, t1 * bn);
     it.clear = context;
     it.last0 = 0;
-    it.kbase = 0;
+    it.kbase = it.held = 0;
     return true;
   }
   __device__ const unsigned long long* mask_row(const RaggedItem& it, int r) const {

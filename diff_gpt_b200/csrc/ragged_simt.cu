@@ -29,9 +29,12 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
   p.check((int)blockIdx.x, tid, kRgThreads);
   RaggedItem it;
   if constexpr (TREE) {
-    if (!p.item((long long)blockIdx.x, kRgBN, it)) return;
+    if (!p.item(blockIdx.x, kRgBN, it)) return;
   } else {
-    if (!p.item((long long)blockIdx.x / p.H, (int)(blockIdx.x % p.H), BM, it)) return;
+    const unsigned slot = blockIdx.x / (unsigned)p.H;
+    typename P::Cursor cur;
+    p.load(p.find((int)slot, BM), BM, cur);
+    if (!p.item((int)slot, cur, (int)(blockIdx.x - slot * (unsigned)p.H), BM, it)) return;
   }
   for (int i = tid; i < BM * VPR; i += kRgThreads) {
     const int r = i / VPR, c = i - r * VPR;

@@ -2,9 +2,11 @@
 // the 64-wide kernel: TMA boxes reach past the tensor and arrive as zeros).
 //
 // A persistent CTA of 512 threads per SM walks through work items: 128 query rows against a run of key tiles of 128.  Lengths lie on the
-// device, so every role works an item's rows and keys out for itself (ragged.cuh).  Sequences are short as often as long, which is why
-// nothing stops between items: score products run two key tiles ahead of the probabilities whatever item they belong to, loads run ahead
-// of those, and a warpgroup of its own takes a finished item's output out of TMEM while the softmax threads are at the next one.
+// device, so a warp of its own works out the items' rows and keys (ragged.cuh) and hands them to the others through a ring in shared memory.
+// Sequences are short as often as long, which is why nothing stops between items: score products run two key tiles ahead of the
+// probabilities whatever item they belong to, loads run ahead of those, and a warpgroup of its own takes a finished item's output out
+// of TMEM while the softmax threads are at the next one.
+//   warp 14          items
 //   warp 13          loader: TMA loads of Q, and of K and V tiles into rings of 3 and 2 slots (128-byte swizzle, one box per page and 64-wide
 //                    half of the head); page numbers are fetched 32 at a time
 //   warp 12, lane 0  issuer: S_g = Q K_g^T into one of two score buffers, O += P_g V_g with P from TMEM.  P V of tile g goes before S of tile
@@ -23,51 +25,58 @@ namespace dgpt {
 namespace tc {
 
 constexpr int kRtThreads = 512;
-constexpr int kRtSoftmaxRegs = 160, kRtOutputRegs = 112, kRtHelperRegs = 80;  // 2 x 160 + 112 + 80 = 4 x 128, the launch's share
-constexpr int kRtStaged = 1024;  // prompts whose starts are kept in shared memory
+constexpr int kRtSoftmaxRegs = 176, kRtOutputRegs = 88, kRtHelperRegs = 72;  // 2 x 176 + 88 + 72 = 4 x 128, the launch's share
+constexpr int kRtRing = 8;                                                    // items between the warp that finds them and the last role that reads them
 
 struct RtItem {
   RaggedItem it;
-  int tile0, n;  // key tiles tile0 .. tile0 + n - 1
+  int tile0, n;  // key tiles tile0 .. tile0 + n - 1; n < 0: no more items
 };
+static_assert(sizeof(RtItem) % 4 == 0 && sizeof(RtItem) <= 64, "a ring slot is 64 bytes");
 
-// The items of a CTA, one by one; false at the end.  Items without rows are passed over.
+// Items are dealt at run time: the grid has a CTA for each, one per SM is resident, and a resident CTA that wants more work cancels one that
+// has not been launched and takes its number (cluster launch control).  Numbers run from a prompt's last rows, which see the most keys, to its
+// first ones, prompt by prompt, so that the CTAs at work share a prompt's K and V in L2 and the last items are the shortest.  (Dealt in fixed rounds, the
+// busiest SM had 1.25 times the mean of 2 x 16 heads of 128 x 4096; 16 on 4 heads, 4 prompts of 2678 to 3455: 228 us so, 214 dealt at run time.)
+__device__ __forceinline__ void ask_for_cta(uint32_t answer, uint32_t bar) {
+  mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ bool cta_answer(uint32_t answer, unsigned& cta) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .b64 lo, hi;\n\t.reg .pred p;\n\t"
+      "ld.shared.v2.b64 {lo, hi}, [%2];\n\tmov.b128 h, {lo, hi};\n\tmov.u32 %1, 0;\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(ok), "=&r"(x)
+      : "r"(answer)
+      : "memory");
+  cta = x;
+  return ok != 0;
+}
+
+// Item `i` of the launch; false if it has no rows.  For a whole warp.  `seq`: the sequence of the item before, where most items are found.
 template <class P, bool TREE>
-struct RtWalk {
-  const P& p;
-  long long i, total;
-  __device__ RtWalk(const P& q) : p(q), i(blockIdx.x) {
-    if constexpr (TREE) total = q.items();
-    else total = q.slots(kBM) * q.H;
+__device__ __forceinline__ bool rt_item(const P& p, unsigned i, typename P::Cursor& cur, RtItem& x, int lane) {
+  bool there;
+  if constexpr (TREE) {
+    there = p.item(i, kBN, x.it);
+  } else {
+    const unsigned j = gridDim.x - 1u - i, slot = j / (unsigned)p.H;
+    p.seek((int)slot, kBM, lane, cur);
+    there = p.item((int)slot, cur, (int)(j - slot * (unsigned)p.H), kBM, x.it);
   }
-  __device__ bool next(RtItem& x) {
-    for (; i < total; i += gridDim.x) {
-      bool there;
-      if constexpr (TREE) {
-        there = p.item(i, kBN, x.it);
-      } else {
-        const long long slot = i / p.H;  // from the end: a prompt's last rows see the most keys
-        there = p.item(total / p.H - 1 - slot, (int)(i - slot * p.H), kBM, x.it);
-      }
-      if (!there) continue;
-      x.tile0 = x.it.key0 / kBN;
-      x.n = (x.it.key1 - x.it.key0 + kBN - 1) / kBN;
-      i += gridDim.x;
-      return true;
-    }
-    return false;
-  }
-  __device__ bool next_with_keys(RtItem& x) {
-    while (next(x))
-      if (x.n > 0) return true;
-    return false;
-  }
-};
+  if (!there) return false;
+  x.tile0 = x.it.key0 / kBN;
+  x.n = (x.it.key1 - x.it.key0 + kBN - 1) / kBN;
+  return true;
+}
 
 template <int D, class P, bool TREE>
 __global__ void __launch_bounds__(kRtThreads, 1)
 ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-                 const P given, const int d_head) {
+                 const P p, const int d_head) {
   constexpr int kSub = D / 64;
   constexpr uint32_t kSubBytes = kBN * 128;
   constexpr uint32_t kTileBytes = kSub * kSubBytes;
@@ -78,37 +87,35 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sV = smem + 4 * kTileBytes;  // Q | K0 K1 K2 | V0 V1 | barriers | hand-over words | row sums | starts
+  uint8_t* sV = smem + 4 * kTileBytes;  // Q | K0 K1 K2 | V0 V1 | barriers | hand-over words | row sums | items
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * kTileBytes);
-  constexpr int iQ = 0, iQF = 1, iK = 2, iKF = 5, iV = 8, iS = 10, iP = 12, iO = 14, iOF = 16, iL = 17, iLF = 19, nBars = 21;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + nBars);
+  constexpr int iQ = 0, iQF = 1, iK = 2, iKF = 5, iV = 8, iS = 10, iP = 12, iO = 14, iOF = 16, iL = 17, iLF = 19, iR = 21, iRF = iR + kRtRing,
+                iC = iRF + kRtRing, nBars = iC + 1;
+  static_assert(nBars <= 43, "barriers, an answer of 16 bytes and two words in 46 words");
+  uint64_t* answer = bars + 44;  // 16-byte aligned
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 43);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile unsigned long long* xch = reinterpret_cast<volatile unsigned long long*>(bars + 32);  // [2 turns][2 halves][128 rows]
-  float* sums = reinterpret_cast<float*>(bars + 32 + 4 * kBM);                                   // [2 items][l of half 0 | of half 1 | m][128 rows]
-  int* staged = reinterpret_cast<int*>(sums + 2 * 3 * kBM);                                      // packed: query starts, then key starts
+  volatile unsigned long long* xch = reinterpret_cast<volatile unsigned long long*>(bars + 48);  // [2 turns][2 halves][128 rows]
+  float* sums = reinterpret_cast<float*>(bars + 48 + 4 * kBM);                                   // [2 items][l of half 0 | of half 1 | m][128 rows]
+  uint8_t* ring = reinterpret_cast<uint8_t*>(sums + 2 * 3 * kBM);                                // [kRtRing] items
   const uint32_t aQ = smem_u32(smem), aK = aQ + kTileBytes, aV = aQ + 4 * kTileBytes, bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  P p = given;
-  if constexpr (!TREE) {
-    if (given.n_seq < kRtStaged) {
-      for (int s = tid; s <= given.n_seq; s += kRtThreads) {
-        staged[s] = given.q_starts[s];
-        staged[kRtStaged + s] = given.k_starts[s];
-      }
-      p.q_starts = staged;
-      p.k_starts = staged + kRtStaged;
-    }
-  }
   if (tid == 0) {
     *abort_flag = 0;
     for (int i = 0; i < nBars; ++i)
-      mbar_init(bar(i), (i == iP || i == iP + 1 || i == iL || i == iL + 1) ? 2 * kBM : (i == iOF || i == iLF || i == iLF + 1) ? kBM : 1);
+      mbar_init(bar(i), (i == iP || i == iP + 1 || i == iL || i == iL + 1) ? 2 * kBM : (i == iOF || i == iLF || i == iLF + 1) ? kBM : i >= iRF && i < iC ? 14 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
   for (int i = tid; i < 4 * kBM; i += kRtThreads) xch[i] = 0ull;  // turn numbers of an earlier CTA must not be taken for this one's
+  if constexpr (TREE) {  // rows of Q that no load reaches: level scores keep their warp on the short path
+    for (int i = p.rows_per_tile * 8 + tid; i < kBM * 8; i += kRtThreads)
+#pragma unroll
+      for (int s = 0; s < kSub; ++s) reinterpret_cast<uint4*>(smem + s * kSubBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_async_smem();
+  }
   if (warp == 0) {
     tmem_alloc(smem_u32(tmem_slot), kTmem);
     tmem_relinquish();
@@ -117,8 +124,31 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  RtWalk<P, TREE> walk(p);
   RtItem x;
+  // A role's place in the ring.  `take` waits for the next item and reads it (every lane that calls gets it); false at the end or after a
+  // wait that ran out (`ok` tells).  A slot is free when the loader, the issuer and every softmax and output warp have said `done`.
+  // (Output and item warps wait for thousands of cycles at a time: they sleep between looks, so that their polling takes no issue slots from
+  // the softmax warps that share their schedulers.)
+  auto wait_asleep = [&](int b, unsigned parity) -> bool {
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar(b), parity)) {
+      if (*abort_flag) return false;
+      if (clock64() - t0 > kWaitLimitCycles) {
+        *abort_flag = 2;
+        return false;
+      }
+      __nanosleep(100);
+    }
+    return true;
+  };
+  unsigned taken = 0u;
+  auto take = [&](RtItem& y, unsigned at, bool& ok) -> bool {
+    ok = wait_or_abort(bar(iR + (int)(at % kRtRing)), (at / kRtRing) & 1u, abort_flag);
+    if (!ok) return false;
+    y = *reinterpret_cast<const RtItem*>(ring + (at % kRtRing) * 64);
+    return y.n >= 0;
+  };
+  auto done = [&](unsigned at) { mbar_arrive(bar(iRF + (int)(at % kRtRing))); };
 
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRtHelperRegs));
@@ -132,43 +162,72 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       unsigned items = 0u, kn = 0u, vn = 0u;  // loads issued: Q, K tiles, V tiles
       bool ok = true;
       auto wait = [&](int b, unsigned parity) { return __all_sync(0xffffffffu, wait_or_abort(bar(b), parity, abort_flag)) != 0; };
-      int page0 = 0, page_seq = -1, page_id = 0;  // tree: this lane's page number is that of page page0 + lane of sequence page_seq
-      auto load_tile = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, const RtItem& w, int t) {
+      // tree: this lane holds the numbers of pages page0 + lane and page0 + 32 + lane of sequence page_seq, the latter on their way while the
+      // former are used, and those of page `lane` of the last two K tiles, of which one is the next V tile
+      int page0 = 0, page_seq = -1, page_id = 0, page_next = 0, newer = 0, older = 0;
+      int pt = 0, max_pages = 0;  // pt 0: a dense run per sequence
+      const int* tables = nullptr;
+      if constexpr (TREE) {
+        tables = p.kv.page_table;
+        max_pages = p.kv.max_pages;
+        pt = tables ? p.kv.page_tokens : 0;
+      }
+      const bool dense = pt == 0;
+      const int per = dense || pt >= kBN ? 1 : kBN / pt;  // pages of a tile
+      auto find_pages = [&](const RtItem& w, int t) {
+        older = newer;
+        if (dense) {
+          newer = w.it.seq;
+          return;
+        }
+        const int first = t * kBN / pt;
+        if (page_seq != w.it.seq || first < page0 || first + per > page0 + 32) {
+          const int* table = tables + (long long)w.it.seq * max_pages;
+          auto fetch = [&](int lp) { return table[min(lp + lane, max_pages - 1)]; };
+          // (32 pages hold a whole number of tiles, so a tile's pages end where a block of 32 ends)
+          page_id = page_seq == w.it.seq && first == page0 + 32 ? page_next : fetch(first);
+          page_seq = w.it.seq;
+          page0 = first;
+          page_next = fetch(first + 32);
+        }
+        newer = __shfl_sync(0xffffffffu, page_id, (first - page0 + lane) & 31);
+      };
+      auto load_tile = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, const RtItem& w, int t, int pages) {
         const int t0 = t * kBN;
         if constexpr (!TREE) {
           if (lane == 0) {
             mbar_expect_tx(full, kTileBytes);
 #pragma unroll
-            for (int s = 0; s < kSub; ++s) tma_load_4d(dst + s * kSubBytes, map, full, s * 64, w.it.g, (int)(w.it.kbase + t0), 0);
+            for (int s = 0; s < kSub; ++s) tma_load_4d(dst + s * kSubBytes, map, full, s * 64, w.it.g, w.it.kbase + t0, 0);
           }
         } else {
-          const int pt = p.kv.page_tokens;
-          const bool dense = p.kv.page_table == nullptr;
-          const int per = dense || pt >= kBN ? 1 : kBN / pt;
-          const int first = dense ? 0 : t0 / pt;
           const int valid = per == 1 ? 1 : min(per, (w.it.key1 - t0 + pt - 1) / pt);
-          if (!dense && (page_seq != w.it.seq || first < page0 || first + valid > page0 + 32)) {
-            page_seq = w.it.seq;
-            page0 = first;
-            const int at = min(first + lane, p.kv.max_pages - 1);
-            page_id = p.kv.page_table[(long long)w.it.seq * p.kv.max_pages + at];
-          }
+          const int in = per > 1 ? 0 : dense ? t0 : t0 % pt;
           if (lane == 0) mbar_expect_tx(full, per == 1 ? kTileBytes : (uint32_t)valid * pt * 128u * kSub);
-          for (int q = 0; q < valid; ++q) {
-            const int pg = dense ? w.it.seq : __shfl_sync(0xffffffffu, page_id, first + q - page0);
-            if (lane == 0) {
+          __syncwarp();
+          // a lane per page
+          if (lane < valid) {
 #pragma unroll
-              for (int s = 0; s < kSub; ++s)
-                tma_load_4d(dst + s * kSubBytes + q * pt * 128, map, full, s * 64, per == 1 ? t0 - first * pt : 0, w.it.g, pg);
-            }
+            for (int s = 0; s < kSub; ++s) tma_load_4d(dst + s * kSubBytes + lane * pt * 128, map, full, s * 64, in, w.it.g, pages);
           }
         }
       };
+      auto take_all = [&](RtItem& y, unsigned& at, bool free) -> bool {  // the next item with keys, for the whole warp
+        for (;;) {
+          bool fine;
+          const bool there = take(y, at, fine);
+          ok = __all_sync(0xffffffffu, fine) != 0;
+          if (!ok || !there) return false;
+          ++at;
+          if (y.n > 0) return true;
+          if (free && lane == 0) done(at - 1);
+        }
+      };
       // K runs one tile ahead of V, across items too
-      RtWalk<P, TREE> ahead(p);
       RtItem y;  // item of the K cursor
+      unsigned ahead = 0u;
       int kj = 0;
-      bool more = ahead.next_with_keys(y);
+      bool more = take_all(y, ahead, false);
       auto load_k = [&]() {
         if (kj == 0) {
           if (items > 0) ok = wait(iQF, (items - 1) & 1u);  // the last S of the item before is done
@@ -189,24 +248,27 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         const unsigned ks = kn % 3u, ku = kn / 3u;
         if (ku > 0) ok = wait(iKF + (int)ks, (ku - 1) & 1u);
         if (!ok) return;
-        load_tile(&mk, aK + ks * kTileBytes, bar(iK + (int)ks), y, y.tile0 + kj);
+        if constexpr (TREE) find_pages(y, y.tile0 + kj);
+        load_tile(&mk, aK + ks * kTileBytes, bar(iK + (int)ks), y, y.tile0 + kj, newer);
         ++kn;
         if (++kj == y.n) {
           kj = 0;
-          more = ahead.next_with_keys(y);
+          more = take_all(y, ahead, false);
         }
       };
       if (more) load_k();
-      while (ok && walk.next_with_keys(x)) {
+      while (ok && take_all(x, taken, true)) {
         for (int j = 0; ok && j < x.n; ++j) {
           if (more) load_k();
           if (!ok) break;
           const unsigned vs = vn & 1u;
           if (vn >= 2) ok = wait(iO + (int)vs, ((vn - 2) >> 1) & 1u);
           if (!ok) break;
-          load_tile(&mv, aV + vs * kTileBytes, bar(iV + (int)vs), x, x.tile0 + j);
+          load_tile(&mv, aV + vs * kTileBytes, bar(iV + (int)vs), x, x.tile0 + j, kn == vn + 1u ? newer : older);
           ++vn;
         }
+        __syncwarp();
+        if (lane == 0) done(taken - 1);
       }
       if (!ok || *abort_flag) {  // something ran out of time: give the copies still in flight a bounded chance to land
         if (lane == 0 && p.status) atomicOr(p.status, 2);
@@ -218,11 +280,19 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       // ================= MMA issuer (one lane) =================
       if (lane == 0) {
         const uint64_t dQK = smem_desc(0, 16, 1024), dV = smem_desc(0, kSubBytes, 1024);
-        RtWalk<P, TREE> ahead(p);
         RtItem y;  // item of the score cursor
         int sj = 0;
-        unsigned items = 0u, sg = 0u, g = 0u;
-        bool ok = true, more = ahead.next_with_keys(y);
+        unsigned items = 0u, sg = 0u, g = 0u, ahead = 0u;
+        bool ok = true;
+        auto take_one = [&](RtItem& z, unsigned& at, bool free) -> bool {  // the next item with keys
+          for (;;) {
+            if (!take(z, at, ok)) return false;
+            ++at;
+            if (z.n > 0) return true;
+            if (free) done(at - 1);
+          }
+        };
+        bool more = take_one(y, ahead, false);
         auto issue_s = [&]() {  // S(sg & 1) = Q K(sg % 3)^T
           if (sj == 0) {
             ok = wait_or_abort(bar(iQ), items & 1u, abort_flag);
@@ -239,12 +309,12 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
           if (++sj == y.n) {
             umma_commit(bar(iQF));  // Q may be overwritten
             sj = 0;
-            more = ahead.next_with_keys(y);
+            more = take_one(y, ahead, false);
           }
         };
         for (int i = 0; i < 2 && ok && more; ++i) issue_s();
         unsigned outs = 0u;  // items whose first P V has been issued
-        while (ok && walk.next_with_keys(x)) {
+        while (ok && take_one(x, taken, true)) {
           for (int j = 0; ok && j < x.n; ++j, ++g) {
             const unsigned buf = g & 1u, ph = (g >> 1) & 1u;
             // P_g is complete when every row has arrived; by then every row has also consumed S_g
@@ -259,6 +329,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
             umma_commit(bar(iO + (int)buf));
             if (more) issue_s();
           }
+          if (ok) done(taken - 1);
         }
         if (!ok) {
           if (!*abort_flag) *abort_flag = 2;
@@ -266,6 +337,51 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         }
       }
     } else if (warp == 14) {
+      // ================= items =================
+      // An item is asked for when it will be wanted soon and not before, so that none waits behind a long one while another SM idles: beside
+      // the oldest unfinished item there is one more, or as many as make up three key tiles.
+      typename P::Cursor cursor;
+      unsigned at = 0u, freed = 0u, asked = 0u, cta = blockIdx.x;  // items handed out, items finished
+      int ahead = 0;                                               // key tiles of those behind the oldest unfinished one
+      bool ok = true, more = true;
+      auto make_room = [&](bool full_only) {
+        while (ok && at - freed >= (full_only ? (unsigned)kRtRing : 2u) && (full_only || ahead >= 3 || at - freed >= kRtRing)) {
+          ok = __all_sync(0xffffffffu, wait_asleep(iRF + (int)(freed % kRtRing), (freed / kRtRing) & 1u)) != 0;
+          ++freed;
+          if (ok && at > freed) ahead -= reinterpret_cast<const RtItem*>(ring + (freed % kRtRing) * 64)->n;
+        }
+      };
+      auto push = [&]() {
+        make_room(true);
+        if (!ok) return;
+        if (lane == 0) {
+          *reinterpret_cast<RtItem*>(ring + (at % kRtRing) * 64) = x;
+          mbar_arrive(bar(iR + (int)(at % kRtRing)));
+        }
+        __syncwarp();
+        if (at > freed) ahead += x.n;
+        ++at;
+      };
+      while (ok && more) {
+        if (rt_item<P, TREE>(p, cta, cursor, x, lane)) push();
+        make_room(false);
+        if (!ok) break;
+        if (lane == 0) ask_for_cta(smem_u32(answer), bar(iC));
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(iC), asked & 1u))) {
+          *abort_flag = 2;
+          ok = false;
+          break;
+        }
+        ++asked;
+        more = cta_answer(smem_u32(answer), cta);
+        fence_async_smem();  // read here before the next answer is written
+        __syncwarp();
+      }
+      if (ok) {
+        x.n = -1;
+        push();
+      }
+      if (!ok && lane == 0 && p.status) atomicOr(p.status, 2);
       p.check((int)blockIdx.x, lane, 32);
     }
   } else if (warp >= 8) {
@@ -275,7 +391,13 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
     const uint32_t o_addr = tmem + ((uint32_t)(quarter * 32) << 16) + kOCol;
     unsigned items = 0u, g = 0u;
     bool ok = true;
-    while (ok && walk.next(x)) {
+    for (;; ++taken) {
+      bool fine;
+      const bool there = take(x, taken, fine);
+      ok = __all_sync(0xffffffffu, fine) != 0;
+      if (!ok || !there) break;
+      __syncwarp();
+      if (lane == 0) done(taken);
       const bool row_ok = row < x.it.rows;
       float l = 0.f, m = -INFINITY;
       uint32_t packed[D / 2];
@@ -289,7 +411,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       }
       if (x.n > 0) {
         const int slot = (int)(items & 1u);
-        ok = __all_sync(0xffffffffu, wait_or_abort(bar(iL + slot), (items >> 1) & 1u, abort_flag)) != 0;
+        ok = __all_sync(0xffffffffu, wait_asleep(iL + slot, (items >> 1) & 1u)) != 0;
         if (!ok) break;
         const float* sum = sums + slot * 3 * kBM;
         l = sum[row] + sum[kBM + row];
@@ -385,21 +507,29 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         }
       }
     };
-    while (!fail && walk.next_with_keys(x)) {
+    for (;; ++taken) {
+      bool fine;
+      const bool there = take(x, taken, fine);
+      fail = !__all_sync(0xffffffffu, fine);
+      if (fail || !there) break;
+      __syncwarp();
+      if (lane == 0) done(taken);
+      const int n = x.n, rows = x.it.rows, clear = x.it.clear;
+      // Key from which value rows may hold anything: the end of the sequence's keys.
+      const int held_end = TREE ? x.it.key1 : x.it.held;
+      if (n == 0) continue;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < x.n; ++j, ++g) {
+      int t0 = x.tile0 * kBN;
+      for (int j = 0; j < n; ++j, ++g, t0 += kBN) {
         const unsigned buf = g & 1u, ph = (g >> 1) & 1u;
-        const int t0 = (x.tile0 + j) * kBN;
         // exits are taken by whole warps (the vote makes the decision uniform), never by single lanes
         if (!__all_sync(0xffffffffu, wait_or_abort(bar(iS + (int)buf), ph, abort_flag))) {
           fail = true;
           break;
         }
         tc_fence_after();
-        int held;  // key rows of this tile that belong to the sequence
-        if constexpr (TREE) held = x.it.key1 - t0;
-        else held = p.k_start(x.it.seq + 1) - (int)x.it.kbase - t0;
-        if (held < kBN) {  // value rows past them may hold anything: clear them so that 0 * x stays 0
+        if (__builtin_expect(t0 + kBN > held_end, 0)) {  // clear those rows so that 0 * x stays 0
+          const int held = held_end - t0;
           if (!__all_sync(0xffffffffu, wait_or_abort(bar(iV + (int)buf), ph, abort_flag))) {
             fail = true;
             break;
@@ -414,7 +544,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
             fence_async_smem();
           }
         }
-        if (quarter * 32 >= x.it.rows) {  // none of this warp's rows exists: what it leaves in P reaches no other row
+        if (__builtin_expect(quarter * 32 >= rows, 0)) {  // none of this warp's rows exists: what it leaves in P reaches no other row
           tc_fence_before();
           mbar_arrive(bar(iP + (int)buf));
           continue;
@@ -424,16 +554,12 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
 #pragma unroll
         for (int c = 0; c < kHalf / 32; ++c) tmem_ld32_nowait(lane_addr + buf * 128 + half * kHalf + c * 32, &sv[c * 32]);
         tc_wait_ld();
-        if (quarter * 32 + 32 > x.it.rows && row >= x.it.rows) {  // what Q holds there is anything: level scores keep the warp on the short path
-#pragma unroll
-          for (int i = 0; i < kHalf; ++i) sv[i] = 0.f;
-        }
-        if (t0 + kBN > x.it.clear && row < x.it.rows) {
+        if (__builtin_expect(t0 + kBN > clear, 0)) {
           if constexpr (TREE) {
             // bit i: column i is seen
             unsigned long long seen = ~0ull;
-            const int d0 = c0 - x.it.clear;
-            if (d0 > -kHalf) {
+            const int d0 = c0 - clear;
+            if (d0 > -kHalf && row < rows) {
               const unsigned long long* words = p.mask_row(x.it, row);
               auto word = [&](int w) { return w < p.words ? words[w] : 0ull; };
               if (d0 < 0) {
@@ -453,7 +579,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
               sv[32 + i] = (hi >> i) & 1u ? sv[32 + i] : -INFINITY;
             }
           } else {
-            const int last = min(x.it.last0 + row, x.it.key1 - 1) - c0;
+            const int last = row < rows ? min(x.it.last0 + row, x.it.key1 - 1) - c0 : kHalf;
 #pragma unroll
             for (int i = 0; i < kHalf; ++i) sv[i] = i <= last ? sv[i] : -INFINITY;
           }
@@ -491,7 +617,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         bool xok = true, settled = false;
         float mx2, sum = 0.f, top;
         const bool fast = __all_sync(0xffffffffu, m != -INFINITY);
-        if (fast) {
+        if (__builtin_expect(fast, 1)) {
           sum = sweep(m, top);
           mx2 = fmaxf(top, exchange(top, xok)) + m;  // exponents were taken against m
         } else {
@@ -512,7 +638,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
           l += sum;
           settled = true;
         }
-        if (!settled) {
+        if (__builtin_expect(!settled, 0)) {
           float alpha = 1.f;
           if (mx2 > m + 8.f || m == -INFINITY) {
             alpha = m == -INFINITY ? 0.f : ex2(m - mx2);
@@ -525,7 +651,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
               break;
             }
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 64; ++c) {
               float v[32];
               tmem_ld32(lane_addr + kOCol + half * (D / 2) + c * 32, v);
@@ -564,23 +690,27 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
 template <int D, class P, bool TREE>
 static int ragged_tc_go(const TcMaps& maps, const P& p, long long items, int d_head, cudaStream_t st) {
   using namespace tc;
-  static int n_sm[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
     set_error("ragged attention: cannot identify the current device");
     return DGPT_E_CUDA;
   }
-  if (n_sm[dev] == 0) cudaDeviceGetAttribute(&n_sm[dev], cudaDevAttrMultiProcessorCount, dev);
-  const long long ctas = items < n_sm[dev] ? items : n_sm[dev];
-  size_t smem = (size_t)6 * (D / 64) * kBN * 128 + 32 * 8 + 4 * kBM * 8 + 6 * kBM * 4 + (TREE ? 0 : 2 * kRtStaged * 4) + 1024;
+  if (items > 0x7fffffffll) {
+    set_error("ragged attention: too many rows");
+    return DGPT_E_ARG;
+  }
+  size_t smem = (size_t)6 * (D / 64) * kBN * 128 + 48 * 8 + 4 * kBM * 8 + 6 * kBM * 4 + kRtRing * 64 + 1024;
   if (smem < 120 * 1024) smem = 120 * 1024;  // one CTA owns an SM: it takes all 512 TMEM columns
   auto kernel = ragged_tc_kernel<D, P, TREE>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaSuccess;
+  static bool ready[64] = {};  // the attribute is a device's for good
+  if (!ready[dev]) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  ready[dev] = e == cudaSuccess;
   if (e != cudaSuccess) {
     set_error("ragged attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     return DGPT_E_CUDA;
   }
-  kernel<<<(unsigned)ctas, kRtThreads, smem, st>>>(maps.q, maps.k, maps.v, p, d_head);
+  kernel<<<(unsigned)items, kRtThreads, smem, st>>>(maps.q, maps.k, maps.v, p, d_head);
   return launch_status("ragged attention");
 }
 

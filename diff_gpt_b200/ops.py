@@ -52,15 +52,8 @@ def kv_layout(
 ) -> KvLayout:
     """Descriptor of one layer's K/V storage; `k`/`v` are views whose first element is the base."""
     _cuda(k, v, page_table)
-    lay = KvLayout()
-    lay.n_pages = n_pages
-    lay.k_base = k.data_ptr()
-    lay.v_base = v.data_ptr()
-    lay.page_stride = page_stride
-    lay.head_stride = head_stride
-    lay.page_table = _ptr(page_table)
-    lay.page_tokens = page_tokens
-    lay.max_pages = 0 if page_table is None else page_table.shape[-1]
+    table, max_pages = (None, 0) if page_table is None else (page_table.data_ptr(), page_table.shape[-1])
+    lay = KvLayout(k.data_ptr(), v.data_ptr(), page_stride, head_stride, table, page_tokens, max_pages, n_pages)
     lay._keep = (k, v, page_table)  # the struct holds raw addresses: keep their owners alive with it
     return lay
 
@@ -1128,23 +1121,19 @@ def streams_final(
 
 
 # ---- serving with drafted tokens ----------------------------------------------------------------
+# (Calls of a few microseconds on the GPU: what a wrapper asks of its tensors is kept to a few attribute reads each.)
 def _here(*ts: torch.Tensor | None) -> None:
     """The calls below run on the current device's stream, so that is where their tensors have to be."""
-    _cuda(*ts)
-    at = torch._C._cuda_getDevice()
+    at = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1
     for t in ts:
-        if t is not None and t.device.index != at:
+        if t is not None and (t.get_device() != at or at < 0):
+            _cuda(t)
             raise RuntimeError(f"tensors must be on the current device (cuda:{at}), got one on {t.device}")
 
 
-def _i32(name: str, t: torch.Tensor | None, *shape: int) -> None:
-    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous()):
+def _i32(name: str, t: torch.Tensor | None, shape: tuple[int, ...]) -> None:
+    if t is not None and (t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
-
-
-def _stride(t: torch.Tensor, dim: int, least: int) -> int:
-    """The stride of a dimension; of one with a single entry, any that the kernels take."""
-    return t.stride(dim) if t.shape[dim] > 1 else least
 
 
 def fmha_packed(
@@ -1167,31 +1156,40 @@ def fmha_packed(
     its last query sees all (None: the query rows').  lse: fp32 [rows, H] or None.  Rows of no prompt are left as they are.
     """
     _here(q, k, v, seq_starts, o, key_starts, lse, status)
-    if q.dim() != 3 or k.dim() != 3 or q.shape != o.shape or k.shape != v.shape or q.shape[2] != k.shape[2]:
-        raise ValueError(f"fmha_packed: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, o {tuple(o.shape)} do not fit")
-    if not q.dtype == k.dtype == v.dtype == o.dtype:
+    qsh, ksh = q.shape, k.shape
+    if len(qsh) != 3 or len(ksh) != 3 or o.shape != qsh or v.shape != ksh or qsh[2] != ksh[2]:
+        raise ValueError(f"fmha_packed: q {tuple(qsh)}, k {tuple(ksh)}, v {tuple(v.shape)}, o {tuple(o.shape)} do not fit")
+    dtype = q.dtype
+    if k.dtype is not dtype or v.dtype is not dtype or o.dtype is not dtype:
         raise TypeError("fmha_packed: q, k, v and o must have one dtype")
-    if any(t.shape[2] > 1 and t.stride(2) != 1 for t in (q, k, v, o)):
+    (N, H, D), (M, G, _) = qsh, ksh
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), o.stride()
+    if D > 1 and (qs[2] != 1 or ks[2] != 1 or vs[2] != 1 or os_[2] != 1):
         raise ValueError("fmha_packed: the elements of a head must lie side by side")
-    (N, H, D), (M, G, _) = q.shape, k.shape
+    # the stride of a dimension with one entry says nothing
+    if N < 2:
+        qs, os_ = (H * D, *qs[1:]), (H * D, *os_[1:])
+    if M < 2:
+        ks, vs = (G * D, *ks[1:]), (G * D, *vs[1:])
+    if H == 1:
+        qs, os_ = (qs[0], D), (os_[0], D)
+    if G == 1:
+        ks, vs = (ks[0], D), (vs[0], D)
     if seq_starts.dim() != 1 or seq_starts.numel() < 1:
         raise ValueError("fmha_packed: seq_starts must hold one number more than there are prompts")
-    S = seq_starts.numel() - 1
-    _i32("seq_starts", seq_starts, S + 1)
-    _i32("key_starts", key_starts, S + 1)
-    _i32("status", status, 1)
+    many = seq_starts.shape
+    _i32("seq_starts", seq_starts, many)
+    _i32("key_starts", key_starts, many)
+    _i32("status", status, (1,))
     if key_starts is None and M != N:
         raise ValueError(f"fmha_packed: {M} key rows for {N} queries need key_starts")
-    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (N, H) or not lse.is_contiguous()):
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (N, H) or not lse.is_contiguous()):
         raise ValueError(f"fmha_packed: lse must be a contiguous float32 tensor of shape {(N, H)}")
-
-    def at(t: torch.Tensor, heads: int) -> tuple[int, int, int]:
-        return t.data_ptr(), _stride(t, 0, heads * D), _stride(t, 1, D)
-
     check(
         lib.dgpt_fmha_packed(
-            *at(q, H), *at(k, G), *at(v, G), *at(o, H), _ptr(lse), seq_starts.data_ptr(), _ptr(key_starts), S, N, M, H, G, D,
-            attn_scale(D) if scale is None else scale, dtype_code(q), impl, _ptr(status), _stream(),
+            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], o.data_ptr(), os_[0], os_[1], _ptr(lse),
+            seq_starts.data_ptr(), _ptr(key_starts), many[0] - 1, N, M, H, G, D, attn_scale(D) if scale is None else scale, dtype_code(q),
+            impl, _ptr(status), _stream(),
         )
     )
 
@@ -1233,31 +1231,36 @@ def tree_attn(
     least `tree_attn_workspace_bytes` (None: allocated here).
     """
     _here(q, ctx_len, ancestors, out, n_nodes, workspace, status)
-    if ancestors.dim() == 2:
-        ancestors = ancestors.unsqueeze(2)
-    if ancestors.dim() != 3 or ancestors.dtype != torch.int64 or not ancestors.is_contiguous():
+    shape = ancestors.shape
+    if len(shape) not in (2, 3) or ancestors.dtype is not torch.int64 or not ancestors.is_contiguous():
         raise ValueError("tree_attn: ancestors must be a contiguous int64 tensor [B, T, W]")
-    B, T, words = ancestors.shape
-    if tuple(q.shape) != (B * T, H * D) or q.shape != out.shape or q.dtype != out.dtype:
-        raise ValueError(f"tree_attn: q {tuple(q.shape)} and out {tuple(out.shape)} must be {(B * T, H * D)} of one dtype")
-    if B * T > 0 and H * D > 1 and (q.stride(1) != 1 or out.stride(1) != 1):
+    B, T, words = shape if len(shape) == 3 else (*shape, 1)
+    rows = (B * T, H * D)
+    if q.shape != rows or out.shape != rows or q.dtype is not out.dtype:
+        raise ValueError(f"tree_attn: q {tuple(q.shape)} and out {tuple(out.shape)} must be {rows} of one dtype")
+    qs, os_ = q.stride(), out.stride()
+    if rows[1] > 1 and (qs[1] != 1 or os_[1] != 1):
         raise ValueError("tree_attn: the elements of a row must lie side by side")
-    _i32("ctx_len", ctx_len, B)
-    _i32("n_nodes", n_nodes, B)
-    _i32("status", status, 1)
+    if rows[0] < 2:  # the stride of a dimension with one entry says nothing
+        qs = os_ = (H * D, 1)
+    _i32("ctx_len", ctx_len, (B,))
+    _i32("n_nodes", n_nodes, (B,))
+    _i32("status", status, (1,))
+    code = dtype_code(q)
     if n_splits == 0:
         held = (kv.max_pages if kv.page_table else 1) * kv.page_tokens
-        n_splits = tree_attn_splits(B, T, H, G, D, min(max_keys, held) if max_keys > 0 else held, q.dtype) if q.dtype in _DT else 1
-    need = tree_attn_workspace_bytes(B, T, H, D, n_splits)
-    if workspace is None and need > 0:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif workspace is not None and not workspace.is_contiguous():
-        raise ValueError("tree_attn: the workspace must be contiguous")
+        n_splits = lib.dgpt_tree_attn_splits(B, T, H, G, D, min(max_keys, held) if max_keys > 0 else held, code)
+    ws_bytes = 0
+    if n_splits > 1:
+        if workspace is None:
+            workspace = q.new_empty(tree_attn_workspace_bytes(B, T, H, D, n_splits), dtype=torch.uint8)
+        elif not workspace.is_contiguous():
+            raise ValueError("tree_attn: the workspace must be contiguous")
+        ws_bytes = workspace.nbytes
     check(
         lib.dgpt_tree_attn(
-            q.data_ptr(), _stride(q, 0, H * D), C.byref(kv), token_stride or D, ctx_len.data_ptr(), _ptr(n_nodes), ancestors.data_ptr(), words,
-            out.data_ptr(), _stride(out, 0, H * D), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
-            n_splits, B, T, H, G, D, attn_scale(D) if scale is None else scale, dtype_code(q), impl, _ptr(status), _stream(),
+            q.data_ptr(), qs[0], C.byref(kv), token_stride or D, ctx_len.data_ptr(), _ptr(n_nodes), ancestors.data_ptr(), words, out.data_ptr(), os_[0],
+            _ptr(workspace), ws_bytes, n_splits, B, T, H, G, D, attn_scale(D) if scale is None else scale, code, impl, _ptr(status), _stream(),
         )
     )
 
@@ -1281,17 +1284,22 @@ def token_logprobs(
     probable tokens in descending order, equal ones by index.  logits: [R, V] (last dim contiguous), targets: int32 [R].
     (See `dgpt_token_logprobs`; `token_nll` gives the first of these alone, rounded to the logits' type.)"""
     _here(logits, targets, status)
-    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError("token_logprobs: logits must be [R, V] with the elements of a row side by side")
-    R, V = logits.shape
-    _i32("targets", targets, R)
-    _i32("status", status, 1)
-    new = dict(device=logits.device)
-    r = TokenLogprobs(torch.empty(R, **new), torch.empty(R, **new), torch.empty((R, max(top_k, 0)), dtype=torch.int32, **new),
-                      torch.empty((R, max(top_k, 0)), **new))
+    shape = logits.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError("token_logprobs: logits must be [R, V]")
+    R, V = shape
+    stride, side = logits.stride()
+    if side != 1 and V > 1:
+        raise ValueError("token_logprobs: the elements of a row must lie side by side")
+    _i32("targets", targets, (R,))
+    _i32("status", status, (1,))
+    k = max(top_k, 0)
+    f32 = torch.float32
+    r = TokenLogprobs(logits.new_empty((R,), dtype=f32), logits.new_empty((R,), dtype=f32), logits.new_empty((R, k), dtype=torch.int32),
+                      logits.new_empty((R, k), dtype=f32))
     check(
         lib.dgpt_token_logprobs(
-            logits.data_ptr(), _stride(logits, 0, V), targets.data_ptr(), temperature, r.logprob.data_ptr(), r.entropy.data_ptr(),
+            logits.data_ptr(), stride if R > 1 else V, targets.data_ptr(), temperature, r.logprob.data_ptr(), r.entropy.data_ptr(),
             r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), top_k, R, V, dtype_code(logits), _ptr(status), _stream(),
         )
     )
@@ -1317,13 +1325,15 @@ def kv_keep(
     src_start[s] + path[s, i] held before the call, i < count[s].  kv: layer 0's storage; path: int32 [B, T], T up to 256; src_start, dst_start,
     count: int32 [B]; layer_stride, token_stride (0: D): elements."""
     _here(src_start, dst_start, path, count, status)
-    if path.dim() != 2:
+    shape = path.shape
+    if len(shape) != 2:
         raise ValueError("kv_keep: path must be [B, T]")
-    B, T = path.shape
-    _i32("path", path, B, T)
-    for name, t in (("src_start", src_start), ("dst_start", dst_start), ("count", count)):
-        _i32(name, t, B)
-    _i32("status", status, 1)
+    B, T = shape
+    _i32("path", path, shape)
+    _i32("src_start", src_start, (B,))
+    _i32("dst_start", dst_start, (B,))
+    _i32("count", count, (B,))
+    _i32("status", status, (1,))
     if dtype not in _DT:
         raise TypeError(f"unsupported dtype {dtype}: float32 and bfloat16 are built")
     check(
