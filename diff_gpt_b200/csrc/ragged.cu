@@ -122,7 +122,7 @@ extern "C" int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv
   p.n_splits = n_splits;
   p.B = B; p.T = T; p.H = H; p.G = G; p.D = D;
   p.group = H / G;
-  p.rows_per_tile = p.tiles = 0;
+  p.rows_per_tile = p.tiles = p.tile_keys = 0;
   p.scale_log2 = scale * kLog2e;
   p.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -131,7 +131,8 @@ extern "C" int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv
     set_error("tree_attn: the tensor-core kernel does not cover dtype %d, head_dim %d with this layout", dtype, D);
     return DGPT_E_UNSUPPORTED;
   }
-  const int rc = tensor && impl != 1 ? tree_tc(p, st) : tree_simt(p, dtype, st);
+  const bool tc = tensor && impl != 1;
+  const int rc = tc ? tree_tc(p, st) : tree_simt(p, dtype, st);
   if (rc != DGPT_OK || n_splits == 1) return rc;
-  return tree_merge(p, dtype, st);
+  return tree_merge(p, tc ? 128 : 64, dtype, st);
 }

@@ -149,6 +149,7 @@ struct TreeProblem {
   float* part_o;    // [n_splits][B * T * H][D] and their sums' logarithms (base 2) [n_splits][B * T * H]; n_splits == 1: unused
   float* part_lse;
   int n_splits, B, T, H, G, D, group, rows_per_tile, tiles;  // group = H / G
+  int tile_keys;  // keys of a tile, as the pass that joins the splits counts them
   float scale_log2;
   int* status;
 
@@ -160,7 +161,7 @@ struct TreeProblem {
     nodes = n_nodes ? min(max(n_nodes[s], 0), T) : T;
     nodes = (int)min((long long)nodes, room - context);
   }
-  // Splits share the key tiles of `bn` keys evenly; the ones behind may get none.
+  // Splits share the key tiles of `bn` keys evenly; where there are fewer tiles, the splits behind them get none.
   __device__ bool item(unsigned i, int bn, RaggedItem& it) const {
     const unsigned a = i / (unsigned)n_splits, b = a / (unsigned)tiles, c = b / (unsigned)G;
     it.split = (int)(i - a * (unsigned)n_splits);
@@ -225,6 +226,6 @@ int packed_tc(const PackedProblem& p, int D, cudaStream_t st);
 bool tree_tc_supported(const TreeProblem& p, int dtype);
 int tree_tc(const TreeProblem& p, cudaStream_t st);
 // n_splits partials of every row into one (ragged_simt.cu)
-int tree_merge(const TreeProblem& p, int dtype, cudaStream_t st);
+int tree_merge(const TreeProblem& p, int tile_keys, int dtype, cudaStream_t st);
 
 }  // namespace dgpt

@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
   p.check((int)blockIdx.x, tid, kRgThreads);
   RaggedItem it;
   if constexpr (TREE) {
-    if (!p.item(blockIdx.x, kRgBN, it)) return;
+    if (!p.item(blockIdx.x, kRgBN, it) || (p.n_splits > 1 && it.key0 >= it.key1)) return;
   } else {
     const unsigned slot = blockIdx.x / (unsigned)p.H;
     typename P::Cursor cur;
@@ -261,13 +261,16 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeProblem p) {
   const long long row = at / p.H;
   const int s = (int)(row / p.T), t = (int)(row - (long long)s * p.T);
   if (p.n_nodes && t >= p.n_nodes[s]) return;
+  int context, nodes;
+  p.lengths(s, context, nodes);
+  const int splits = min(p.n_splits, (context + nodes + p.tile_keys - 1) / p.tile_keys);  // the ones behind have no keys
   float m = -INFINITY;
-  for (int i = lane; i < p.n_splits; i += 32) m = fmaxf(m, p.part_lse[i * n + at]);
+  for (int i = lane; i < splits; i += 32) m = fmaxf(m, p.part_lse[i * n + at]);
   m = warp_max(m);
   const float ref = m == -INFINITY ? 0.f : m;
   float acc[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f;  // columns lane * 4 .. (D <= 128)
   const bool mine = lane * 4 < p.D;
-  for (int i = 0; i < p.n_splits; ++i) {
+  for (int i = 0; i < splits; ++i) {
     const float lse = p.part_lse[i * n + at];
     if (lse == -INFINITY) continue;  // no key of this share is seen
     const float w = exp2f(lse - ref);
@@ -288,7 +291,9 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeProblem p) {
   for (int c = 0; c < 4; ++c) Io<T>::st(o + c, any ? acc[c] * inv : 0.f);
 }
 
-int tree_merge(const TreeProblem& p, int dtype, cudaStream_t st) {
+int tree_merge(const TreeProblem& full, int tile_keys, int dtype, cudaStream_t st) {
+  TreeProblem p = full;
+  p.tile_keys = tile_keys;
   const long long rows = (long long)p.B * p.T * p.H;
   const dim3 grid((unsigned)((rows + 7) / 8));
   if (dtype == DGPT_F32) launch_few(true, tree_merge_kernel<float>, grid, dim3(256), 0, st, p);

@@ -25,7 +25,7 @@ namespace dgpt {
 namespace tc {
 
 constexpr int kRtThreads = 512;
-constexpr int kRtSoftmaxRegs = 176, kRtOutputRegs = 88, kRtHelperRegs = 72;  // 2 x 176 + 88 + 72 = 4 x 128, the launch's share
+constexpr int kRtSoftmaxRegs = 168, kRtOutputRegs = 96, kRtHelperRegs = 80;  // 2 x 168 + 96 + 80 = 4 x 128, the launch's share
 constexpr int kRtRing = 8;                                                    // items between the warp that finds them and the last role that reads them
 
 struct RtItem {
@@ -71,6 +71,24 @@ __device__ __forceinline__ bool rt_item(const P& p, unsigned i, typename P::Curs
   x.tile0 = x.it.key0 / kBN;
   x.n = (x.it.key1 - x.it.key0 + kBN - 1) / kBN;
   return true;
+}
+
+// The rows of an item without keys: zeros.  (A share without keys of a tree's rows is left out by the pass that joins the shares.)
+template <class P, bool TREE>
+__device__ __forceinline__ void no_keys(const P& p, const RaggedItem& it, int d_head, int lane) {
+  if constexpr (TREE)
+    if (p.n_splits > 1) return;
+#pragma unroll 1
+  for (int r = 0; r < it.rows; ++r) {
+    __nv_bfloat16* o;
+    if constexpr (TREE) {
+      o = static_cast<__nv_bfloat16*>(p.o) + p.out_row(it, r) * p.o_rs + (long long)p.head(it, r) * d_head;
+    } else {
+      o = static_cast<__nv_bfloat16*>(p.o) + (long long)(it.row0 + r) * p.o_rs + (long long)it.h * p.o_hs;
+      if (p.lse && lane == 0) p.lse[(long long)(it.row0 + r) * p.H + it.h] = -INFINITY;
+    }
+    if (lane * 8 < d_head) *reinterpret_cast<uint4*>(o + lane * 8) = make_uint4(0u, 0u, 0u, 0u);
+  }
 }
 
 template <int D, class P, bool TREE>
@@ -212,22 +230,18 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
           }
         }
       };
-      auto take_all = [&](RtItem& y, unsigned& at, bool free) -> bool {  // the next item with keys, for the whole warp
-        for (;;) {
-          bool fine;
-          const bool there = take(y, at, fine);
-          ok = __all_sync(0xffffffffu, fine) != 0;
-          if (!ok || !there) return false;
-          ++at;
-          if (y.n > 0) return true;
-          if (free && lane == 0) done(at - 1);
-        }
+      auto take_all = [&](RtItem& y, unsigned& at) -> bool {  // the next item, for the whole warp
+        bool fine;
+        const bool there = take(y, at, fine);
+        ok = __all_sync(0xffffffffu, fine) != 0;
+        ++at;
+        return ok && there;
       };
       // K runs one tile ahead of V, across items too
       RtItem y;  // item of the K cursor
       unsigned ahead = 0u;
       int kj = 0;
-      bool more = take_all(y, ahead, false);
+      bool more = take_all(y, ahead);
       auto load_k = [&]() {
         if (kj == 0) {
           if (items > 0) ok = wait(iQF, (items - 1) & 1u);  // the last S of the item before is done
@@ -253,11 +267,11 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         ++kn;
         if (++kj == y.n) {
           kj = 0;
-          more = take_all(y, ahead, false);
+          more = take_all(y, ahead);
         }
       };
       if (more) load_k();
-      while (ok && take_all(x, taken, true)) {
+      while (ok && take_all(x, taken)) {
         for (int j = 0; ok && j < x.n; ++j) {
           if (more) load_k();
           if (!ok) break;
@@ -284,15 +298,8 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         int sj = 0;
         unsigned items = 0u, sg = 0u, g = 0u, ahead = 0u;
         bool ok = true;
-        auto take_one = [&](RtItem& z, unsigned& at, bool free) -> bool {  // the next item with keys
-          for (;;) {
-            if (!take(z, at, ok)) return false;
-            ++at;
-            if (z.n > 0) return true;
-            if (free) done(at - 1);
-          }
-        };
-        bool more = take_one(y, ahead, false);
+        auto take_one = [&](RtItem& z, unsigned& at) -> bool { return take(z, at++, ok); };
+        bool more = take_one(y, ahead);
         auto issue_s = [&]() {  // S(sg & 1) = Q K(sg % 3)^T
           if (sj == 0) {
             ok = wait_or_abort(bar(iQ), items & 1u, abort_flag);
@@ -309,12 +316,12 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
           if (++sj == y.n) {
             umma_commit(bar(iQF));  // Q may be overwritten
             sj = 0;
-            more = take_one(y, ahead, false);
+            more = take_one(y, ahead);
           }
         };
         for (int i = 0; i < 2 && ok && more; ++i) issue_s();
         unsigned outs = 0u;  // items whose first P V has been issued
-        while (ok && take_one(x, taken, true)) {
+        while (ok && take_one(x, taken)) {
           for (int j = 0; ok && j < x.n; ++j, ++g) {
             const unsigned buf = g & 1u, ph = (g >> 1) & 1u;
             // P_g is complete when every row has arrived; by then every row has also consumed S_g
@@ -339,7 +346,9 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
     } else if (warp == 14) {
       // ================= items =================
       // An item is asked for when it will be wanted soon and not before, so that none waits behind a long one while another SM idles: beside
-      // the oldest unfinished item there is one more, or as many as make up three key tiles.
+      // the oldest unfinished item there is one more, or as many as make up three key tiles.  (No fewer: the issuer's score cursor is two
+      // tiles ahead of its products and waits for the next item before it goes on, the loader's K cursor one.  The items that they hold
+      // unfinished then have at most two tiles behind the oldest one's, so the next one is always on its way.  Items without a key never get here.)
       typename P::Cursor cursor;
       unsigned at = 0u, freed = 0u, asked = 0u, cta = blockIdx.x;  // items handed out, items finished
       int ahead = 0;                                               // key tiles of those behind the oldest unfinished one
@@ -363,7 +372,10 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         ++at;
       };
       while (ok && more) {
-        if (rt_item<P, TREE>(p, cta, cursor, x, lane)) push();
+        if (rt_item<P, TREE>(p, cta, cursor, x, lane)) {
+          if (x.n > 0) push();
+          else no_keys<P, TREE>(p, x.it, d_head, lane);
+        }
         make_room(false);
         if (!ok) break;
         if (lane == 0) ask_for_cta(smem_u32(answer), bar(iC));
@@ -389,6 +401,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRtOutputRegs));
     const int quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t o_addr = tmem + ((uint32_t)(quarter * 32) << 16) + kOCol;
+    uint8_t* stage = ring + kRtRing * 64 + quarter * 4096;
     unsigned items = 0u, g = 0u;
     bool ok = true;
     for (;; ++taken) {
@@ -398,85 +411,92 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       if (!ok || !there) break;
       __syncwarp();
       if (lane == 0) done(taken);
-      const bool row_ok = row < x.it.rows;
-      float l = 0.f, m = -INFINITY;
-      uint32_t packed[D / 2];
-      float* part = nullptr;
-      long long at = 0;
-      if constexpr (TREE) {
-        if (p.n_splits > 1) {
-          if (row_ok) at = ((long long)x.it.split * p.B * p.T + p.out_row(x.it, row)) * p.H + p.head(x.it, row);
-          part = p.part_o + at * d_head;
+      const int rows = min(max(x.it.rows - quarter * 32, 0), 32);  // of this warp
+      char* mine = nullptr;                                         // where this thread's row goes
+      float* mine_lse = nullptr;
+      bool part = false;
+      if constexpr (TREE) part = p.n_splits > 1;
+      if (lane < rows) {
+        if constexpr (TREE) {
+          const long long at = p.out_row(x.it, row);
+          const int h = p.head(x.it, row);
+          if (part) {
+            const long long slot = ((long long)x.it.split * p.B * p.T + at) * p.H + h;
+            mine = reinterpret_cast<char*>(p.part_o + slot * d_head);
+            mine_lse = p.part_lse + slot;
+          } else {
+            mine = reinterpret_cast<char*>(static_cast<__nv_bfloat16*>(p.o) + at * p.o_rs + (long long)h * d_head);
+          }
+        } else {
+          const long long at = x.it.row0 + row;
+          mine = reinterpret_cast<char*>(static_cast<__nv_bfloat16*>(p.o) + at * p.o_rs + (long long)x.it.h * p.o_hs);
+          if (p.lse) mine_lse = p.lse + at * p.H + x.it.h;
         }
       }
-      if (x.n > 0) {
-        const int slot = (int)(items & 1u);
-        ok = __all_sync(0xffffffffu, wait_asleep(iL + slot, (items >> 1) & 1u)) != 0;
-        if (!ok) break;
-        const float* sum = sums + slot * 3 * kBM;
-        l = sum[row] + sum[kBM + row];
-        m = sum[2 * kBM + row];
-        mbar_arrive(bar(iLF + slot));
-        const unsigned last = g + (unsigned)x.n - 1u;
-        ok = __all_sync(0xffffffffu, wait_or_abort(bar(iO + (int)(last & 1u)), (last >> 1) & 1u, abort_flag)) != 0;
-        if (!ok) break;
-        tc_fence_after();
-        g += (unsigned)x.n;
-        ++items;
-      }
+      const int slot = (int)(items & 1u);
+      ok = __all_sync(0xffffffffu, wait_asleep(iL + slot, (items >> 1) & 1u)) != 0;
+      if (!ok) break;
+      const float* sum = sums + slot * 3 * kBM;
+      const float l = sum[row] + sum[kBM + row], m = sum[2 * kBM + row];
+      mbar_arrive(bar(iLF + slot));
+      const unsigned last = g + (unsigned)x.n - 1u;
+      ok = __all_sync(0xffffffffu, wait_or_abort(bar(iO + (int)(last & 1u)), (last >> 1) & 1u, abort_flag)) != 0;
+      if (!ok) break;
+      tc_fence_after();
+      g += (unsigned)x.n;
+      ++items;
       const bool any = !(l <= 0.f);  // a row with a score that is not a number keeps saying so
       const float inv = any ? 1.f / l : 0.f;
+      // 128 bytes of every row at a time go through shared memory, so that eight lanes store a row's 128 bytes and not each lane 16 of its own
+      // (an item of 128 rows of 128 bf16 numbers: 4000 cycles so, 1000 now)
+      auto store = [&](const uint32_t* w, int col, int bytes) {  // w: this row's words; col, bytes: where they go in the row
+        __syncwarp();
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        float v[32];
-        if (x.n > 0) {  // warp-uniform
-          tmem_ld32(o_addr + c * 32, v);
-        } else {
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+        __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + (lane >> 3), c = lane & 7;
+          char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), r));
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
+          if (r < rows && c * 16 < bytes) *reinterpret_cast<uint4*>(to + col + c * 16) = v;
         }
-        if (!any) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0.f;
-        }
-        if constexpr (TREE) {
+      };
+      if (rows > 0) {  // warp-uniform
+        const int passes = part ? d_head / 32 : (d_head + 63) / 64;
+#pragma unroll 1
+        for (int c = 0; c < passes; ++c) {
+          uint32_t w[32];
+          float v[32];
           if (part) {
-            if (row_ok && c * 32 < d_head) {
+            tmem_ld32(o_addr + c * 32, v);
 #pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<float4*>(part + c * 32 + i) = make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
+            for (int i = 0; i < 32; ++i) w[i] = any ? __float_as_uint(v[i] * inv) : 0u;
+          } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              tmem_ld32(o_addr + c * 64 + u * 32, v);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i] * inv, v[2 * i + 1] * inv);
+                w[u * 16 + i] = any ? *reinterpret_cast<const uint32_t*>(&h) : 0u;
+              }
             }
-            continue;
           }
+          if (c == passes - 1) {
+            tc_fence_before();
+            mbar_arrive(bar(iOF));
+          }
+          store(w, c * 128, part ? 128 : min(128, d_head * 2 - c * 128));
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i] * inv, v[2 * i + 1] * inv);
-          packed[c * 16 + i] = *reinterpret_cast<const uint32_t*>(&h);
+        if (mine_lse) {
+          const float base2 = m + log2f(l);
+          *mine_lse = !any ? -INFINITY : TREE ? base2 : base2 * kLn2;
         }
-      }
-      if (x.n > 0) {
-        tc_fence_before();
+      } else {
         mbar_arrive(bar(iOF));
       }
-      if (!row_ok) continue;
-      if constexpr (TREE) {
-        if (part) {
-          p.part_lse[at] = any ? m + log2f(l) : -INFINITY;
-          continue;
-        }
-      }
-      __nv_bfloat16* dst;
-      if constexpr (TREE) {
-        dst = static_cast<__nv_bfloat16*>(p.o) + p.out_row(x.it, row) * p.o_rs + (long long)p.head(x.it, row) * d_head;
-      } else {
-        dst = static_cast<__nv_bfloat16*>(p.o) + (long long)(x.it.row0 + row) * p.o_rs + (long long)x.it.h * p.o_hs;
-        if (p.lse) p.lse[(long long)(x.it.row0 + row) * p.H + x.it.h] = any ? (m + log2f(l)) * kLn2 : -INFINITY;
-      }
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c)
-        if (c * 8 < d_head)
-          *reinterpret_cast<uint4*>(dst + c * 8) = make_uint4(packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
     }
     if (!ok && lane == 0 && p.status) atomicOr(p.status, 2);
   } else {
@@ -517,7 +537,6 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       const int n = x.n, rows = x.it.rows, clear = x.it.clear;
       // Key from which value rows may hold anything: the end of the sequence's keys.
       const int held_end = TREE ? x.it.key1 : x.it.held;
-      if (n == 0) continue;
       float m = -INFINITY, l = 0.f;
       int t0 = x.tile0 * kBN;
       for (int j = 0; j < n; ++j, ++g, t0 += kBN) {
@@ -699,7 +718,7 @@ static int ragged_tc_go(const TcMaps& maps, const P& p, long long items, int d_h
     set_error("ragged attention: too many rows");
     return DGPT_E_ARG;
   }
-  size_t smem = (size_t)6 * (D / 64) * kBN * 128 + 48 * 8 + 4 * kBM * 8 + 6 * kBM * 4 + kRtRing * 64 + 1024;
+  size_t smem = (size_t)6 * (D / 64) * kBN * 128 + 48 * 8 + 4 * kBM * 8 + 6 * kBM * 4 + kRtRing * 64 + 4 * 4096 + 1024;
   if (smem < 120 * 1024) smem = 120 * 1024;  // one CTA owns an SM: it takes all 512 TMEM columns
   auto kernel = ragged_tc_kernel<D, P, TREE>;
   cudaError_t e = cudaSuccess;

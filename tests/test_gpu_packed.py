@@ -137,6 +137,14 @@ def test_rising_scores(D, dtype):
     check_rows(out[:, 0].cpu(), lse[:, 0].cpu(), want, D, n, dtype, dtype == BF)
 
 
+@pytest.mark.parametrize("impl", [0, 1])
+@pytest.mark.parametrize("D,dtype", [(64, BF), (128, BF), (16, F32)])
+def test_many_prompts_without_keys(D, dtype, impl):
+    """More tiles than the GPU holds at a time, most of whose queries see no key, between ones with up to nine tiles of them."""
+    lens = [130, 5, 1, 260, 64] * 40
+    run(lens, 2, 2, D, dtype, impl, past=[-200, -5, 1100, -300, 0] * 40, seed=9)
+
+
 @pytest.mark.parametrize("D,dtype", [(128, BF), (16, F32)])
 def test_repeats_graphs_and_streams(D, dtype):
     """The same bits from call to call, from a graph that is replayed over new numbers, and on another stream."""

@@ -122,6 +122,14 @@ def test_splits(n_splits, D, dtype, impl):
 
 
 @pytest.mark.parametrize("impl", [0, 1])
+@pytest.mark.parametrize("n_splits", [5, 16, 64])
+@pytest.mark.parametrize("D,dtype", [(64, BF), (128, BF), (16, F32)])
+def test_many_shares_without_keys(n_splits, D, dtype, impl):
+    """More items than the GPU holds at a time, most of them without a key, between ones with up to nine tiles."""
+    run([100, 0, 1100, 300, 5, 130] * 7, [3, 1, 2, 3, 1, 3] * 7, 3, 4, 2, D, dtype, impl, n_splits=n_splits, seed=11)
+
+
+@pytest.mark.parametrize("impl", [0, 1])
 @pytest.mark.parametrize("n_splits", [1, 3])
 @pytest.mark.parametrize("D,dtype", [(64, BF), (128, BF), (16, F32)])
 def test_masks(D, dtype, n_splits, impl):
