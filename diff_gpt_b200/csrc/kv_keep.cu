@@ -1,8 +1,10 @@
 // Rows of accepted drafts move to where they belong in the cache: for every sequence s, layer, head, and for keys and values alike,
 //   slot dst[s] + i  <-  slot src[s] + path[s][i],   i < count[s].
-// A copy of rows, bound by memory or, where few rows move, by the launch.  A CTA owns 32 columns of 16 bytes of one sequence and all of
-// its rows, reads every row before it writes the first, and columns do not mix: source and target may overlap in any way.  A thread
-// keeps its rows in registers (up to 2, 8 or 32 of them, by the most rows that a sequence may move).
+// A copy of rows, bound by memory or, where few rows move, by the launch and the loads that depend on one another: count, path, page, row.
+// A CTA owns 256 columns of 16 bytes of one sequence and all of its rows; it works out once where the rows lie and then reads every row of a
+// column before it writes the first, and columns do not mix: source and target may overlap in any way.  Up to 16 rows are one thread's per
+// column, in registers; more are shared by 32 threads, which wait for one another between reading and writing.
+// (Eight threads per column in all cases, each finding its rows' places itself: 192 sequences, 12 layers, 12 heads of 64, 5 rows each, 95 us; so, 22.)
 #include "common.cuh"
 
 namespace dgpt {
@@ -16,55 +18,73 @@ struct KeepParams {
   int* status;
 };
 
-constexpr int kKeepCols = 32, kKeepRows = 8;
+constexpr int kKeepCols = 256, kKeepOwn = 16, kKeepMost = 256;
 
-template <int RPT>
-__global__ void __launch_bounds__(kKeepCols * kKeepRows) kv_keep_kernel(const KeepParams p, const unsigned blocks_per_seq) {
-  const int s = (int)(blockIdx.x / blocks_per_seq);
-  const long long col = (long long)(blockIdx.x % blocks_per_seq) * kKeepCols + (threadIdx.x & 31);
-  const int row0 = threadIdx.x >> 5;
+template <bool MANY>
+__global__ void __launch_bounds__(kKeepCols) kv_keep_kernel(const KeepParams p, const unsigned blocks_per_seq) {
+  __shared__ long long from[MANY ? kKeepMost : kKeepOwn], to[MANY ? kKeepMost : kKeepOwn];  // bytes from a column's base, or -1
+  const int s = (int)(blockIdx.x / blocks_per_seq), tid = threadIdx.x;
+  const unsigned block = blockIdx.x % blocks_per_seq;
   const int asked = p.count[s], n = min(max(asked, 0), p.T);
-  bool bad = asked != n;
-  const bool on = col < p.columns;
-  const int vec = (int)(col % p.vecs);
-  const long long lkh = col / p.vecs, lk = lkh / p.H;
-  const int h = (int)(lkh - lk * p.H), kind = (int)(lk % p.kinds);
-  char* base = static_cast<char*>(kind == 0 ? p.kv.k : p.kv.v) + (lk / p.kinds) * p.layer_bytes + (long long)h * p.head_bytes + (long long)vec * 16;
   const int* table = p.kv.page_table ? p.kv.page_table + (long long)s * p.kv.max_pages : nullptr;
-  const long long room = (long long)(table ? p.kv.max_pages : 1) * p.kv.page_tokens;
-  auto place = [&](long long slot, char*& at) {  // false: no such slot, or its page is none
-    if (slot < 0 || slot >= room) return false;
-    const int lp = (int)(slot / p.kv.page_tokens), in = (int)(slot - (long long)lp * p.kv.page_tokens);
-    const long long pg = table ? (long long)table[lp] : s;
-    if (pg < 0 || (p.kv.n_pages > 0 && pg >= p.kv.n_pages)) return false;
-    at = base + pg * p.page_bytes + (long long)in * p.token_bytes;
-    return true;
+  bool bad = asked != n;
+  if (tid < n) {
+    const long long room = (long long)(table ? p.kv.max_pages : 1) * p.kv.page_tokens;
+    auto place = [&](long long slot) -> long long {  // -1: no such slot, or its page is none
+      if (slot < 0 || slot >= room) return -1;
+      const unsigned lp = (unsigned)slot / (unsigned)p.kv.page_tokens, in = (unsigned)slot - lp * (unsigned)p.kv.page_tokens;
+      const long long pg = table ? (long long)table[lp] : s;
+      if (pg < 0 || (p.kv.n_pages > 0 && pg >= p.kv.n_pages)) return -1;
+      return pg * p.page_bytes + (long long)in * p.token_bytes;
+    };
+    const int node = p.path[(long long)s * p.T + tid];
+    const long long a = node < 0 ? -1 : place((long long)p.src[s] + node), b = place((long long)p.dst[s] + tid);
+    from[tid] = a < 0 || b < 0 ? -1 : a;
+    to[tid] = b;
+    bad |= a < 0 || b < 0;
+  }
+  if (bad && block == 0 && p.status) atomicOr(p.status, 1);
+  __syncthreads();
+  auto base = [&](long long col) -> char* {
+    const int vec = (int)(col % p.vecs);
+    const long long lkh = col / p.vecs, lk = lkh / p.H;
+    return static_cast<char*>(p.kinds > 1 && (lk & 1) ? p.kv.v : p.kv.k) + (p.kinds > 1 ? lk >> 1 : lk) * p.layer_bytes +
+           (lkh - lk * p.H) * p.head_bytes + (long long)vec * 16;
   };
-  const int* path = p.path + (long long)s * p.T;
-  uint4 x[RPT];
-  char* to[RPT];
+  const long long col0 = (long long)block * kKeepCols;
+  if (!MANY || n <= kKeepOwn) {
+    if (col0 + tid >= p.columns) return;
+    char* at = base(col0 + tid);
+    uint4 x[kKeepOwn];
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    const int row = row0 + i * kKeepRows;
-    to[i] = nullptr;
-    if (row < n) {
-      char *from, *at;
-      const int node = path[row];
-      if (node >= 0 && place((long long)p.src[s] + node, from) && place((long long)p.dst[s] + row, at)) {
-        if (on) {
-          x[i] = *reinterpret_cast<const uint4*>(from);
-          to[i] = at;
-        }
-      } else {
-        bad = true;
+    for (int i = 0; i < kKeepOwn; ++i)
+      if (i < n && from[i] >= 0) x[i] = *reinterpret_cast<const uint4*>(at + from[i]);
+#pragma unroll
+    for (int i = 0; i < kKeepOwn; ++i)
+      if (i < n && from[i] >= 0) *reinterpret_cast<uint4*>(at + to[i]) = x[i];
+    return;
+  }
+  if constexpr (MANY) {
+    constexpr int kRows = kKeepMost / 32;
+    const int row0 = tid >> 3;
+    for (int c = 0; c < kKeepCols && col0 + c < p.columns; c += 8) {
+      const long long col = col0 + c + (tid & 7);
+      const bool on = col < p.columns;
+      char* at = on ? base(col) : nullptr;
+      uint4 x[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int row = row0 + i * 32;
+        if (on && row < n && from[row] >= 0) x[i] = *reinterpret_cast<const uint4*>(at + from[row]);
+      }
+      __syncthreads();  // every row of these columns has been read
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int row = row0 + i * 32;
+        if (on && row < n && from[row] >= 0) *reinterpret_cast<uint4*>(at + to[row]) = x[i];
       }
     }
   }
-  __syncthreads();  // every row of these columns has been read
-#pragma unroll
-  for (int i = 0; i < RPT; ++i)
-    if (to[i]) *reinterpret_cast<uint4*>(to[i]) = x[i];
-  if (bad && p.status && (threadIdx.x & 31) == 0) atomicOr(p.status, 1);
 }
 
 }  // namespace dgpt
@@ -107,9 +127,7 @@ extern "C" int dgpt_kv_keep(const dgpt_kv_layout* kv, int64_t kv_token_stride, c
   const long long per = (p.columns + kKeepCols - 1) / kKeepCols, blocks = per * B;
   DGPT_REQUIRE(blocks <= 0x7fffffffll, "kv_keep: too many rows");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)blocks), block(kKeepCols * kKeepRows);
-  if (T <= 2 * kKeepRows) kv_keep_kernel<2><<<grid, block, 0, st>>>(p, (unsigned)per);
-  else if (T <= 8 * kKeepRows) kv_keep_kernel<8><<<grid, block, 0, st>>>(p, (unsigned)per);
-  else kv_keep_kernel<32><<<grid, block, 0, st>>>(p, (unsigned)per);
+  if (T <= kKeepOwn) kv_keep_kernel<false><<<(unsigned)blocks, kKeepCols, 0, st>>>(p, (unsigned)per);
+  else kv_keep_kernel<true><<<(unsigned)blocks, kKeepCols, 0, st>>>(p, (unsigned)per);
   return launch_status("kv_keep");
 }

@@ -1,9 +1,10 @@
 // Log probability of a given token per row of logits, the entropy of the row's distribution, and its most probable tokens.
 //   z = logits / temperature,  lse = log sum_j e^(z_j):   logprob = z_target - lse,   entropy = lse - sum_j p_j z_j,   p_j = e^(z_j - lse)
-// in one pass over the row.  With x_j = (logit_j - m) c, m the running maximum and c = log2(e) / temperature, a thread carries s = sum 2^x
-// and w = sum x 2^x; then lse = m / temperature + ln s and entropy = (log2 s - w / s) ln 2, and when m moves, by d = (old - new) c, s <- s 2^d and
-// w <- (w + d s) 2^d.  (The difference first, then the factor: m c alone would be rounded, which logits of the type's lowest value turn into more than
-// any exponent holds.)
+// in one pass over the row.  With c = log2(e) / temperature, M = m c rounded, m the running maximum, and x_j = logit_j c - M (one fma), a thread
+// carries s = sum 2^x and w = sum x 2^x; then lse = (M + log2 s) ln 2 and entropy = (log2 s - w / s) ln 2, and when M moves by d = old - new,
+// s <- s 2^d and w <- (w + d s) 2^d.  How M was rounded cancels out, unless it is so large that the rounding itself outgrows an exponent (logits of
+// the type's lowest value throughout, temperatures next to 0): M is kept within 2^30, and a row whose maximum lies beyond is summed once more as
+// (logit - m) c, two roundings that need no M.
 //
 // The top tokens come from the same pass.  A token's key is its logit, made an unsigned number of the same order, above the
 // complement of its index: keys differ, and ties go to the lower index.  Each thread knows the vector with its largest logit; the k-th
@@ -11,15 +12,20 @@
 // a few dozen, all read by the few threads whose own maximum reaches it.  Those threads' vectors are read again (from L2, one in twenty or so of the row)
 // and the tokens found are ranked by counting.
 //
-// A cluster of 1 to 8 CTAs shares a row where rows are few; its first CTA joins the others' sums and lists through distributed shared memory.
-// What bounds it: one read of the logits.
+// Eight warps of a CTA stream a row, two more finish a row each (sums, top tokens, outputs) while the eight are at the next ones; rows are handed
+// over through two buffers.  A cluster of 1 to 8 CTAs shares a row where rows are few; its first CTA joins the others' sums and lists through distributed shared memory.
+// What bounds it: one read of the logits, then the exponentials (16 a clock and SM: three quarters of a read's time in bf16) and the instructions
+// around them, which is why pairs share them (fma, add, max) and the next vectors are on their way while these are worked on.  4096 rows of
+// 32001 bf16 logits: 60 us without top tokens, 75 with 5, 93 with 20; their reading alone takes 40.5.  (A CTA of 256 threads per row whose every warp goes through
+// every phase: 132 with 20.)
 #include "common.cuh"
 
 namespace dgpt {
 
 constexpr int kLpMost = 32;       // most top tokens
+constexpr float kLpBig = 1073741824.f;  // 2^30: M is kept within it
 constexpr float kLpFar = -1e4f;  // an exponent whose power is 0: keeps 0 times infinity out of the sums
-constexpr int kLpFound = 1024;    // tokens found above the bound that are ranked at once
+constexpr int kLpFound = 512;     // tokens found above the bound that are ranked at once
 
 __device__ __forceinline__ uint32_t lp_order(float v) {
   const uint32_t u = __float_as_uint(v + 0.f);  // -0 is 0
@@ -48,7 +54,7 @@ __device__ __forceinline__ unsigned long long lp_ld_u64(uint32_t a) {
   return v;
 }
 __device__ __forceinline__ void lp_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
 }
 __device__ __forceinline__ float lp_exp2(float x) {
   float y;
@@ -56,17 +62,44 @@ __device__ __forceinline__ float lp_exp2(float x) {
   return y;
 }
 
-struct LpStat {  // sums against the largest logit m met; -inf: nothing yet
-  float m, s, w;
+struct LpStat {  // largest logit m, sums against M (lp_ref(m)); m = -inf: nothing yet
+  float m, M, s, w;
 };
-__device__ __forceinline__ LpStat lp_join(const LpStat& a, const LpStat& b, float c) {
+__device__ __forceinline__ float lp_ref(float m, float c) { return fminf(fmaxf(m * c, -kLpBig), kLpBig); }
+__device__ __forceinline__ LpStat lp_join(const LpStat& a, const LpStat& b) {
   LpStat r;
   r.m = fmaxf(a.m, b.m);
-  const float ref = r.m == -INFINITY ? 0.f : r.m;
-  const float da = fmaxf((a.m - ref) * c, kLpFar), db = fmaxf((b.m - ref) * c, kLpFar);  // m = -inf: the sums are 0 (or not numbers)
+  r.M = fmaxf(a.M, b.M);
+  const float da = fmaxf(a.M - r.M, kLpFar), db = fmaxf(b.M - r.M, kLpFar);
   const float fa = lp_exp2(da), fb = lp_exp2(db);
   r.s = a.s * fa + b.s * fb;
   r.w = (a.w + a.s * da) * fa + (b.w + b.s * db) * fb;
+  return r;
+}
+// All lanes' sums, the same in every lane: over to the largest maximum, then added.
+__device__ __forceinline__ LpStat lp_warp_join(const LpStat& a) {
+  LpStat r;
+  r.m = warp_max(a.m);
+  r.M = warp_max(a.M);
+  const float d = fmaxf(a.M - r.M, kLpFar), f = lp_exp2(d);
+  r.s = warp_sum(a.s * f);
+  r.w = warp_sum((a.w + a.s * d) * f);
+  return r;
+}
+__device__ __forceinline__ uint64_t lp_pack(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void lp_unpack(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t lp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t lp_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 
@@ -92,222 +125,413 @@ struct LpRow {
     n = (off + V + VEC - 1) / VEC;
   }
   __device__ int first(int vec) const { return vec * VEC - off; }  // index of a vector's first element
-  __device__ bool whole(int vec) const { return first(vec) >= 0 && first(vec) + VEC <= V; }
-  __device__ void load(int vec, float (&x)[VEC]) const {
-    if (whole(vec)) {
-      unpack16<T>(__ldg(reinterpret_cast<const uint4*>(row + first(vec))), x);
-    } else {
+  // Vectors [whole0(), whole1()) lie in the row from end to end; of the others, at most one on either side, `edge` gives the ones that are.
+  __device__ int whole0() const { return off > 0 ? 1 : 0; }
+  __device__ int whole1() const { return max((off + V) / VEC, whole0()); }
+  __device__ bool edge(int side, int& vec) const {
+    vec = side == 0 ? 0 : n - 1;
+    return side == 0 ? off > 0 : (off + V) % VEC != 0 && !(n == 1 && off > 0);
+  }
+  __device__ uint4 inner(int vec) const { return __ldg(reinterpret_cast<const uint4*>(row - off) + vec); }
+  static constexpr uint32_t kNothing = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;  // -inf: adds nothing to the sums
+  // Any vector, with nothing where it is outside the row.  (It is read whole: memory is allocated in larger pieces than 16 bytes.  Element by element
+  // the two edges of a row of 32001 cost a tenth of its time.)
+  __device__ uint4 raw(int vec) const {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(row - off) + vec);
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int j = first(vec) + i;
-        x[i] = j >= 0 && j < V ? Io<T>::ld(row + j) : -INFINITY;  // adds nothing to the sums
+    for (int i = 0; i < VEC; ++i) {
+      const int j = first(vec) + i;
+      if (j >= 0 && j < V) continue;
+      if constexpr (sizeof(T) == 2) {
+        w[i >> 1] = (i & 1) ? (w[i >> 1] & 0xffffu) | (kNothing << 16) : (w[i >> 1] & 0xffff0000u) | (kNothing & 0xffffu);
+      } else {
+        w[i] = kNothing;
       }
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 
-template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LpParams p, const int cluster) {
-  constexpr int VEC = Io<T>::kVec16, WARPS = THREADS / 32, UNROLL = 4;
-  __shared__ unsigned long long bound[WARPS][32];
-  __shared__ unsigned long long found[kLpFound];
-  __shared__ unsigned long long best[8 * kLpMost];  // this CTA's top k in order; in the first CTA then those of all
-  __shared__ unsigned long long limit;
-  __shared__ int n_found, n_owners;
-  __shared__ short owners[THREADS];
-  __shared__ float stat[WARPS][3];
-  __shared__ float mine[3];
+// Largest number of some vectors (NaN only where there is nothing else).
+template <int N>
+__device__ __forceinline__ float lp_top(const uint4 (&v)[N], __nv_bfloat16) {
+  auto h = [](uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  };
+  uint32_t m = h(h(v[0].x, v[0].y), h(v[0].z, v[0].w));
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = h(m, h(h(v[i].x, v[i].y), h(v[i].z, v[i].w)));
+  return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+}
+template <int N>
+__device__ __forceinline__ float lp_top(const uint4 (&v)[N], float) {
+  float m = __uint_as_float(v[0].x);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    m = fmaxf(fmaxf(fmaxf(m, __uint_as_float(v[i].x)), __uint_as_float(v[i].y)), fmaxf(__uint_as_float(v[i].z), __uint_as_float(v[i].w)));
+  return m;
+}
+// Pairs of a vector, raised to -1e30 (a -inf times its power 0 is not a number).
+__device__ __forceinline__ void lp_pairs(const uint4& v, uint64_t (&p)[4], __nv_bfloat16) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w[i]), "r"(0xf149f149u));  // -9.95e29 twice
+    p[i] = lp_pack(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
+  }
+}
+__device__ __forceinline__ void lp_pairs(const uint4& v, uint64_t (&p)[2], float) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("max.NaN.f32 %0, %1, %2;" : "=f"(x[i]) : "f"(__uint_as_float(w[i])), "f"(-1e30f));
+  p[0] = lp_pack(x[0], x[1]);
+  p[1] = lp_pack(x[2], x[3]);
+}
+
+// The k largest of n keys (all different, n <= kLpFound) in order, for one warp: a key's place is the number of larger ones.
+__device__ __forceinline__ void lp_rank(unsigned long long* keys, int n, unsigned long long* best, int k, int lane) {
+  if (lane < 8) keys[n + lane] = 0ull;  // up to whole rounds
+  if (lane < k) best[lane] = 0ull;
+  __syncwarp();
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const unsigned long long a = i0 + lane < n ? keys[i0 + lane] : 0ull, b = i0 + 32 + lane < n ? keys[i0 + 32 + lane] : 0ull;
+    int over_a = 0, over_b = 0;
+    for (int j = 0; j < n; j += 8) {
+#pragma unroll
+      for (int u = 0; u < 8; u += 2) {
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(keys + j + u);
+        over_a += (o.x > a) + (o.y > a);
+        over_b += (o.x > b) + (o.y > b);
+      }
+    }
+    if (a != 0ull && over_a < k) best[over_a] = a;
+    if (b != 0ull && over_b < k) best[over_b] = b;
+  }
+  __syncwarp();
+}
+
+template <int BAR, int THREADS>
+__device__ __forceinline__ void lp_bar_sync(int which) { asm volatile("bar.sync %0, %1;" ::"r"(BAR + which), "n"(THREADS) : "memory"); }
+template <int BAR, int THREADS>
+__device__ __forceinline__ void lp_bar_arrive(int which) { asm volatile("bar.arrive %0, %1;" ::"r"(BAR + which), "n"(THREADS) : "memory"); }
+
+template <typename T, int STREAM, int ENDS, int CTAS, int UNROLL>
+__global__ void __launch_bounds__(STREAM + 32 * ENDS, CTAS) token_logprobs_kernel(const LpParams p, const int log_cluster) {
+  constexpr int VEC = Io<T>::kVec16, WARPS = STREAM / 32;
+  constexpr int kFull = 1, kFree = 3;  // named barriers, one per buffer
+  constexpr int kStream = 5;
+  __shared__ unsigned long long lows[2][STREAM];                        // what the key of each streaming thread's largest logit is at least
+  __shared__ __align__(16) unsigned long long groups[32];
+  __shared__ unsigned char owners[WARPS][32];
+  __shared__ __align__(16) unsigned long long founds[2][kLpFound + 8];  // tokens that reach the bound
+  __shared__ int mets[2];                                               // how many do (there may be more than there is room for)
+  __shared__ unsigned long long limits[2];                              // the bound
+  __shared__ unsigned long long bests[2][kLpMost];                      // the top k in order
+  __shared__ LpStat stat[2][WARPS], mine;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r = (int)(blockIdx.x / (unsigned)cluster), rank = (int)(blockIdx.x % (unsigned)cluster);
-  const LpRow<T> row(static_cast<const T*>(p.logits) + (long long)r * p.stride, p.V);
-  const int v0 = (int)((long long)row.n * rank / cluster), v1 = (int)((long long)row.n * (rank + 1) / cluster);
+  const int cluster = 1 << log_cluster;
+  const int rank = (int)(blockIdx.x & (unsigned)(cluster - 1)), step = (int)(gridDim.x >> log_cluster), row0 = (int)(blockIdx.x >> log_cluster);
+  auto row_of = [&](int r) { return LpRow<T>(static_cast<const T*>(p.logits) + (long long)r * p.stride, p.V); };
+  // Whole vectors [part(rank), part(rank + 1)) are this CTA's; the row's partial ones are the first and the last CTA's (threads 0 and 1).
+  auto part = [&](const LpRow<T>& w, int i) { return w.whole0() + (int)(((unsigned)(w.whole1() - w.whole0()) * (unsigned)i) >> log_cluster); };
 
-  float top = -INFINITY;  // this thread's largest logit, and the vector it was first met in
-  int top_vec = -1;
-  LpStat a = {-INFINITY, 0.f, 0.f};
-  for (int base = v0 + tid; base < v1; base += THREADS * UNROLL) {
-    float x[UNROLL][VEC];
-    float vm[UNROLL];
+  // A lane's vector: its tokens that reach the bound (`least`: the bound's logit, NaN for a bound of 0: nothing is below it).
+  auto look = [&](const LpRow<T>& row, int vec, const uint4& v, unsigned long long lim, float least, int b) {
+    float x[VEC];
+    unpack16<T>(v, x);
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int vec = base + u * THREADS;
-      if (vec < v1) {
-        row.load(vec, x[u]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) x[u][i] = -INFINITY;
-      }
+    for (int e = 0; e < VEC; ++e) {
+      if (x[e] < least) continue;
+      const int j = row.first(vec) + e;
+      if (j < 0 || j >= p.V) continue;
+      const unsigned long long key = lp_key(x[e], j);
+      if (key < lim) continue;
+      const int place = atomicAdd(&mets[b], 1);
+      if (place < kLpFound) founds[b][place] = key;
     }
+  };
+  if (tid < 2) mets[tid] = 0;
+  __syncthreads();
+  if (warp < WARPS) {
+    // ================= streaming warps: the sums, and the tokens that may be among the top k =================
+    const uint64_t c2 = lp_pack(p.c, p.c);
+    uint4 now[UNROLL];
+    auto fetch = [&](const LpRow<T>& w, int base, int v1, uint4 (&to)[UNROLL]) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      vm[u] = x[u][0];
+      for (int u = 0; u < UNROLL; ++u) to[u] = w.inner(min(base + u * STREAM, v1 - 1));  // (what lies behind is replaced when it is its turn)
+    };
+    auto begin = [&](int r) {  // the first vectors of a row
+      const LpRow<T> w = row_of(r);
+      const int v0 = part(w, rank), v1 = part(w, rank + 1);
+      if (v1 > v0) fetch(w, v0 + tid, v1, now);
+    };
+    begin(row0);
+    // (more than one row only without a cluster; a row's first vectors are on their way while the one before is finished)
+    int n = 0;
+    for (int r = row0; r < p.R; r += step, ++n) {
+      const LpRow<T> row = row_of(r);
+      const int v0 = part(row, rank), v1 = part(row, rank + 1);
+      int top_vec = -1;
+      LpStat a = {-INFINITY, -kLpBig, 0.f, 0.f};
+      auto meet = [&](float vm, int vec) {
+        if (vm > a.m || (top_vec < 0 && vm == vm)) {  // the first of equal ones stays
+          a.m = vm;
+          top_vec = vec;
+        }
+      };
+      auto refer = [&]() {  // sums go over to the new maximum
+        const float M = lp_ref(a.m, p.c), d = fmaxf(a.M - M, kLpFar), f = lp_exp2(d);
+        a.w = (a.w + a.s * d) * f;
+        a.s *= f;
+        a.M = M;
+      };
+      auto sum = [&](const uint4& v, uint64_t& s2, uint64_t& w2) {
+        const uint64_t ref2 = lp_pack(-a.M, -a.M);
+        uint64_t x2[VEC / 2];
+        lp_pairs(v, x2, T{});
 #pragma unroll
-      for (int i = 1; i < VEC; ++i) vm[u] = fmaxf(vm[u], x[u][i]);
-      const int vec = base + u * THREADS;
-      if (vec < v1 && vm[u] == vm[u] && (vm[u] > top || top_vec < 0)) {  // the first of equal ones stays
-        top = vm[u];
-        top_vec = vec;
+        for (int i = 0; i < VEC / 2; ++i) {
+          const uint64_t y2 = lp_fma2(x2[i], c2, ref2);
+          float y0, y1;
+          lp_unpack(y2, y0, y1);
+          const uint64_t e2 = lp_pack(lp_exp2(y0), lp_exp2(y1));
+          s2 = lp_add2(s2, e2);
+          w2 = lp_fma2(e2, y2, w2);
+        }
+      };
+      auto add = [&](uint64_t s2, uint64_t w2) {
+        float s0, s1, w0, w1;
+        lp_unpack(s2, s0, s1);
+        lp_unpack(w2, w0, w1);
+        a.s += s0 + s1;
+        a.w += w0 + w1;
+      };
+      auto take_edge = [&](int vec) {  // (its missing elements are -inf to the sums and nothing to the maximum)
+        const uint4 v = row.raw(vec);
+        float x[VEC], vm = __int_as_float(0x7fc00000);
+        unpack16<T>(v, x);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const int j = row.first(vec) + i;
+          if (j >= 0 && j < p.V) vm = fmaxf(vm, x[i]);
+        }
+        meet(vm, vec);
+        refer();
+        uint64_t s2 = 0ull, w2 = 0ull;
+        sum(v, s2, w2);
+        add(s2, w2);
+      };
+      int edge_vec = 0;
+      const bool edge = tid < 2 && rank == (tid == 0 ? 0 : cluster - 1) && row.edge(tid, edge_vec);
+      if (edge && tid == 0) take_edge(edge_vec);
+      for (int base = v0 + tid; base < v1; base += STREAM * UNROLL) {
+        uint4 next[UNROLL];
+        fetch(row, base + UNROLL * STREAM, v1, next);
+        if (UNROLL > 1 && base + (UNROLL - 1) * STREAM >= v1) {  // the last round
+#pragma unroll
+          for (int u = 1; u < UNROLL; ++u)
+            if (base + u * STREAM >= v1) now[u] = make_uint4(row.kNothing, row.kNothing, row.kNothing, row.kNothing);
+        }
+        if (lp_top(now, T{}) > a.m || top_vec < 0) {
+#pragma unroll
+          for (int u = 0; u < UNROLL; ++u)
+            if (u == 0 || base + u * STREAM < v1) meet(lp_top<1>({now[u]}, T{}), base + u * STREAM);
+          refer();
+        }
+        uint64_t s2 = 0ull, w2 = 0ull;
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+          sum(now[u], s2, w2);
+          now[u] = next[u];
+        }
+        add(s2, w2);
       }
-    }
-    if (top > a.m) {
-      const float d = fmaxf((a.m - top) * p.c, kLpFar), f = lp_exp2(d);
-      a.w = (a.w + a.s * d) * f;
-      a.s *= f;
-      a.m = top;
-    }
-    const float ref = a.m == -INFINITY ? 0.f : a.m;
+      if (edge && tid == 1) take_edge(edge_vec);
+      if (r + step < p.R) begin(r + step);
+      const int b = n & 1;
+      if (n >= 2) lp_bar_sync<kFree, STREAM + 32>(b);  // the row before last has been read
+      if (p.k > 0) {
+        // The key of this thread's largest logit lies between that of its vector's last element and that of its first.
+        const unsigned long long high = top_vec < 0 ? 0ull : lp_key(a.m, max(row.first(top_vec), 0));
+        lows[b][tid] = top_vec < 0 ? 0ull : lp_key(a.m, min(row.first(top_vec) + VEC - 1, p.V - 1));
+        asm volatile("bar.sync %0, %1;" ::"n"(kStream), "n"(STREAM) : "memory");
+        if (warp == 0) {
+          unsigned long long g = 0ull;
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
+          for (int w = 0; w < WARPS; ++w) g = max(g, lows[b][w * 32 + lane]);
+          groups[lane] = g;
+          __syncwarp();
+          int above = 0;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float y = (x[u][i] - ref) * p.c, e = lp_exp2(y);
-        a.s += e;
-        a.w = fmaf(e, fmaxf(y, kLpFar), a.w);
-      }
-  }
-  // ---- the sums of the CTA ----
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    LpStat b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    b.w = __shfl_xor_sync(0xffffffffu, a.w, o);
-    a = lane & o ? lp_join(b, a, p.c) : lp_join(a, b, p.c);  // the same sum in both lanes
-  }
-  if (lane == 0) {
-    stat[warp][0] = a.m;
-    stat[warp][1] = a.s;
-    stat[warp][2] = a.w;
-  }
-  // ---- its top k ----
-  if (p.k > 0) {
-    // The key of this thread's largest logit lies between these two, by its vector's first and last element.
-    const unsigned long long low = top_vec < 0 ? 0ull : lp_key(top, min(row.first(top_vec) + VEC - 1, p.V - 1));
-    const unsigned long long high = top_vec < 0 ? 0ull : lp_key(top, max(row.first(top_vec), 0));
-    bound[warp][lane] = low;
-    if (tid == 0) n_found = n_owners = 0;
-    __syncthreads();
-    if (warp == 0) {
-      unsigned long long g = 0ull;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) g = max(g, bound[w][lane]);
-      int above = 0;
-      for (int i = 0; i < 32; ++i) {
-        const unsigned long long o = __shfl_sync(0xffffffffu, g, i);
-        above += o > g || (o == g && i < lane);
-      }
-      if (above == p.k - 1) limit = g;
-    }
-    __syncthreads();
-    unsigned long long lim = limit;
-    if (high >= lim) owners[atomicAdd(&n_owners, 1)] = (short)tid;  // (bound 0: fewer maxima than k, everything is looked at)
-    __syncthreads();
-    const int per = (v1 - v0 + THREADS - 1) / THREADS;  // vectors of a thread
-    const long long todo = (long long)n_owners * per;
-    for (;;) {
-      for (long long i = tid; i < todo; i += THREADS) {
-        const int vec = v0 + owners[i / per] + (int)(i % per) * THREADS;
-        if (vec >= v1) continue;
-        float x[VEC];
-        row.load(vec, x);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const int j = row.first(vec) + e;
-          if (j < 0 || j >= p.V) continue;
-          const unsigned long long key = lp_key(x[e], j);
-          if (key >= lim) {
-            const int at = atomicAdd(&n_found, 1);
-            if (at < kLpFound) found[at] = key;
+          for (int i = 0; i < 32; i += 2) {
+            const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&groups[i]);
+            above += (o.x > g || (o.x == g && i < lane)) + (o.y > g || (o.y == g && i + 1 < lane));
           }
+          if (above == p.k - 1) limits[b] = g;  // 0: fewer maxima than k, everything is looked at
+        }
+        asm volatile("bar.sync %0, %1;" ::"n"(kStream), "n"(STREAM) : "memory");
+        const unsigned long long lim = limits[b];
+        const float least = lp_value((uint32_t)(lim >> 32));
+        if (edge) look(row, edge_vec, row.raw(edge_vec), lim, least, b);
+        const unsigned who = __ballot_sync(0xffffffffu, high >= lim), per = (unsigned)(v1 - v0 + STREAM - 1) / STREAM;
+        if (high >= lim) owners[warp][__popc(who & ((1u << lane) - 1u))] = (unsigned char)lane;
+        __syncwarp();
+        const unsigned todo = __popc(who) * per;  // vectors of the warp's threads whose largest logit may reach it
+        for (unsigned i = lane; i < todo; i += 64u) {
+          const unsigned o0 = i / per, i1 = i + 32u, o1 = i1 / per;
+          const int vec0 = v0 + warp * 32 + owners[warp][o0] + (int)((i - o0 * per) * STREAM);
+          const int vec1 = i1 < todo ? v0 + warp * 32 + owners[warp][o1] + (int)((i1 - o1 * per) * STREAM) : v1;
+          const uint4 x0 = row.inner(min(vec0, v1 - 1)), x1 = row.inner(min(vec1, v1 - 1));
+          if (vec0 < v1) look(row, vec0, x0, lim, least, b);
+          if (vec1 < v1) look(row, vec1, x1, lim, least, b);
+        }
+        __syncwarp();
+      }
+      a = lp_warp_join(a);
+      if (lane == 0) stat[b][warp] = a;
+      lp_bar_arrive<kFull, STREAM + 32>(b);
+    }
+    if (n >= 2) lp_bar_sync<kFree, STREAM + 32>(n & 1);  // the last two rows' signals are taken too
+    if (n >= 1) lp_bar_sync<kFree, STREAM + 32>((n - 1) & 1);
+    if (cluster > 1) {
+      lp_cluster_sync();
+      lp_cluster_sync();
+    }
+    return;
+  }
+  // ================= the last two warps, a buffer each: a row's numbers, while the others are at the next ones =================
+  const int end = warp - WARPS;
+  if (cluster > 1 && end > 0) {  // one row, the first one's
+    lp_cluster_sync();
+    lp_cluster_sync();
+    return;
+  }
+  int n = end;
+  for (int r = row0 + end * step; r < p.R; r += ENDS * step, n += ENDS) {
+    const int b = n & 1;
+    unsigned long long *found = founds[b], *best = bests[b];
+    const LpRow<T> row = row_of(r);
+    const int v0 = part(row, rank), v1 = part(row, rank + 1);
+    const int target = p.targets[r];
+    const bool target_ok = target >= 0 && target < p.V;
+    const float target_logit = target_ok ? Io<T>::ld(row.row + target) : 0.f;
+    lp_bar_sync<kFull, STREAM + 32>(b);
+    LpStat a = lp_warp_join(lane < WARPS ? stat[b][lane] : LpStat{-INFINITY, -kLpBig, 0.f, 0.f});
+    unsigned long long top = 0ull;  // lane i: key of the i-th of the top k
+    if (p.k > 0) {
+      unsigned long long lim = limits[b];
+      for (;;) {
+        const int n_found = mets[b];
+        __syncwarp();
+        if (lane == 0) mets[b] = 0;
+        lp_rank(found, min(n_found, kLpFound), best, p.k, lane);
+        // More tokens reach the bound than there is room for: the k-th of those that were kept is a higher one.  Fewer than k (a thread whose
+        // bound was not a number's): everything is looked at.  Either way this warp goes through the CTA's vectors by itself.
+        const unsigned long long kth = best[p.k - 1];
+        const bool again = n_found > kLpFound;
+        if (!again && (kth != 0ull || lim == 0ull)) break;
+        lim = again ? kth : 0ull;
+        const float least = lp_value((uint32_t)(lim >> 32));
+        __syncwarp();
+        for (int vec = v0 + lane; vec < v1; vec += 32) look(row, vec, row.inner(vec), lim, least, b);
+        int edge_vec = 0;
+        if (lane < 2 && rank == (lane == 0 ? 0 : cluster - 1) && row.edge(lane, edge_vec)) look(row, edge_vec, row.raw(edge_vec), lim, least, b);
+        __syncwarp();
+      }
+      if (lane < p.k) top = best[lane];
+    }
+    __syncwarp();
+    lp_bar_arrive<kFree, STREAM + 32>(b);
+    if (cluster > 1) {  // one row: the first CTA joins
+      if (lane == 0) mine = a;
+      lp_cluster_sync();
+      if (rank == 0) {
+        LpStat other = {-INFINITY, -kLpBig, 0.f, 0.f};
+        if (lane < cluster) {
+          other.m = lp_ld_f32(lp_map(&mine.m, lane));
+          other.M = lp_ld_f32(lp_map(&mine.M, lane));
+          other.s = lp_ld_f32(lp_map(&mine.s, lane));
+          other.w = lp_ld_f32(lp_map(&mine.w, lane));
+        }
+        a = lp_warp_join(other);
+        if (lane < p.k)
+          for (int c = 0; c < cluster; ++c) found[c * p.k + lane] = lp_ld_u64(lp_map(&best[lane], c));
+      }
+      lp_cluster_sync();  // the others may leave
+      if (rank != 0) return;
+      // lists of k in order: a key's place is the sum of its places in all of them
+      const int all = cluster * p.k;
+      if (lane < p.k) best[lane] = 0ull;
+      __syncwarp();
+      for (int i = lane; i < all; i += 32) {
+        const unsigned long long key = found[i];
+        if (key == 0ull) continue;
+        int over = 0;
+        for (int c = 0; c < cluster; ++c) {
+          const unsigned long long* list = found + c * p.k;
+          int at = 0;
+#pragma unroll
+          for (int half = 32; half > 0; half >>= 1)
+            if (at + half <= p.k && list[at + half - 1] > key) at += half;
+          over += at;
+        }
+        if (over < p.k) best[over] = key;
+      }
+      __syncwarp();
+      if (lane < p.k) top = best[lane];
+    }
+    // A row beyond M's range: once more, by this warp alone.
+    const float m = a.m;
+    const bool far = m < INFINITY && m > -INFINITY && (!(fabsf(m * p.c) < kLpBig) || p.c > 1e7f);
+    if (far) {
+      float s = 0.f, w = 0.f;
+      for (int vec = lane; vec < row.n; vec += 32) {
+        float x[VEC];
+        unpack16<T>(row.raw(vec), x);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float y = (x[i] - m) * p.c, e = lp_exp2(y);
+          s += e;
+          w = fmaf(e, fmaxf(y, kLpFar), w);
         }
       }
-      __syncthreads();
-      const int n = min(n_found, kLpFound);
-      const bool again = n_found > kLpFound;
-      if (tid < p.k) best[tid] = 0ull;
-      __syncthreads();
-      for (int i = tid; i < n; i += THREADS) {
-        const unsigned long long key = found[i];
-        int above = 0;
-        for (int j = 0; j < n; ++j) above += found[j] > key;
-        if (above < p.k) best[above] = key;
-      }
-      __syncthreads();
-      if (!again) break;
-      // More tokens reach the bound than there is room for: the k-th of those that were kept is a higher one.
-      lim = best[p.k - 1];
-      if (tid == 0) n_found = 0;
-      __syncthreads();
+      a.s = warp_sum(s);
+      a.w = warp_sum(w);
     }
-  } else {
-    __syncthreads();
-  }
-  if (warp == 0) {
-    LpStat b = {-INFINITY, 0.f, 0.f};
-    for (int w = 0; w < WARPS; ++w) b = lp_join(b, LpStat{stat[w][0], stat[w][1], stat[w][2]}, p.c);
-    a = b;
-    if (lane == 0) {
-      mine[0] = a.m;
-      mine[1] = a.s;
-      mine[2] = a.w;
-    }
-  }
-  if (cluster > 1) {
-    __syncthreads();
-    lp_cluster_sync();
-    unsigned long long key = 0ull;
-    if (rank == 0) {
-      if (warp == 0) {
-        a = LpStat{-INFINITY, 0.f, 0.f};
-        for (int c = 0; c < cluster; ++c)
-          a = lp_join(a, LpStat{lp_ld_f32(lp_map(&mine[0], c)), lp_ld_f32(lp_map(&mine[1], c)), lp_ld_f32(lp_map(&mine[2], c))}, p.c);
-      }
-      if (tid < cluster * p.k) key = lp_ld_u64(lp_map(&best[tid % p.k], tid / p.k));
-    }
-    lp_cluster_sync();  // the others may leave
-    if (rank != 0) return;
-    if (p.k > 0) {
-      if (tid < cluster * p.k) found[tid] = key;
-      __syncthreads();
-      if (tid < cluster * p.k) {
-        int above = 0;
-        for (int j = 0; j < cluster * p.k; ++j) above += found[j] > key || (found[j] == key && j < tid);
-        if (above < p.k) best[above] = key;
-      }
-      __syncthreads();
-    }
-  }
-  if (warp == 0) {
     const float log_s = log2f(a.s);
     // nothing but -inf, or something that is not a number or +inf: no distribution
-    const bool none = !(a.s > 0.f) || !(a.m < INFINITY);
+    const bool none = !(a.s > 0.f) || !(m < INFINITY);
     const float nan = __int_as_float(0x7fc00000);
-    auto logprob = [&](float z) { return none ? nan : fmaf(z - a.m, p.inv_t, -log_s * kLn2); };
+    auto logprob = [&](float z) {
+      if (none) return nan;
+      if (far || z * p.c < -1e30f) return fmaf(z - m, p.inv_t, -log_s * kLn2);
+      return (fmaf(z, p.c, -a.M) - log_s) * kLn2;
+    };
     if (lane == 0) {
-      const int t = p.targets[r];
-      const bool ok = t >= 0 && t < p.V;
-      if (!ok && p.status) atomicOr(p.status, 4);
-      p.logprob[r] = ok ? logprob(Io<T>::ld(row.row + t)) : nan;
+      if (!target_ok && p.status) atomicOr(p.status, 4);
+      p.logprob[r] = target_ok ? logprob(target_logit) : nan;
       p.entropy[r] = none ? nan : fmaxf((log_s - a.w / a.s) * kLn2, 0.f);
     }
     if (lane < p.k) {
-      const unsigned long long key = best[lane];
-      p.top_ids[(long long)r * p.k + lane] = (int)(0xffffffffu - (uint32_t)key);
-      p.top_logprobs[(long long)r * p.k + lane] = logprob(lp_value((uint32_t)(key >> 32)));
+      p.top_ids[(long long)r * p.k + lane] = (int)(0xffffffffu - (uint32_t)top);
+      p.top_logprobs[(long long)r * p.k + lane] = logprob(lp_value((uint32_t)(top >> 32)));
     }
   }
 }
 
-template <typename T>
-static int logprobs_launch(const LpParams& p, cudaStream_t st) {
-  constexpr int THREADS = 256;
-  int cluster = 1;
-  // one row's vectors over more CTAs while there are SMs without one and each thread keeps a vector
-  while (cluster < 8 && (long long)p.R * cluster * 2 <= 296 && p.V / (Io<T>::kVec16 * THREADS) >= cluster * 2) cluster *= 2;
+template <typename T, int STREAM, int ENDS, int CTAS, int UNROLL>
+static int logprobs_go(const LpParams& p, int log_cluster, cudaStream_t st) {
+  const int cluster = 1 << log_cluster;
+  const long long most = 148 * CTAS;  // resident CTAs: the rows behind them follow in the same CTAs
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((long long)p.R * cluster));
-  cfg.blockDim = dim3(THREADS);
+  cfg.gridDim = dim3((unsigned)(cluster > 1 ? (long long)p.R * cluster : p.R < most ? p.R : most));
+  cfg.blockDim = dim3(STREAM + 32 * ENDS);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -315,8 +539,17 @@ static int logprobs_launch(const LpParams& p, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, THREADS>, p, cluster);
+  cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, STREAM, ENDS, CTAS, UNROLL>, p, log_cluster);
   return launch_status("token_logprobs");
+}
+
+template <typename T>
+static int logprobs_launch(const LpParams& p, cudaStream_t st) {
+  const int vecs = p.V / (Io<T>::kVec16 * 256);  // of a thread, with 256 of them to a row
+  // one row's vectors over more CTAs while there are SMs without one and each thread keeps a vector
+  int log = 0;
+  while (log < 3 && ((long long)p.R << (log + 1)) <= 296 && vecs >= 2 << log) ++log;
+  return vecs >> log >= 4 ? logprobs_go<T, 256, 1, 4, 4>(p, log, st) : logprobs_go<T, 256, 1, 4, 1>(p, log, st);
 }
 
 }  // namespace dgpt

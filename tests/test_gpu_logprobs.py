@@ -1,5 +1,7 @@
 """ops.token_logprobs against float64, and ops.kv_keep against indexing."""
 
+import math
+
 import pytest
 import torch
 
@@ -108,6 +110,42 @@ def test_rows_without_a_distribution(V, dtype):
     ok = [0, 5]
     part = ops.token_logprobs(logits[ok].contiguous(), targets[ok].contiguous(), top_k=8)
     check(logits[ok], targets[ok], 1.0, 8, part)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [11, 40, 5001])
+def test_ids_of_rows_with_nans_at_the_ends(V, dtype):
+    """NaN where a row's first and last vectors are partly another row's, -inf and nothing else between: ids are tokens, NaN behind -inf."""
+    from diff_gpt_b200 import ops
+
+    logits = torch.full((9, V), float("-inf"), dtype=dtype, device="cuda")
+    logits[:, :3] = float("nan")
+    logits[:, -2:] = float("nan")
+    r = ops.token_logprobs(logits, torch.zeros(9, dtype=torch.int32, device="cuda"), top_k=8)
+    want = (list(range(3, V - 2)) + [0, 1, 2, V - 2, V - 1])[:8]
+    assert r.top_ids.tolist() == [want] * 9 and bool(torch.isnan(r.top_logprobs).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rows_beyond_the_range_of_one_exponent(dtype):
+    """Nothing but the type's lowest value, huge logits of either sign, temperatures next to zero."""
+    from diff_gpt_b200 import ops
+
+    low = torch.finfo(dtype).min
+    for V in (100, 40000):
+        logits, targets = make(4, V, dtype, 8)
+        logits[0] = low
+        logits[1, :] = low / 2
+        logits[1, 7] = low / 4
+        logits[2] = logits[2] * 1e30
+        logits[3, 5] = -low
+        r = ops.token_logprobs(logits, targets, top_k=3)
+        lp, ent, ids, top = logprobs(logits.cpu(), targets.cpu(), 1.0, 3)
+        assert torch.equal(r.top_ids.cpu().long(), ids) and bool(torch.isfinite(r.entropy).all())
+        assert torch.allclose(r.entropy.cpu().double(), ent, atol=1e-5, rtol=1e-5)  # log V, 0, 0, 0: see check()
+        assert torch.allclose(r.top_logprobs.cpu().double(), top.float().double(), atol=1e-5, rtol=2.0**-21)
+        cold = ops.token_logprobs(logits[:1] * 0 + 1.0, targets[:1], top_k=1, temperature=1e-30)
+        assert abs(cold.entropy.item() - math.log(V)) < 1e-5
 
 
 def test_targets_outside_the_vocabulary():
