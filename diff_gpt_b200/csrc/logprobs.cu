@@ -12,8 +12,8 @@
 // a few dozen, all read by the few threads whose own maximum reaches it.  Those threads' vectors are read again (from L2, one in twenty or so of the row)
 // and the tokens found are ranked by counting.
 //
-// Eight warps of a CTA stream a row, two more finish a row each (sums, top tokens, outputs) while the eight are at the next ones; rows are handed
-// over through two buffers.  A cluster of 1 to 8 CTAs shares a row where rows are few; its first CTA joins the others' sums and lists through distributed shared memory.
+// Eight warps of a CTA stream a row, a ninth finishes it (sums, top tokens, outputs) while they are at the next one; rows are handed over through
+// two buffers.  A cluster of 1 to 8 CTAs shares a row where rows are few; its first CTA joins the others' sums and lists through distributed shared memory.
 // What bounds it: one read of the logits, then the exponentials (16 a clock and SM: three quarters of a read's time in bf16) and the instructions
 // around them, which is why pairs share them (fma, add, max) and the next vectors are on their way while these are worked on.  4096 rows of
 // 32001 bf16 logits: 60 us without top tokens, 75 with 5, 93 with 20; their reading alone takes 40.5.  (A CTA of 256 threads per row whose every warp goes through
@@ -23,6 +23,8 @@
 namespace dgpt {
 
 constexpr int kLpMost = 32;       // most top tokens
+constexpr int kLpStream = 256;    // threads that stream a row; a warp more finishes it
+constexpr int kLpCtas = 4;        // of an SM
 constexpr float kLpBig = 1073741824.f;  // 2^30: M is kept within it
 constexpr float kLpFar = -1e4f;  // an exponent whose power is 0: keeps 0 times infinity out of the sums
 constexpr int kLpFound = 512;     // tokens found above the bound that are ranked at once
@@ -215,14 +217,14 @@ __device__ __forceinline__ void lp_rank(unsigned long long* keys, int n, unsigne
   __syncwarp();
 }
 
-template <int BAR, int THREADS>
-__device__ __forceinline__ void lp_bar_sync(int which) { asm volatile("bar.sync %0, %1;" ::"r"(BAR + which), "n"(THREADS) : "memory"); }
-template <int BAR, int THREADS>
-__device__ __forceinline__ void lp_bar_arrive(int which) { asm volatile("bar.arrive %0, %1;" ::"r"(BAR + which), "n"(THREADS) : "memory"); }
+template <int BAR>
+__device__ __forceinline__ void lp_bar_sync(int which) { asm volatile("bar.sync %0, %1;" ::"r"(BAR + which), "n"(kLpStream + 32) : "memory"); }
+template <int BAR>
+__device__ __forceinline__ void lp_bar_arrive(int which) { asm volatile("bar.arrive %0, %1;" ::"r"(BAR + which), "n"(kLpStream + 32) : "memory"); }
 
-template <typename T, int STREAM, int ENDS, int CTAS, int UNROLL>
-__global__ void __launch_bounds__(STREAM + 32 * ENDS, CTAS) token_logprobs_kernel(const LpParams p, const int log_cluster) {
-  constexpr int VEC = Io<T>::kVec16, WARPS = STREAM / 32;
+template <typename T, int UNROLL>
+__global__ void __launch_bounds__(kLpStream + 32, kLpCtas) token_logprobs_kernel(const LpParams p, const int log_cluster) {
+  constexpr int VEC = Io<T>::kVec16, STREAM = kLpStream, WARPS = STREAM / 32;
   constexpr int kFull = 1, kFree = 3;  // named barriers, one per buffer
   constexpr int kStream = 5;
   __shared__ unsigned long long lows[2][STREAM];                        // what the key of each streaming thread's largest logit is at least
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(STREAM + 32 * ENDS, CTAS) token_logprobs_kerne
       if (edge && tid == 1) take_edge(edge_vec);
       if (r + step < p.R) begin(r + step);
       const int b = n & 1;
-      if (n >= 2) lp_bar_sync<kFree, STREAM + 32>(b);  // the row before last has been read
+      if (n >= 2) lp_bar_sync<kFree>(b);  // the row before last has been read
       if (p.k > 0) {
         // The key of this thread's largest logit lies between that of its vector's last element and that of its first.
         const unsigned long long high = top_vec < 0 ? 0ull : lp_key(a.m, max(row.first(top_vec), 0));
@@ -395,25 +397,19 @@ __global__ void __launch_bounds__(STREAM + 32 * ENDS, CTAS) token_logprobs_kerne
       }
       a = lp_warp_join(a);
       if (lane == 0) stat[b][warp] = a;
-      lp_bar_arrive<kFull, STREAM + 32>(b);
+      lp_bar_arrive<kFull>(b);
     }
-    if (n >= 2) lp_bar_sync<kFree, STREAM + 32>(n & 1);  // the last two rows' signals are taken too
-    if (n >= 1) lp_bar_sync<kFree, STREAM + 32>((n - 1) & 1);
+    if (n >= 2) lp_bar_sync<kFree>(n & 1);  // the last two rows' signals are taken too
+    if (n >= 1) lp_bar_sync<kFree>((n - 1) & 1);
     if (cluster > 1) {
       lp_cluster_sync();
       lp_cluster_sync();
     }
     return;
   }
-  // ================= the last two warps, a buffer each: a row's numbers, while the others are at the next ones =================
-  const int end = warp - WARPS;
-  if (cluster > 1 && end > 0) {  // one row, the first one's
-    lp_cluster_sync();
-    lp_cluster_sync();
-    return;
-  }
-  int n = end;
-  for (int r = row0 + end * step; r < p.R; r += ENDS * step, n += ENDS) {
+  // ================= the last warp: a row's numbers, while the others are at the next one =================
+  int n = 0;
+  for (int r = row0; r < p.R; r += step, ++n) {
     const int b = n & 1;
     unsigned long long *found = founds[b], *best = bests[b];
     const LpRow<T> row = row_of(r);
@@ -421,7 +417,7 @@ __global__ void __launch_bounds__(STREAM + 32 * ENDS, CTAS) token_logprobs_kerne
     const int target = p.targets[r];
     const bool target_ok = target >= 0 && target < p.V;
     const float target_logit = target_ok ? Io<T>::ld(row.row + target) : 0.f;
-    lp_bar_sync<kFull, STREAM + 32>(b);
+    lp_bar_sync<kFull>(b);
     LpStat a = lp_warp_join(lane < WARPS ? stat[b][lane] : LpStat{-INFINITY, -kLpBig, 0.f, 0.f});
     unsigned long long top = 0ull;  // lane i: key of the i-th of the top k
     if (p.k > 0) {
@@ -447,7 +443,7 @@ __global__ void __launch_bounds__(STREAM + 32 * ENDS, CTAS) token_logprobs_kerne
       if (lane < p.k) top = best[lane];
     }
     __syncwarp();
-    lp_bar_arrive<kFree, STREAM + 32>(b);
+    lp_bar_arrive<kFree>(b);
     if (cluster > 1) {  // one row: the first CTA joins
       if (lane == 0) mine = a;
       lp_cluster_sync();
@@ -525,13 +521,13 @@ __global__ void __launch_bounds__(STREAM + 32 * ENDS, CTAS) token_logprobs_kerne
   }
 }
 
-template <typename T, int STREAM, int ENDS, int CTAS, int UNROLL>
+template <typename T, int UNROLL>
 static int logprobs_go(const LpParams& p, int log_cluster, cudaStream_t st) {
   const int cluster = 1 << log_cluster;
-  const long long most = 148 * CTAS;  // resident CTAs: the rows behind them follow in the same CTAs
+  const long long most = 148 * kLpCtas;  // resident CTAs: the rows behind them follow in the same CTAs
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(cluster > 1 ? (long long)p.R * cluster : p.R < most ? p.R : most));
-  cfg.blockDim = dim3(STREAM + 32 * ENDS);
+  cfg.blockDim = dim3(kLpStream + 32);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -539,17 +535,17 @@ static int logprobs_go(const LpParams& p, int log_cluster, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, STREAM, ENDS, CTAS, UNROLL>, p, log_cluster);
+  cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, UNROLL>, p, log_cluster);
   return launch_status("token_logprobs");
 }
 
 template <typename T>
 static int logprobs_launch(const LpParams& p, cudaStream_t st) {
-  const int vecs = p.V / (Io<T>::kVec16 * 256);  // of a thread, with 256 of them to a row
+  const int vecs = p.V / (Io<T>::kVec16 * kLpStream);  // of a thread, with one CTA a row
   // one row's vectors over more CTAs while there are SMs without one and each thread keeps a vector
   int log = 0;
   while (log < 3 && ((long long)p.R << (log + 1)) <= 296 && vecs >= 2 << log) ++log;
-  return vecs >> log >= 4 ? logprobs_go<T, 256, 1, 4, 4>(p, log, st) : logprobs_go<T, 256, 1, 4, 1>(p, log, st);
+  return vecs >> log >= 4 ? logprobs_go<T, 4>(p, log, st) : logprobs_go<T, 1>(p, log, st);
 }
 
 }  // namespace dgpt

@@ -58,16 +58,6 @@ struct PackedProblem {
     }
     return lo;
   }
-  // The same by halves, for a thread.
-  __device__ int find(int slot, int bm) const {
-    int lo = 0, hi = n_seq - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (q_start(mid) / bm + mid <= slot) lo = mid;
-      else hi = mid - 1;
-    }
-    return lo;
-  }
   // A sequence and what is known of it.
   struct Cursor {
     int seq = 0, first = 0, end = 0, kb = 0, nk = 0, slot0 = 0, slot1 = 0;  // it has slots [slot0, slot1)
@@ -136,7 +126,7 @@ struct PackedProblem {
 // whose bit is set: word j / 64, bit j % 64 of ancestors[s][t].  The rows of one key/value head are its T * (H / G) pairs of node and
 // query head, node-major, so that K and V are read once for all of them.
 struct TreeProblem {
-  struct Cursor {};
+  static constexpr int kSorted = 64;  // sequences, at most, that are taken from the longest to the shortest
   const void* q;
   long long q_rs;
   KvView kv;
@@ -162,12 +152,12 @@ struct TreeProblem {
     nodes = (int)min((long long)nodes, room - context);
   }
   // Splits share the key tiles of `bn` keys evenly; where there are fewer tiles, the splits behind them get none.
-  __device__ bool item(unsigned i, int bn, RaggedItem& it) const {
+  __device__ bool item(unsigned i, int bn, RaggedItem& it, const int* order = nullptr) const {
     const unsigned a = i / (unsigned)n_splits, b = a / (unsigned)tiles, c = b / (unsigned)G;
     it.split = (int)(i - a * (unsigned)n_splits);
     const int tile = (int)(a - b * (unsigned)tiles);
     it.g = (int)(b - c * (unsigned)G);
-    it.seq = (int)c;
+    it.seq = order ? order[c] : (int)c;
     it.h = it.g * group;
     int context, nodes;
     lengths(it.seq, context, nodes);
@@ -184,6 +174,24 @@ struct TreeProblem {
     it.last0 = 0;
     it.kbase = it.held = 0;
     return true;
+  }
+  // order[i]: the i-th longest sequence (B <= kSorted; for a whole warp).
+  __device__ void sort(int* order, int lane) const {
+    int c[2], r[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      c[u] = lane + 32 * u < B ? ctx[lane + 32 * u] : -1;
+      r[u] = 0;
+    }
+    for (int j = 0; j < B; ++j) {
+      const int o = __shfl_sync(0xffffffffu, j < 32 ? c[0] : c[1], j & 31);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) r[u] += o > c[u] || (o == c[u] && j < lane + 32 * u);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (lane + 32 * u < B) order[r[u]] = lane + 32 * u;
+    __syncwarp();
   }
   __device__ const unsigned long long* mask_row(const RaggedItem& it, int r) const {
     return ancestors + ((long long)it.seq * T + (it.row0 + r) / group) * words;

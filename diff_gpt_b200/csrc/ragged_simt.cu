@@ -9,6 +9,13 @@
 
 namespace dgpt {
 
+// 2^x within 2 units of the last place; -inf gives 0
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 constexpr int kRgThreads = 256;
 constexpr int kRgBN = 64;
 
@@ -33,7 +40,7 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
   } else {
     const unsigned slot = blockIdx.x / (unsigned)p.H;
     typename P::Cursor cur;
-    p.load(p.find((int)slot, BM), BM, cur);
+    p.load(p.find((int)slot, BM, tid & 31), BM, cur);
     if (!p.item((int)slot, cur, (int)(blockIdx.x - slot * (unsigned)p.H), BM, it)) return;
   }
   for (int i = tid; i < BM * VPR; i += kRgThreads) {
@@ -58,25 +65,38 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
 #pragma unroll
     for (int c = 0; c < CO; ++c) acc[i][c] = 0.f;
   }
-  for (int j0 = it.key0; j0 < it.key1; j0 += kRgBN) {
-    __syncthreads();  // Q is in place; the last step's K, V and P have been read
-    for (int i = tid; i < kRgBN * VPR; i += kRgThreads) {
-      const int jj = i / VPR, c = i - jj * VPR, j = j0 + jj;
-      float kf[VEC], vf[VEC];
+  // A step's keys and values are on their way in registers while the step before is worked on.
+  constexpr int NV = (kRgBN * VPR + kRgThreads - 1) / kRgThreads;
+  uint4 kr[NV], vr[NV];
+  auto fetch = [&](int j0) {
 #pragma unroll
-      for (int x = 0; x < VEC; ++x) kf[x] = vf[x] = 0.f;
-      if (j < it.key1) {
+    for (int u = 0; u < NV; ++u) {
+      const int i = tid + u * kRgThreads, jj = i / VPR, c = i - jj * VPR, j = j0 + jj;
+      kr[u] = vr[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (jj < kRgBN && j < it.key1) {
         if constexpr (TREE) {
           const long long off = p.key_offset(it, j);
           if (off >= 0) {
-            ld16<T>(static_cast<const T*>(p.kv.k) + off + c * VEC, kf);
-            ld16<T>(static_cast<const T*>(p.kv.v) + off + c * VEC, vf);
+            kr[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.kv.k) + off + c * VEC));
+            vr[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.kv.v) + off + c * VEC));
           }
         } else {
-          ld16<T>(p.template k_row<T>(it, j) + c * VEC, kf);
-          ld16<T>(p.template v_row<T>(it, j) + c * VEC, vf);
+          kr[u] = __ldg(reinterpret_cast<const uint4*>(p.template k_row<T>(it, j) + c * VEC));
+          vr[u] = __ldg(reinterpret_cast<const uint4*>(p.template v_row<T>(it, j) + c * VEC));
         }
       }
+    }
+  };
+  fetch(it.key0);
+  for (int j0 = it.key0; j0 < it.key1; j0 += kRgBN) {
+    __syncthreads();  // Q is in place; the last step's K, V and P have been read
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int i = tid + u * kRgThreads, jj = i / VPR, c = i - jj * VPR;
+      if (jj >= kRgBN) continue;
+      float kf[VEC], vf[VEC];
+      unpack16<T>(kr[u], kf);
+      unpack16<T>(vr[u], vf);
 #pragma unroll
       for (int x = 0; x < VEC; x += 4) {
         *reinterpret_cast<float4*>(&Ks[jj * PITCH + c * VEC + x]) = make_float4(kf[x], kf[x + 1], kf[x + 2], kf[x + 3]);
@@ -84,6 +104,7 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
       }
     }
     __syncthreads();
+    if (j0 + kRgBN < it.key1) fetch(j0 + kRgBN);
     // scores: rows ty * RM + i, keys tx + 16 j
     float s[RM][KC];
 #pragma unroll
@@ -119,11 +140,11 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
 #pragma unroll
       for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
       const float mn = fmaxf(m[i], top), ref = mn == -INFINITY ? 0.f : mn;
-      const float f = exp2f(m[i] - ref);  // m = -inf: 0
+      const float f = ex2(m[i] - ref);  // m = -inf: 0
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
-        const float e = exp2f(s[i][j] - ref);
+        const float e = ex2(s[i][j] - ref);
         sum += e;
         Ps[r * PPITCH + tx + 16 * j] = e;
       }
@@ -251,7 +272,8 @@ int tree_simt(const TreeProblem& full, int dtype, cudaStream_t st) {
 }
 
 // ---- partials of a tree's rows into one -------------------------------------------------------------------------
-// One warp per (row, head): y = sum_s 2^(lse_s - m) o_s / sum_s 2^(lse_s - m).
+// One warp per (row, head): y = sum_s 2^(lse_s - m) o_s / sum_s 2^(lse_s - m), with the running maximum m, four shares at a time.  Their loads, and
+// those of the lengths that say how many shares there are, do not wait for one another (what is read of shares that were not written counts for nothing).
 template <typename T>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeProblem p) {
   dep_wait();
@@ -260,27 +282,44 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeProblem p) {
   const int lane = threadIdx.x & 31, h = (int)(at % p.H);
   const long long row = at / p.H;
   const int s = (int)(row / p.T), t = (int)(row - (long long)s * p.T);
-  if (p.n_nodes && t >= p.n_nodes[s]) return;
-  int context, nodes;
-  p.lengths(s, context, nodes);
-  const int splits = min(p.n_splits, (context + nodes + p.tile_keys - 1) / p.tile_keys);  // the ones behind have no keys
-  float m = -INFINITY;
-  for (int i = lane; i < splits; i += 32) m = fmaxf(m, p.part_lse[i * n + at]);
-  m = warp_max(m);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f;  // columns lane * 4 .. (D <= 128)
-  const bool mine = lane * 4 < p.D;
-  for (int i = 0; i < splits; ++i) {
-    const float lse = p.part_lse[i * n + at];
-    if (lse == -INFINITY) continue;  // no key of this share is seen
-    const float w = exp2f(lse - ref);
-    total += w;
-    if (mine) {
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (i * n + at) * p.D + lane * 4);
-      acc[0] = fmaf(w, v.x, acc[0]);
-      acc[1] = fmaf(w, v.y, acc[1]);
-      acc[2] = fmaf(w, v.z, acc[2]);
-      acc[3] = fmaf(w, v.w, acc[3]);
+  const bool mine = lane * 4 < p.D;  // columns lane * 4 .. (D <= 128)
+  int splits = p.n_splits;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f, m = -INFINITY;
+  for (int i0 = 0; i0 < splits; i0 += 4) {
+    float lse[4];
+    float4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long slot = min(i0 + u, p.n_splits - 1) * n + at;
+      lse[u] = p.part_lse[slot];
+      v[u] = mine ? *reinterpret_cast<const float4*>(p.part_o + slot * p.D + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (i0 == 0) {
+      if (p.n_nodes && t >= p.n_nodes[s]) return;
+      int context, nodes;
+      p.lengths(s, context, nodes);
+      splits = min(p.n_splits, (context + nodes + p.tile_keys - 1) / p.tile_keys);  // the ones behind have no keys
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (i0 + u >= splits) lse[u] = -INFINITY;
+      top = fmaxf(top, lse[u]);
+    }
+    const float ref = top == -INFINITY ? 0.f : top, f = ex2(m - ref);
+    m = top;
+    total *= f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] *= f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (lse[u] == -INFINITY) continue;  // no key of this share is seen
+      const float w = ex2(lse[u] - ref);
+      total += w;
+      acc[0] = fmaf(w, v[u].x, acc[0]);
+      acc[1] = fmaf(w, v[u].y, acc[1]);
+      acc[2] = fmaf(w, v[u].z, acc[2]);
+      acc[3] = fmaf(w, v[u].w, acc[3]);
     }
   }
   if (!mine) return;

@@ -18,6 +18,8 @@
 // TMEM columns: S0 [0,128)  S1 [128,256)  P0 [256,320)  P1 [320,384)  O [384, 384 + D).
 // No cluster launch and no multicast.  Every wait is bounded in clock cycles; one that runs out raises the CTA's abort flag, on which the other
 // roles stop too, sets bit 1 of the status word, and the CTA drains its copies, frees its TMEM and returns.
+#include <type_traits>
+
 #include "ragged.cuh"
 #include "tcgen05.cuh"
 
@@ -56,22 +58,29 @@ __device__ __forceinline__ bool cta_answer(uint32_t answer, unsigned& cta) {
   return ok != 0;
 }
 
-// Item `i` of the launch; false if it has no rows.  For a whole warp.  `seq`: the sequence of the item before, where most items are found.
-template <class P, bool TREE>
-__device__ __forceinline__ bool rt_item(const P& p, unsigned i, typename P::Cursor& cur, RtItem& x, int lane) {
-  bool there;
-  if constexpr (TREE) {
-    there = p.item(i, kBN, x.it);
-  } else {
+// The items of a launch by their numbers, for a whole warp.  Prompts: a tile's sequence is mostly that of the tile before.  Trees: from the longest
+// sequence to the shortest where they are few enough to be sorted, so that the last items are short ones.
+struct PackedItems {
+  const PackedProblem& p;
+  PackedProblem::Cursor cur;
+  __device__ PackedItems(const PackedProblem& q, int*, int) : p(q) {}
+  __device__ bool get(unsigned i, RaggedItem& it, int lane) {
     const unsigned j = gridDim.x - 1u - i, slot = j / (unsigned)p.H;
     p.seek((int)slot, kBM, lane, cur);
-    there = p.item((int)slot, cur, (int)(j - slot * (unsigned)p.H), kBM, x.it);
+    return p.item((int)slot, cur, (int)(j - slot * (unsigned)p.H), kBM, it);
   }
-  if (!there) return false;
-  x.tile0 = x.it.key0 / kBN;
-  x.n = (x.it.key1 - x.it.key0 + kBN - 1) / kBN;
-  return true;
-}
+};
+struct TreeItems {
+  const TreeProblem& p;
+  const int* order = nullptr;
+  __device__ TreeItems(const TreeProblem& q, int* room, int lane) : p(q) {
+    if (p.B > 1 && p.B <= TreeProblem::kSorted && p.items() > 148) {
+      p.sort(room, lane);
+      order = room;
+    }
+  }
+  __device__ bool get(unsigned i, RaggedItem& it, int) { return p.item(i, kBN, it, order); }
+};
 
 // The rows of an item without keys: zeros.  (A share without keys of a tree's rows is left out by the pass that joins the shares.)
 template <class P, bool TREE>
@@ -349,7 +358,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       // the oldest unfinished item there is one more, or as many as make up three key tiles.  (No fewer: the issuer's score cursor is two
       // tiles ahead of its products and waits for the next item before it goes on, the loader's K cursor one.  The items that they hold
       // unfinished then have at most two tiles behind the oldest one's, so the next one is always on its way.  Items without a key never get here.)
-      typename P::Cursor cursor;
+      std::conditional_t<TREE, TreeItems, PackedItems> items(p, reinterpret_cast<int*>(ring + kRtRing * 64 + 4 * 4096), lane);
       unsigned at = 0u, freed = 0u, asked = 0u, cta = blockIdx.x;  // items handed out, items finished
       int ahead = 0;                                               // key tiles of those behind the oldest unfinished one
       bool ok = true, more = true;
@@ -372,7 +381,9 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         ++at;
       };
       while (ok && more) {
-        if (rt_item<P, TREE>(p, cta, cursor, x, lane)) {
+        if (items.get(cta, x.it, lane)) {
+          x.tile0 = x.it.key0 / kBN;
+          x.n = (x.it.key1 - x.it.key0 + kBN - 1) / kBN;
           if (x.n > 0) push();
           else no_keys<P, TREE>(p, x.it, d_head, lane);
         }
@@ -718,7 +729,7 @@ static int ragged_tc_go(const TcMaps& maps, const P& p, long long items, int d_h
     set_error("ragged attention: too many rows");
     return DGPT_E_ARG;
   }
-  size_t smem = (size_t)6 * (D / 64) * kBN * 128 + 48 * 8 + 4 * kBM * 8 + 6 * kBM * 4 + kRtRing * 64 + 4 * 4096 + 1024;
+  size_t smem = (size_t)6 * (D / 64) * kBN * 128 + 48 * 8 + 4 * kBM * 8 + 6 * kBM * 4 + kRtRing * 64 + 4 * 4096 + TreeProblem::kSorted * 4 + 1024;
   if (smem < 120 * 1024) smem = 120 * 1024;  // one CTA owns an SM: it takes all 512 TMEM columns
   auto kernel = ragged_tc_kernel<D, P, TREE>;
   cudaError_t e = cudaSuccess;
