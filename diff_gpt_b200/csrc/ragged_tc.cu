@@ -15,6 +15,8 @@
 //                    finds the tile's own maximum too; the two swap that through shared memory, and only where it exceeds the running one by more than 2^8
 //                    is O rescaled and the tile redone
 //   warps 8-11       output: row sums from shared memory, O from TMEM, one row per thread
+// (Two CTAs an SM for heads of 64, each with one score buffer, its softmax threads storing the output: 512 prompts of 128 143 us instead of 161, 40 mixed
+// ones 106 instead of 102, 8 of 4096 597 instead of 615; not kept.)
 // TMEM columns: S0 [0,128)  S1 [128,256)  P0 [256,320)  P1 [320,384)  O [384, 384 + D).
 // No cluster launch and no multicast.  Every wait is bounded in clock cycles; one that runs out raises the CTA's abort flag, on which the other
 // roles stop too, sets bit 1 of the status word, and the CTA drains its copies, frees its TMEM and returns.
@@ -27,7 +29,9 @@ namespace dgpt {
 namespace tc {
 
 constexpr int kRtThreads = 512;
-constexpr int kRtSoftmaxRegs = 168, kRtOutputRegs = 96, kRtHelperRegs = 80;  // 2 x 168 + 96 + 80 = 4 x 128, the launch's share
+// Registers per thread: the launch's, and a softmax and a helper thread's after the warpgroups have traded them (an output thread keeps the launch's).
+constexpr int kRtRegs = 128, kRtSoftmaxRegs = 144, kRtHelperRegs = 96;
+static_assert(2 * kRtSoftmaxRegs + kRtRegs + kRtHelperRegs == 4 * kRtRegs, "the warpgroups share what the launch has");
 constexpr int kRtRing = 8;                                                    // items between the warp that finds them and the last role that reads them
 
 struct RtItem {
@@ -409,7 +413,6 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
     }
   } else if (warp >= 8) {
     // ================= output: one thread per row =================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRtOutputRegs));
     const int quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t o_addr = tmem + ((uint32_t)(quarter * 32) << 16) + kOCol;
     uint8_t* stage = ring + kRtRing * 64 + quarter * 4096;
@@ -580,14 +583,11 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
           continue;
         }
         const int c0 = t0 + half * kHalf;  // key of this thread's first column
-        float sv[kHalf];
-#pragma unroll
-        for (int c = 0; c < kHalf / 32; ++c) tmem_ld32_nowait(lane_addr + buf * 128 + half * kHalf + c * 32, &sv[c * 32]);
-        tc_wait_ld();
-        if (__builtin_expect(t0 + kBN > clear, 0)) {
+        // Bit i: this thread's column i is seen.
+        unsigned long long seen = ~0ull;
+        const bool masked = t0 + kBN > clear;
+        if (__builtin_expect(masked, 0)) {
           if constexpr (TREE) {
-            // bit i: column i is seen
-            unsigned long long seen = ~0ull;
             const int d0 = c0 - clear;
             if (d0 > -kHalf && row < rows) {
               const unsigned long long* words = p.mask_row(x.it, row);
@@ -602,31 +602,36 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
             }
             const int left = x.it.key1 - c0;
             if (left < kHalf) seen = left > 0 ? seen & ((1ull << left) - 1ull) : 0ull;
-            const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              sv[i] = (lo >> i) & 1u ? sv[i] : -INFINITY;
-              sv[32 + i] = (hi >> i) & 1u ? sv[32 + i] : -INFINITY;
-            }
           } else {
-            const int last = row < rows ? min(x.it.last0 + row, x.it.key1 - 1) - c0 : kHalf;
-#pragma unroll
-            for (int i = 0; i < kHalf; ++i) sv[i] = i <= last ? sv[i] : -INFINITY;
+            const int n_seen = row < rows ? min(x.it.last0 + row, x.it.key1 - 1) - c0 + 1 : kHalf;
+            if (n_seen < kHalf) seen = n_seen > 0 ? (1ull << n_seen) - 1ull : 0ull;
           }
         }
+        // 32 scores at a time, in loops that stay loops: with all 64 in registers at once, and the code for them, the softmax warps waited for
+        // instructions: 40 prompts of 17 to 1000, 12 heads of 64, 110 us so, 102 in this form; 512 of 128 172 and 161; 8 of 4096, 16 of 128, 618 and 631)
+        auto scores = [&](int c, float (&sv)[32]) {
+          tmem_ld32(lane_addr + buf * 128 + half * kHalf + c * 32, sv);
+          if (__builtin_expect(masked, 0)) {
+            const uint32_t bits = c ? (uint32_t)(seen >> 32) : (uint32_t)seen;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sv[i] = (bits >> i) & 1u ? sv[i] : -INFINITY;
+          }
+        };
         // One sweep turns this thread's scores into probabilities against a reference (log2 domain), writes them as packed bf16 and
         // returns their sum, and the largest exponent met.
         auto sweep = [&](float ref, float& top) -> float {
           const uint64_t scale2 = pack2(scale_log2, scale_log2), negm2 = pack2(-ref, -ref);
           uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
           float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < kHalf / 32; ++c) {
+            float sv[32];
+            scores(c, sv);
             uint32_t packed[16];
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               float x0, x1;
-              unpack2(fma2(pack2(sv[c * 32 + i], sv[c * 32 + i + 1]), scale2, negm2), x0, x1);
+              unpack2(fma2(pack2(sv[i], sv[i + 1]), scale2, negm2), x0, x1);
               tops[(i >> 1) & 3] = max3(tops[(i >> 1) & 3], x0, x1);
               const float p0 = ex2(x0), p1 = ex2(x1);  // -inf -> 0
               rs2[(i >> 1) & 3] = add2(rs2[(i >> 1) & 3], pack2(p0, p1));
@@ -651,13 +656,18 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
           sum = sweep(m, top);
           mx2 = fmaxf(top, exchange(top, xok)) + m;  // exponents were taken against m
         } else {
-          float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float mine = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < kHalf / 32; ++c) {
+            float sv[32], mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            scores(c, sv);
 #pragma unroll
-          for (int i = 0; i < kHalf; i += 8) {
+            for (int i = 0; i < 32; i += 8) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) mxs[c] = max3(mxs[c], sv[i + 2 * c], sv[i + 2 * c + 1]);
+              for (int u = 0; u < 4; ++u) mxs[u] = max3(mxs[u], sv[i + 2 * u], sv[i + 2 * u + 1]);
+            }
+            mine = fmaxf(mine, fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])));
           }
-          const float mine = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
           mx2 = fmaxf(mine, exchange(mine, xok)) * scale_log2;
         }
         if (!__all_sync(0xffffffffu, xok)) {
@@ -734,8 +744,16 @@ static int ragged_tc_go(const TcMaps& maps, const P& p, long long items, int d_h
   auto kernel = ragged_tc_kernel<D, P, TREE>;
   cudaError_t e = cudaSuccess;
   static bool ready[64] = {};  // the attribute is a device's for good
-  if (!ready[dev]) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  ready[dev] = e == cudaSuccess;
+  if (!ready[dev]) {
+    cudaFuncAttributes attr;
+    e = cudaFuncGetAttributes(&attr, kernel);
+    if (e == cudaSuccess && attr.numRegs != kRtRegs) {  // setmaxnreg would wait for registers that the launch does not have
+      set_error("ragged attention: built with %d registers a thread instead of %d", attr.numRegs, kRtRegs);
+      return DGPT_E_UNSUPPORTED;
+    }
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    ready[dev] = e == cudaSuccess;
+  }
   if (e != cudaSuccess) {
     set_error("ragged attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     return DGPT_E_CUDA;
