@@ -153,7 +153,7 @@ PROTOTYPES = {
     "dgpt_tree_attn_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32]),
     "dgpt_tree_attn": (
         C.c_int,
-        [_p, _i64, _kvp, _i64, _p, _p, _p, _i32, _p, _i64, _p, _sz, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _p, _p],
+        [_p, _i64, _kvp, _i64, _p, _p, _p, _p, _p, _i32, _p, _i64, _p, _sz, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _p, _p],
     ),
     "dgpt_token_logprobs": (C.c_int, [_p, _i64, _p, _f32, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _p]),
     "dgpt_kv_keep": (C.c_int, [_kvp, _i64, _p, _p, _p, _p, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _p, _p]),

@@ -75,7 +75,7 @@ extern "C" size_t dgpt_tree_attn_workspace_bytes(int32_t B, int32_t T, int32_t H
 }
 
 extern "C" int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv_layout* kv, int64_t kv_token_stride, const int32_t* ctx_len,
-                              const int32_t* n_nodes, const uint64_t* ancestors, int32_t words, void* out, int64_t out_row_stride,
+                              const int32_t* gap_start, const int32_t* gap_end, const int32_t* n_nodes, const uint64_t* ancestors, int32_t words, void* out, int64_t out_row_stride,
                               void* workspace, size_t workspace_bytes, int32_t n_splits, int32_t B, int32_t T, int32_t H, int32_t G, int32_t D,
                               float scale, int32_t dtype, int32_t impl, int32_t* status, void* stream) {
   DGPT_REQUIRE(B >= 0 && T >= 0 && H > 0 && G > 0 && H % G == 0, "tree_attn: bad sizes");
@@ -94,6 +94,7 @@ extern "C" int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv
   }
   if (B == 0 || T == 0) return DGPT_OK;
   DGPT_REQUIRE(q && ctx_len && ancestors && out, "tree_attn: NULL pointer");
+  DGPT_REQUIRE((gap_start == nullptr) == (gap_end == nullptr), "tree_attn: a gap has a start and an end");
   if (int e = validate_kv(kv, D)) return e;
   DGPT_REQUIRE(aligned16(q) && aligned16(out), "tree_attn: pointers must be 16-byte aligned");
   DGPT_REQUIRE(q_row_stride >= (int64_t)H * D && out_row_stride >= (int64_t)H * D && q_row_stride % 8 == 0 && out_row_stride % 8 == 0,
@@ -112,6 +113,8 @@ extern "C" int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv
   p.kv = make_view(kv);
   p.kv.token_stride = kv_token_stride;
   p.ctx = ctx_len;
+  p.gap_start = gap_start;
+  p.gap_end = gap_end;
   p.n_nodes = n_nodes;
   p.ancestors = reinterpret_cast<const unsigned long long*>(ancestors);
   p.words = words;

@@ -22,6 +22,7 @@ struct RaggedItem {
   int split;       // tree: which share of the keys
   int kbase;       // packed: row of the sequence's key 0
   int held;        // packed: the sequence's keys
+  int gap0, gap1;  // tree: slots [gap0, gap1) before the drafts hold nothing
 };
 
 // ---- packed prompts ---------------------------------------------------------------------------------------------
@@ -93,6 +94,7 @@ struct PackedProblem {
     it.split = 0;
     it.kbase = kb;
     it.held = nk;
+    it.gap0 = it.gap1 = 0;
     return true;
   }
   __device__ bool sees(const RaggedItem& it, int r, int j) const { return j < it.key1 && j <= it.last0 + r; }
@@ -122,8 +124,8 @@ struct PackedProblem {
 };
 
 // ---- trees of drafted tokens ------------------------------------------------------------------------------------
-// Node t < n_nodes[s] of sequence s sits in cache slot ctx[s] + t and sees slots [0, ctx[s]) and those nodes j of its own sequence
-// whose bit is set: word j / 64, bit j % 64 of ancestors[s][t].  The rows of one key/value head are its T * (H / G) pairs of node and
+// Node t < n_nodes[s] of sequence s sits in cache slot ctx[s] + t and sees slots [0, ctx[s]), but for a gap [gap_start[s], gap_end[s]) (what a prompt
+// leaves free of its last page), and those nodes j of its own sequence whose bit is set: word j / 64, bit j % 64 of ancestors[s][t].  The rows of one key/value head are its T * (H / G) pairs of node and
 // query head, node-major, so that K and V are read once for all of them.
 struct TreeProblem {
   static constexpr int kSorted = 64;  // sequences, at most, that are taken from the longest to the shortest
@@ -131,6 +133,7 @@ struct TreeProblem {
   long long q_rs;
   KvView kv;
   const int* ctx;
+  const int *gap_start, *gap_end;      // both NULL: no gaps
   const int* n_nodes;                  // NULL: T everywhere
   const unsigned long long* ancestors; // [B][T][words]
   int words;
@@ -173,6 +176,11 @@ struct TreeProblem {
     it.clear = context;
     it.last0 = 0;
     it.kbase = it.held = 0;
+    it.gap0 = it.gap1 = 0;
+    if (gap_start) {
+      it.gap1 = min(max(gap_end[it.seq], 0), context);
+      it.gap0 = min(max(gap_start[it.seq], 0), it.gap1);
+    }
     return true;
   }
   // order[i]: the i-th longest sequence (B <= kSorted; for a whole warp).
@@ -197,7 +205,7 @@ struct TreeProblem {
     return ancestors + ((long long)it.seq * T + (it.row0 + r) / group) * words;
   }
   __device__ bool sees(const RaggedItem& it, int r, int j) const {
-    if (j < it.clear) return true;
+    if (j < it.clear) return j < it.gap0 || j >= it.gap1;
     const int d = j - it.clear;
     return (mask_row(it, r)[d >> 6] >> (d & 63)) & 1ull;
   }
@@ -207,8 +215,9 @@ struct TreeProblem {
   __device__ const E* q_row(const RaggedItem& it, int r) const {
     return static_cast<const E*>(q) + out_row(it, r) * q_rs + (long long)head(it, r) * D;
   }
-  // Offset of key j, or -1 where the page table names no page: its key and value count as zeros, as they do in the tensor-core kernel.
+  // Offset of key j; -1 in the gap, and where the page table names no page: there key and value count as zeros, as in the tensor-core kernel.
   __device__ long long key_offset(const RaggedItem& it, int j) const {
+    if (j >= it.gap0 && j < it.gap1) return -1;
     const int lp = j / kv.page_tokens, in = j - lp * kv.page_tokens;
     const long long pg = kv.page_table ? (long long)kv.page_table[(long long)it.seq * kv.max_pages + lp] : it.seq;
     if (pg < 0 || (kv.n_pages > 0 && pg >= kv.n_pages)) return -1;
@@ -220,7 +229,9 @@ struct TreeProblem {
     const long long room = (long long)(kv.page_table ? kv.max_pages : 1) * kv.page_tokens;
     for (int s = thread; s < B; s += threads) {
       const int n = n_nodes ? n_nodes[s] : T;
-      if (ctx[s] < 0 || n < 0 || n > T || (long long)ctx[s] + n > room) atomicOr(status, 1);
+      bool bad = ctx[s] < 0 || n < 0 || n > T || (long long)ctx[s] + n > room;
+      if (gap_start) bad |= gap_start[s] < 0 || gap_end[s] < gap_start[s] || gap_end[s] > ctx[s];
+      if (bad) atomicOr(status, 1);
     }
   }
 };

@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
 #pragma unroll
         for (int j = 0; j < KC; ++j) s[i][j] = fmaf(a[i].w, b[j].w, fmaf(a[i].z, b[j].z, fmaf(a[i].y, b[j].y, fmaf(a[i].x, b[j].x, s[i][j]))));
     }
-    const bool masked = j0 + kRgBN > it.clear || j0 + kRgBN > it.key1;
+    const bool masked = j0 + kRgBN > it.clear || j0 + kRgBN > it.key1 || (j0 < it.gap1 && j0 + kRgBN > it.gap0);
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
       const int r = ty * RM + i;

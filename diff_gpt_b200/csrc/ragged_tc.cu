@@ -548,7 +548,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       if (fail || !there) break;
       __syncwarp();
       if (lane == 0) done(taken);
-      const int n = x.n, rows = x.it.rows, clear = x.it.clear;
+      const int n = x.n, rows = x.it.rows, clear = x.it.clear, gap0 = x.it.gap0, gap1 = x.it.gap1;
       // Key from which value rows may hold anything: the end of the sequence's keys.
       const int held_end = TREE ? x.it.key1 : x.it.held;
       float m = -INFINITY, l = 0.f;
@@ -561,13 +561,14 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
           break;
         }
         tc_fence_after();
-        if (__builtin_expect(t0 + kBN > held_end, 0)) {  // clear those rows so that 0 * x stays 0
-          const int held = held_end - t0;
+        const bool in_gap = TREE && t0 < gap1 && t0 + kBN > gap0;
+        if (__builtin_expect(t0 + kBN > held_end || in_gap, 0)) {  // clear those rows so that 0 * x stays 0
+          const int key = t0 + row;
           if (!__all_sync(0xffffffffu, wait_or_abort(bar(iV + (int)buf), ph, abort_flag))) {
             fail = true;
             break;
           }
-          if (half == 0 && row >= held) {
+          if (half == 0 && (key >= held_end || (in_gap && key >= gap0 && key < gap1))) {
 #pragma unroll
             for (int s = 0; s < kSub; ++s) {
               uint4* vrow = reinterpret_cast<uint4*>(sV + buf * kTileBytes + s * kSubBytes + row * 128);
@@ -585,7 +586,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         const int c0 = t0 + half * kHalf;  // key of this thread's first column
         // Bit i: this thread's column i is seen.
         unsigned long long seen = ~0ull;
-        const bool masked = t0 + kBN > clear;
+        const bool masked = t0 + kBN > clear || in_gap;
         if (__builtin_expect(masked, 0)) {
           if constexpr (TREE) {
             const int d0 = c0 - clear;
@@ -599,6 +600,10 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                 seen = word(w) >> s;
                 if (s) seen |= word(w + 1) << (64 - s);
               }
+            }
+            if (in_gap) {
+              const int a = max(gap0 - c0, 0), b = min(gap1 - c0, kHalf);  // columns [a, b)
+              if (a < b) seen &= ~((b < 64 ? (1ull << b) - 1ull : ~0ull) & ~((1ull << a) - 1ull));
             }
             const int left = x.it.key1 - c0;
             if (left < kHalf) seen = left > 0 ? seen & ((1ull << left) - 1ull) : 0ull;

@@ -8,6 +8,7 @@ on the host and nothing falls back to torch ops: a CPU tensor is an error.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import NamedTuple
 
@@ -1203,6 +1204,12 @@ def tree_attn_workspace_bytes(B: int, T: int, H: int, D: int, n_splits: int) -> 
     return int(lib.dgpt_tree_attn_workspace_bytes(B, T, H, D, n_splits))
 
 
+@functools.lru_cache(maxsize=4096)
+def _tree_plan(B: int, T: int, H: int, G: int, D: int, keys: int, code: int) -> tuple[int, int]:
+    n = int(lib.dgpt_tree_attn_splits(B, T, H, G, D, keys, code))
+    return n, int(lib.dgpt_tree_attn_workspace_bytes(B, T, H, D, n))
+
+
 def tree_attn(
     q: torch.Tensor,
     kv: KvLayout,
@@ -1215,6 +1222,8 @@ def tree_attn(
     D: int,
     max_keys: int = 0,
     n_nodes: torch.Tensor | None = None,
+    gap_start: torch.Tensor | None = None,
+    gap_end: torch.Tensor | None = None,
     token_stride: int = 0,
     scale: float | None = None,
     n_splits: int = 0,
@@ -1226,11 +1235,12 @@ def tree_attn(
 
     q, out: [B * T, H * D], draft t of sequence s in row s * T + t; ctx_len: int32 [B], cached tokens before the drafts, which lie in the
     slots behind them; ancestors: int64 [B, T, W] (or [B, T] for W = 1), bit j % 64 of word j / 64 says that the draft sees draft j;
-    n_nodes: int32 [B], drafts of each sequence (None: T; the rows behind are left as they are).  token_stride: elements between a
+    n_nodes: int32 [B], drafts of each sequence (None: T; the rows behind are left as they are); gap_start, gap_end: int32 [B], slots before the
+    drafts that hold nothing (a `PagedKVCache` row's from its prompt's length to `suffix_slot0`).  token_stride: elements between a
     head's consecutive tokens (0: D).  n_splits 0: chosen for about `max_keys` keys a sequence (0: what the layout holds).  workspace: at
     least `tree_attn_workspace_bytes` (None: allocated here).
     """
-    _here(q, ctx_len, ancestors, out, n_nodes, workspace, status)
+    _here(q, ctx_len, ancestors, out, n_nodes, gap_start, gap_end, workspace, status)
     shape = ancestors.shape
     if len(shape) not in (2, 3) or ancestors.dtype is not torch.int64 or not ancestors.is_contiguous():
         raise ValueError("tree_attn: ancestors must be a contiguous int64 tensor [B, T, W]")
@@ -1245,22 +1255,26 @@ def tree_attn(
         qs = os_ = (H * D, 1)
     _i32("ctx_len", ctx_len, (B,))
     _i32("n_nodes", n_nodes, (B,))
+    _i32("gap_start", gap_start, (B,))
+    _i32("gap_end", gap_end, (B,))
     _i32("status", status, (1,))
     code = dtype_code(q)
     if n_splits == 0:
         held = (kv.max_pages if kv.page_table else 1) * kv.page_tokens
-        n_splits = lib.dgpt_tree_attn_splits(B, T, H, G, D, min(max_keys, held) if max_keys > 0 else held, code)
+        n_splits, need = _tree_plan(B, T, H, G, D, min(max_keys, held) if max_keys > 0 else held, code)
+    else:
+        need = tree_attn_workspace_bytes(B, T, H, D, n_splits)
     ws_bytes = 0
-    if n_splits > 1:
+    if need > 0:
         if workspace is None:
-            workspace = q.new_empty(tree_attn_workspace_bytes(B, T, H, D, n_splits), dtype=torch.uint8)
+            workspace = q.new_empty(need, dtype=torch.uint8)
         elif not workspace.is_contiguous():
             raise ValueError("tree_attn: the workspace must be contiguous")
         ws_bytes = workspace.nbytes
     check(
         lib.dgpt_tree_attn(
-            q.data_ptr(), qs[0], C.byref(kv), token_stride or D, ctx_len.data_ptr(), _ptr(n_nodes), ancestors.data_ptr(), words, out.data_ptr(), os_[0],
-            _ptr(workspace), ws_bytes, n_splits, B, T, H, G, D, attn_scale(D) if scale is None else scale, code, impl, _ptr(status), _stream(),
+            q.data_ptr(), qs[0], C.byref(kv), token_stride or D, ctx_len.data_ptr(), _ptr(gap_start), _ptr(gap_end),
+            _ptr(n_nodes), ancestors.data_ptr(), words, out.data_ptr(), os_[0], _ptr(workspace), ws_bytes, n_splits, B, T, H, G, D, attn_scale(D) if scale is None else scale, code, impl, _ptr(status), _stream(),
         )
     )
 

@@ -609,24 +609,25 @@ int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_head_stride,
                      const int32_t* key_starts, int32_t n_seq, int32_t n_rows, int32_t n_keys, int32_t H, int32_t G, int32_t D,
                      float scale, int32_t dtype, int32_t impl, int32_t* status, void* stream);
 
-/* Attention of a tree of drafted tokens over a cache.  Sequence s has ctx_len[s] cached tokens in slots 0 .. ctx_len[s] - 1 and
+/* Attention of a tree of drafted tokens over a cache.  Sequence s has its cached tokens in slots 0 .. ctx_len[s] - 1, but for a gap
+ * gap_start[s] .. gap_end[s] - 1 of slots that hold nothing (what a shared prompt leaves free of its last page; both NULL: none), and
  * n_nodes[s] drafts (NULL: T) in the slots behind them.  Draft t sees every cached token, and draft j of its own sequence where
  * bit j % 64 of ancestors[s][t][j / 64] is set (its ancestors' and its own, for a tree; any mask is allowed).  Bits of drafts from n_nodes[s] on count
  * for nothing.  A draft that sees nothing gets zeros; rows from n_nodes[s] on are left as they are.
  * q, out: device [B * T, H * D], row s * T + t, with row strides that are multiples of 8; kv: keys and values of G heads, query head h
- * reads h / (H / G), consecutive tokens of a head kv_token_stride elements apart; slots behind a sequence's last draft may
- * hold anything, those before it finite numbers; a page number outside the pool stands for zeros.
- * ancestors: device [B][T][words] with 64 * words >= T; T <= 256.  ctx_len, n_nodes: device int32 [B]; status bit 0 is set
- * where they do not fit T or the layout (what does not fit is left out).
+ * reads h / (H / G), consecutive tokens of a head kv_token_stride elements apart; slots behind a sequence's last draft and in the gap may
+ * hold anything, the others finite numbers; a page number outside the pool stands for zeros.
+ * ancestors: device [B][T][words] with 64 * words >= T; T <= 256.  ctx_len, gap_start, gap_end, n_nodes: device int32 [B]; status bit 0 is
+ * set where they do not fit T, the layout or one another (what does not fit is left out).
  * n_splits (1 to 256) splits each sequence's keys; workspace from the _bytes call (not needed for 1), 16-byte aligned.  _splits chooses a
  * number for sequences of about max_keys keys; any number gives the same rows but for the order of their sums.
  * D, impl, status as in dgpt_fmha_packed. */
 int32_t dgpt_tree_attn_splits(int32_t B, int32_t T, int32_t H, int32_t G, int32_t D, int32_t max_keys, int32_t dtype);
 size_t dgpt_tree_attn_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t D, int32_t n_splits);
 int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv_layout* kv, int64_t kv_token_stride,
-                   const int32_t* ctx_len, const int32_t* n_nodes, const uint64_t* ancestors, int32_t words, void* out,
-                   int64_t out_row_stride, void* workspace, size_t workspace_bytes, int32_t n_splits, int32_t B, int32_t T, int32_t H,
-                   int32_t G, int32_t D, float scale, int32_t dtype, int32_t impl, int32_t* status, void* stream);
+                   const int32_t* ctx_len, const int32_t* gap_start, const int32_t* gap_end, const int32_t* n_nodes,
+                   const uint64_t* ancestors, int32_t words, void* out, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                   int32_t n_splits, int32_t B, int32_t T, int32_t H, int32_t G, int32_t D, float scale, int32_t dtype, int32_t impl, int32_t* status, void* stream);
 
 /* Log probability of one given token per row under p = softmax(logits / temperature), the entropy of p (natural logarithms), and the
  * top_k (0 to 32) most probable tokens with their log probabilities, in descending order of the logits, equal ones by index:

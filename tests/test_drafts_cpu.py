@@ -33,12 +33,12 @@ def layout(**wrong):
     return lay
 
 
-def tree(kv=None, q=P, qr=256, ts=64, ctx=P, anc=P, words=1, out=P, ws=None, ws_bytes=0, splits=1, B=2, T=8, H=4, G=2, D=64, scale=0.1, dtype=1, impl=0):
-    return lib.dgpt_tree_attn(q, qr, C.byref(kv or layout()), ts, ctx, None, anc, words, out, 256, ws, ws_bytes, splits, B, T, H, G, D, scale, dtype, impl, None, None)
+def tree(kv=None, q=P, qr=256, ts=64, ctx=P, gap=(None, None), anc=P, words=1, out=P, ws=None, ws_bytes=0, splits=1, B=2, T=8, H=4, G=2, D=64, scale=0.1, dtype=1, impl=0):
+    return lib.dgpt_tree_attn(q, qr, C.byref(kv or layout()), ts, ctx, *gap, None, anc, words, out, 256, ws, ws_bytes, splits, B, T, H, G, D, scale, dtype, impl, None, None)
 
 
 @pytest.mark.parametrize("wrong,code,word", [
-    (dict(q=None), ARG, "NULL"), (dict(anc=None), ARG, "NULL"), (dict(ctx=None), ARG, "NULL"), (dict(T=257, words=5), ARG, "256"), (dict(T=65), ARG, "words"),
+    (dict(q=None), ARG, "NULL"), (dict(anc=None), ARG, "NULL"), (dict(ctx=None), ARG, "NULL"), (dict(gap=(P, None)), ARG, "gap"), (dict(T=257, words=5), ARG, "256"), (dict(T=65), ARG, "words"),
     (dict(words=5), ARG, "words"), (dict(H=5), ARG, "sizes"), (dict(scale=-1.0), ARG, "scale"), (dict(impl=-1), ARG, "impl"), (dict(splits=0), ARG, "n_splits"),
     (dict(splits=257), ARG, "n_splits"), (dict(splits=2), WORKSPACE, "workspace"), (dict(splits=2, ws=P, ws_bytes=100), WORKSPACE, "workspace"),
     (dict(splits=2, ws=P + 4, ws_bytes=10**9), ARG, "aligned"), (dict(qr=250), ARG, "strides"), (dict(qr=128), ARG, "strides"), (dict(ts=60), ARG, "token stride"), (dict(ts=32), ARG, "token stride"),

@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
 
 
-def run(ctx, nodes, T, H, G, D, dtype, impl=0, page=64, layout="heads", n_splits=0, seed=0, bits=None, hole=False, ragged=True, scale=None):
+def run(ctx, nodes, T, H, G, D, dtype, impl=0, page=64, layout="heads", n_splits=0, seed=0, bits=None, hole=False, ragged=True, scale=None, gaps=None):
     """layout: "heads" as PagedKVCache ([page][kv][head][token][D]), "rows" as PagedRowCache ([page][token][keys | values]),
     "dense" without a page table; hole: a page number outside the pool (its keys and values count as zeros)."""
     from diff_gpt_b200 import ops
@@ -28,6 +28,9 @@ def run(ctx, nodes, T, H, G, D, dtype, impl=0, page=64, layout="heads", n_splits
     for b in range(B):
         keys[b, :, need[b] :] = nan  # behind the last draft anything may lie
         vals[b, :, need[b] :] = nan
+        if gaps:  # and in the gap
+            keys[b, :, gaps[b][0] : gaps[b][1]] = nan
+            vals[b, :, gaps[b][0] : gaps[b][1]] = float("inf")
     tokens = 0
     if layout == "dense":
         store = torch.stack([keys, vals], dim=1).cuda()  # [B][kv][G][cap][D]
@@ -64,7 +67,8 @@ def run(ctx, nodes, T, H, G, D, dtype, impl=0, page=64, layout="heads", n_splits
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     i32 = dict(dtype=torch.int32, device="cuda")
     ops.tree_attn(q.cuda(), kv, torch.tensor(ctx, **i32), anc.cuda(), out, H=H, G=G, D=D, max_keys=max(need),
-                  n_nodes=torch.tensor(nodes, **i32) if ragged else None, token_stride=tokens, n_splits=n_splits, impl=impl, status=status, scale=scale)
+                  n_nodes=torch.tensor(nodes, **i32) if ragged else None, token_stride=tokens, n_splits=n_splits, impl=impl, status=status, scale=scale,
+                  gap_start=torch.tensor([a for a, _ in gaps], **i32) if gaps else None, gap_end=torch.tensor([e for _, e in gaps], **i32) if gaps else None)
     torch.cuda.synchronize()
     assert status.item() == 0
     got = out.cpu().view(B, T, H, D)
@@ -76,9 +80,12 @@ def run(ctx, nodes, T, H, G, D, dtype, impl=0, page=64, layout="heads", n_splits
             continue
         see = torch.ones(n, c + n, dtype=torch.bool)
         see[:, c:] = torch.tensor([[(bits[b][t] >> j) & 1 for j in range(n)] for t in range(n)], dtype=torch.bool).view(n, n)
+        held = torch.ones(c + n, dtype=torch.bool)
+        if gaps:
+            held[gaps[b][0] : gaps[b][1]] = False
         for h in range(H):
             kvh = h // (H // G)
-            want = rows(qh[b, :n, h], keys[b, kvh, : c + n], vals[b, kvh, : c + n], see, scale or scale_of(D))
+            want = rows(qh[b, :n, h], keys[b, kvh, : c + n][held], vals[b, kvh, : c + n][held], see[:, held], scale or scale_of(D))
             check_rows(got[b, :n, h], None, want, D, c + n, dtype, dtype == BF and impl != 1)
     return out
 
@@ -144,6 +151,15 @@ def test_masks(D, dtype, n_splits, impl):
 @pytest.mark.parametrize("D,dtype", [(64, BF), (128, BF), (16, F32)])
 def test_pages_outside_the_pool_are_zeros(D, dtype, impl):
     run([300, 100, 200], [5, 5, 5], 5, 4, 2, D, dtype, impl, hole=True, seed=6)
+
+
+@pytest.mark.parametrize("impl", [0, 1])
+@pytest.mark.parametrize("n_splits", [1, 3])
+@pytest.mark.parametrize("D,dtype", [(32, BF), (64, BF), (128, BF), (16, F32)])
+def test_gaps(D, dtype, n_splits, impl):
+    """What a prompt leaves free of its last page: inside a tile, over tiles, whole tiles, at either end, none, and with nothing before it."""
+    gaps = [(100, 128), (120, 400), (128, 384), (0, 70), (300, 300), (299, 300), (0, 300), (64, 65)]
+    run([500, 500, 500, 200, 300, 300, 300, 66], [9, 5, 9, 9, 1, 9, 9, 9], 9, 4, 2, D, dtype, impl, n_splits=n_splits, seed=12, gaps=gaps)
 
 
 @pytest.mark.parametrize("impl", [0, 1])
@@ -234,4 +250,10 @@ def test_wrong_lengths_are_reported(impl):
         out = torch.zeros_like(q)
         ops.tree_attn(q, kv, torch.tensor(ctx, **i32), anc, out, H=H, G=H, D=D, n_nodes=torch.tensor(n, **i32), impl=impl, status=status)
         assert status.item() == 1, (ctx, n)
+        assert bool(torch.isfinite(out).all())
+    for a, e in ((-1, 3), (5, 4), (3, 11)):
+        status = torch.zeros(1, **i32)
+        ops.tree_attn(q, kv, torch.tensor([10, 10], **i32), anc, out, H=H, G=H, D=D, gap_start=torch.tensor([0, a], **i32),
+                      gap_end=torch.tensor([0, e], **i32), impl=impl, status=status)
+        assert status.item() == 1, (a, e)
         assert bool(torch.isfinite(out).all())
