@@ -1,10 +1,12 @@
 // Rows of accepted drafts move to where they belong in the cache: for every sequence s, layer, head, and for keys and values alike,
 //   slot dst[s] + i  <-  slot src[s] + path[s][i],   i < count[s].
-// A copy of rows, bound by memory or, where few rows move, by the launch and the loads that depend on one another: count, path, page, row.
-// A CTA owns 256 columns of 16 bytes of one sequence and all of its rows; it works out once where the rows lie and then reads every row of a
-// column before it writes the first, and columns do not mix: source and target may overlap in any way.  Up to 16 rows are one thread's per
-// column, in registers; more are shared by 32 threads, which wait for one another between reading and writing.
-// (Eight threads per column in all cases, each finding its rows' places itself: 192 sequences, 12 layers, 12 heads of 64, 5 rows each, 95 us; so, 22.)
+// A copy of rows, bound by memory or, where few rows move, by the launch and the loads that depend on one another: count and path, page, row.
+// A CTA owns 256 columns of 16 bytes of one sequence and all of its rows, a thread a column; the CTA works out once where the rows lie.  Eight rows
+// at a time are read into registers before the first of them is written.  That is all the care that source and target need to overlap in any
+// way, unless a row of a later round comes from a slot that an earlier round writes (it cannot where a path's rows only move down or away);
+// then 32 threads share a column, and read all of its rows before they write one.
+// (192 sequences, 12 layers, 12 heads of 64, 5 rows each: 95 us with 32 threads per column throughout, each finding its rows' places itself, 22 with
+// 16 rows in registers and two CTAs an SM, 14.6 so; reading and writing them takes 12.)
 #include "common.cuh"
 
 namespace dgpt {
@@ -18,16 +20,17 @@ struct KeepParams {
   int* status;
 };
 
-constexpr int kKeepCols = 256, kKeepOwn = 16, kKeepMost = 256;
+constexpr int kKeepCols = 256, kKeepRound = 8, kKeepMost = 256;
 
-template <bool MANY>
+template <int MOST>
 __global__ void __launch_bounds__(kKeepCols) kv_keep_kernel(const KeepParams p, const unsigned blocks_per_seq) {
-  __shared__ long long from[MANY ? kKeepMost : kKeepOwn], to[MANY ? kKeepMost : kKeepOwn];  // bytes from a column's base, or -1
+  __shared__ long long from[MOST], to[MOST];  // bytes from a column's base, or -1
   const int s = (int)(blockIdx.x / blocks_per_seq), tid = threadIdx.x;
-  const unsigned block = blockIdx.x % blocks_per_seq;
-  const int asked = p.count[s], n = min(max(asked, 0), p.T);
+  const unsigned block = blockIdx.x - (unsigned)s * blocks_per_seq;
+  const int asked = p.count[s], src = p.src[s], dst = p.dst[s], node = tid < p.T ? p.path[(long long)s * p.T + tid] : 0;
+  const int n = min(max(asked, 0), p.T);
   const int* table = p.kv.page_table ? p.kv.page_table + (long long)s * p.kv.max_pages : nullptr;
-  bool bad = asked != n;
+  bool bad = asked != n, later = false;
   if (tid < n) {
     const long long room = (long long)(table ? p.kv.max_pages : 1) * p.kv.page_tokens;
     auto place = [&](long long slot) -> long long {  // -1: no such slot, or its page is none
@@ -37,52 +40,52 @@ __global__ void __launch_bounds__(kKeepCols) kv_keep_kernel(const KeepParams p, 
       if (pg < 0 || (p.kv.n_pages > 0 && pg >= p.kv.n_pages)) return -1;
       return pg * p.page_bytes + (long long)in * p.token_bytes;
     };
-    const int node = p.path[(long long)s * p.T + tid];
-    const long long a = node < 0 ? -1 : place((long long)p.src[s] + node), b = place((long long)p.dst[s] + tid);
+    const long long a = node < 0 ? -1 : place((long long)src + node), b = place((long long)dst + tid);
     from[tid] = a < 0 || b < 0 ? -1 : a;
     to[tid] = b;
     bad |= a < 0 || b < 0;
+    const long long ahead = (long long)src + node - dst;  // the row whose target is this one's source
+    later = ahead >= 0 && ahead < (tid & ~(kKeepRound - 1));
   }
   if (bad && block == 0 && p.status) atomicOr(p.status, 1);
-  __syncthreads();
+  const bool shared = __syncthreads_or(later) != 0;
   auto base = [&](long long col) -> char* {
-    const int vec = (int)(col % p.vecs);
-    const long long lkh = col / p.vecs, lk = lkh / p.H;
-    return static_cast<char*>(p.kinds > 1 && (lk & 1) ? p.kv.v : p.kv.k) + (p.kinds > 1 ? lk >> 1 : lk) * p.layer_bytes +
-           (lkh - lk * p.H) * p.head_bytes + (long long)vec * 16;
+    const unsigned c = (unsigned)col, lkh = c / (unsigned)p.vecs, lk = lkh / (unsigned)p.H;
+    return static_cast<char*>(p.kinds > 1 && (lk & 1u) ? p.kv.v : p.kv.k) + (long long)(p.kinds > 1 ? lk >> 1 : lk) * p.layer_bytes +
+           (long long)(lkh - lk * (unsigned)p.H) * p.head_bytes + (long long)(c - lkh * (unsigned)p.vecs) * 16;
   };
   const long long col0 = (long long)block * kKeepCols;
-  if (!MANY || n <= kKeepOwn) {
+  if (!shared) {
     if (col0 + tid >= p.columns) return;
     char* at = base(col0 + tid);
-    uint4 x[kKeepOwn];
+    for (int i0 = 0; i0 < n; i0 += kKeepRound) {
+      uint4 x[kKeepRound];
 #pragma unroll
-    for (int i = 0; i < kKeepOwn; ++i)
-      if (i < n && from[i] >= 0) x[i] = *reinterpret_cast<const uint4*>(at + from[i]);
+      for (int i = 0; i < kKeepRound; ++i)
+        if (i0 + i < n && from[i0 + i] >= 0) x[i] = *reinterpret_cast<const uint4*>(at + from[i0 + i]);
 #pragma unroll
-    for (int i = 0; i < kKeepOwn; ++i)
-      if (i < n && from[i] >= 0) *reinterpret_cast<uint4*>(at + to[i]) = x[i];
+      for (int i = 0; i < kKeepRound; ++i)
+        if (i0 + i < n && from[i0 + i] >= 0) *reinterpret_cast<uint4*>(at + to[i0 + i]) = x[i];
+    }
     return;
   }
-  if constexpr (MANY) {
-    constexpr int kRows = kKeepMost / 32;
-    const int row0 = tid >> 3;
-    for (int c = 0; c < kKeepCols && col0 + c < p.columns; c += 8) {
-      const long long col = col0 + c + (tid & 7);
-      const bool on = col < p.columns;
-      char* at = on ? base(col) : nullptr;
-      uint4 x[kRows];
+  constexpr int kRows = (MOST + 31) / 32;
+  const int row0 = tid >> 3;
+  for (int c = 0; c < kKeepCols && col0 + c < p.columns; c += 8) {
+    const long long col = col0 + c + (tid & 7);
+    const bool on = col < p.columns;
+    char* at = on ? base(col) : nullptr;
+    uint4 x[kRows];
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        const int row = row0 + i * 32;
-        if (on && row < n && from[row] >= 0) x[i] = *reinterpret_cast<const uint4*>(at + from[row]);
-      }
-      __syncthreads();  // every row of these columns has been read
+    for (int i = 0; i < kRows; ++i) {
+      const int row = row0 + i * 32;
+      if (on && row < n && from[row] >= 0) x[i] = *reinterpret_cast<const uint4*>(at + from[row]);
+    }
+    __syncthreads();  // every row of these columns has been read
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        const int row = row0 + i * 32;
-        if (on && row < n && from[row] >= 0) *reinterpret_cast<uint4*>(at + to[row]) = x[i];
-      }
+    for (int i = 0; i < kRows; ++i) {
+      const int row = row0 + i * 32;
+      if (on && row < n && from[row] >= 0) *reinterpret_cast<uint4*>(at + to[row]) = x[i];
     }
   }
 }
@@ -125,9 +128,9 @@ extern "C" int dgpt_kv_keep(const dgpt_kv_layout* kv, int64_t kv_token_stride, c
   p.columns = (long long)n_layer * p.kinds * H * p.vecs;
   p.status = status;
   const long long per = (p.columns + kKeepCols - 1) / kKeepCols, blocks = per * B;
-  DGPT_REQUIRE(blocks <= 0x7fffffffll, "kv_keep: too many rows");
+  DGPT_REQUIRE(blocks <= 0x7fffffffll && p.columns <= 0x7fffffffll, "kv_keep: too many rows");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (T <= kKeepOwn) kv_keep_kernel<false><<<(unsigned)blocks, kKeepCols, 0, st>>>(p, (unsigned)per);
-  else kv_keep_kernel<true><<<(unsigned)blocks, kKeepCols, 0, st>>>(p, (unsigned)per);
+  if (T <= 64) kv_keep_kernel<64><<<(unsigned)blocks, kKeepCols, 0, st>>>(p, (unsigned)per);
+  else kv_keep_kernel<kKeepMost><<<(unsigned)blocks, kKeepCols, 0, st>>>(p, (unsigned)per);
   return launch_status("kv_keep");
 }

@@ -1308,9 +1308,8 @@ def token_logprobs(
     _i32("targets", targets, (R,))
     _i32("status", status, (1,))
     k = max(top_k, 0)
-    f32 = torch.float32
-    r = TokenLogprobs(logits.new_empty((R,), dtype=f32), logits.new_empty((R,), dtype=f32), logits.new_empty((R, k), dtype=torch.int32),
-                      logits.new_empty((R, k), dtype=f32))
+    logprob = logits.new_empty(R, dtype=torch.float32)
+    r = TokenLogprobs(logprob, torch.empty_like(logprob), targets.new_empty(R, k), logprob.new_empty(R, k))
     check(
         lib.dgpt_token_logprobs(
             logits.data_ptr(), stride if R > 1 else V, targets.data_ptr(), temperature, r.logprob.data_ptr(), r.entropy.data_ptr(),
