@@ -11,9 +11,10 @@
 //                    half of the head); page numbers are fetched 32 at a time
 //   warp 12, lane 0  issuer: S_g = Q K_g^T into one of two score buffers, O += P_g V_g with P from TMEM.  P V of tile g goes before S of tile
 //                    g + 2, so that the arrival of those scores also says that P_g has been read
-//   warps 0-7        softmax, two threads per row with 64 of a tile's scores each: probabilities against the running maximum in one sweep that
-//                    finds the tile's own maximum too; the two swap that through shared memory, and only where it exceeds the running one by more than 2^8
-//                    is O rescaled and the tile redone
+//   warps 0-7        softmax, 16 rows a warp and four threads a row (tcgen05.ld.16x256b): probabilities against the running maximum in one sweep
+//                    that finds the tile's own maximum too; only where a score exceeds the running one by more than 2^8 is O rescaled and the tile
+//                    redone.  (Two threads per row in different warps, each with half of a tile's columns and its maximum handed over through
+//                    shared memory: 8 x 16 heads of 128 x 4096 631 us, so 588; of 64 614 and 520; 40 mixed prompts 102 and 95.)
 //   warps 8-11       output: row sums from shared memory, O from TMEM, one row per thread
 // (Two CTAs an SM for heads of 64, each with one score buffer, its softmax threads storing the output: 512 prompts of 128 143 us instead of 161, 40 mixed
 // ones 106 instead of 102, 8 of 4096 597 instead of 615; not kept.)
@@ -30,7 +31,7 @@ namespace tc {
 
 constexpr int kRtThreads = 512;
 // Registers per thread: the launch's, and a softmax and a helper thread's after the warpgroups have traded them (an output thread keeps the launch's).
-constexpr int kRtRegs = 128, kRtSoftmaxRegs = 144, kRtHelperRegs = 96;
+constexpr int kRtRegs = 128, kRtSoftmaxRegs = 152, kRtHelperRegs = 80;
 static_assert(2 * kRtSoftmaxRegs + kRtRegs + kRtHelperRegs == 4 * kRtRegs, "the warpgroups share what the launch has");
 constexpr int kRtRing = 8;                                                    // items between the warp that finds them and the last role that reads them
 
@@ -39,6 +40,48 @@ struct RtItem {
   int tile0, n;  // key tiles tile0 .. tile0 + n - 1; n < 0: no more items
 };
 static_assert(sizeof(RtItem) % 4 == 0 && sizeof(RtItem) <= 64, "a ring slot is 64 bytes");
+
+// A warp's 16 rows in the registers of four lanes each: lane t holds of every 8 columns the two from 2 (t % 4) on, of row t / 4 in registers 4 j and
+// 4 j + 1 and of row t / 4 + 8 in 4 j + 2 and 4 j + 3.  A row's maximum and sum are then two shuffles away.
+__device__ __forceinline__ void rows16_ld(uint32_t addr, float (&v)[32]) {  // 64 columns
+  uint32_t r[32];
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(addr)
+               : "memory");
+  tc_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void rows16_ld(uint32_t addr, float (&v)[16]) {  // 32 columns
+  uint32_t r[16];
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(addr)
+               : "memory");
+  tc_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void rows16_ld(uint32_t addr, float (&v)[4]) {  // 8 columns
+  uint32_t r[4];
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  tc_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void rows16_st(uint32_t addr, const float (&v)[16]) {
+  uint32_t r[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(v[i]);
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+// The same rows' columns as pairs of bf16: word t % 4 of every 4, of row t / 4 in register 2 j and of row t / 4 + 8 in 2 j + 1.  32 words.
+__device__ __forceinline__ void rows16_st_pairs(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
 
 // Items are dealt at run time: the grid has a CTA for each, one per SM is resident, and a resident CTA that wants more work cancels one that
 // has not been launched and takes its number (cluster launch control).  Numbers run from a prompt's last rows, which see the most keys, to its
@@ -118,7 +161,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sV = smem + 4 * kTileBytes;  // Q | K0 K1 K2 | V0 V1 | barriers | hand-over words | row sums | items
+  uint8_t* sV = smem + 4 * kTileBytes;  // Q | K0 K1 K2 | V0 V1 | barriers | row sums | items | output | order
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * kTileBytes);
   constexpr int iQ = 0, iQF = 1, iK = 2, iKF = 5, iV = 8, iS = 10, iP = 12, iO = 14, iOF = 16, iL = 17, iLF = 19, iR = 21, iRF = iR + kRtRing,
                 iC = iRF + kRtRing, nBars = iC + 1;
@@ -126,9 +169,8 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
   uint64_t* answer = bars + 44;  // 16-byte aligned
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 43);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile unsigned long long* xch = reinterpret_cast<volatile unsigned long long*>(bars + 48);  // [2 turns][2 halves][128 rows]
-  float* sums = reinterpret_cast<float*>(bars + 48 + 4 * kBM);                                   // [2 items][l of half 0 | of half 1 | m][128 rows]
-  uint8_t* ring = reinterpret_cast<uint8_t*>(sums + 2 * 3 * kBM);                                // [kRtRing] items
+  float* sums = reinterpret_cast<float*>(bars + 48);        // [2 items][l | m][128 rows]
+  uint8_t* ring = reinterpret_cast<uint8_t*>(sums + 2 * 2 * kBM);                                // [kRtRing] items
   const uint32_t aQ = smem_u32(smem), aK = aQ + kTileBytes, aV = aQ + 4 * kTileBytes, bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
 
@@ -140,7 +182,6 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
-  for (int i = tid; i < 4 * kBM; i += kRtThreads) xch[i] = 0ull;  // turn numbers of an earlier CTA must not be taken for this one's
   if constexpr (TREE) {  // rows of Q that no load reaches: level scores keep their warp on the short path
     for (int i = p.rows_per_tile * 8 + tid; i < kBM * 8; i += kRtThreads)
 #pragma unroll
@@ -450,8 +491,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       const int slot = (int)(items & 1u);
       ok = __all_sync(0xffffffffu, wait_asleep(iL + slot, (items >> 1) & 1u)) != 0;
       if (!ok) break;
-      const float* sum = sums + slot * 3 * kBM;
-      const float l = sum[row] + sum[kBM + row], m = sum[2 * kBM + row];
+      const float l = sums[slot * 2 * kBM + row], m = sums[(slot * 2 + 1) * kBM + row];
       mbar_arrive(bar(iLF + slot));
       const unsigned last = g + (unsigned)x.n - 1u;
       ok = __all_sync(0xffffffffu, wait_or_abort(bar(iO + (int)(last & 1u)), (last >> 1) & 1u, abort_flag)) != 0;
@@ -514,33 +554,14 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
     }
     if (!ok && lane == 0 && p.status) atomicOr(p.status, 2);
   } else {
-    // ================= softmax: two threads per row, one for each half of the key tile =================
+    // ================= softmax: 16 rows a warp =================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRtSoftmaxRegs));
-    constexpr int kHalf = kBN / 2;
-    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
-    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int quarter = warp & 3, half = warp >> 2, row0 = quarter * 32 + half * 16;
+    const int row_of[2] = {row0 + (lane >> 2), row0 + (lane >> 2) + 8}, col = 2 * (lane & 3);  // this thread's rows, its first column of every 8
+    const uint32_t lane_addr = tmem + ((uint32_t)row0 << 16);
     const float scale_log2 = p.scale_log2;
-    unsigned g = 0u, turn = 0u, items = 0u;
+    unsigned g = 0u, items = 0u;
     bool fail = false;
-    // Hand-over of one float between the two threads of a row: value and turn number travel in one 8-byte word (a single store, so no
-    // fence is needed), slots alternate, and the reader polls with a clock limit.
-    auto exchange = [&](float mine, bool& ok) -> float {
-      const unsigned xb = turn & 1u;
-      const unsigned long long want = (unsigned long long)(turn + 1u) << 32;
-      xch[(xb * 2 + half) * kBM + row] = want | __float_as_uint(mine);
-      const volatile unsigned long long* partner = xch + (xb * 2 + (half ^ 1)) * kBM + row;
-      ++turn;
-      const long long t_begin = clock64();
-      for (int spin = 0;; ++spin) {
-        const unsigned long long got = *partner;
-        if ((got >> 32) == (want >> 32)) return __uint_as_float((uint32_t)got);
-        if ((spin & 63) == 63 && (*abort_flag || clock64() - t_begin > kWaitLimitCycles)) {
-          if (!*abort_flag) *abort_flag = 2;
-          ok = false;
-          return 0.f;
-        }
-      }
-    };
     for (;; ++taken) {
       bool fine;
       const bool there = take(x, taken, fine);
@@ -551,7 +572,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       const int n = x.n, rows = x.it.rows, clear = x.it.clear, gap0 = x.it.gap0, gap1 = x.it.gap1;
       // Key from which value rows may hold anything: the end of the sequence's keys.
       const int held_end = TREE ? x.it.key1 : x.it.held;
-      float m = -INFINITY, l = 0.f;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // l: of this thread's columns
       int t0 = x.tile0 * kBN;
       for (int j = 0; j < n; ++j, ++g, t0 += kBN) {
         const unsigned buf = g & 1u, ph = (g >> 1) & 1u;
@@ -563,149 +584,198 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         tc_fence_after();
         const bool in_gap = TREE && t0 < gap1 && t0 + kBN > gap0;
         if (__builtin_expect(t0 + kBN > held_end || in_gap, 0)) {  // clear those rows so that 0 * x stays 0
-          const int key = t0 + row;
           if (!__all_sync(0xffffffffu, wait_or_abort(bar(iV + (int)buf), ph, abort_flag))) {
             fail = true;
             break;
           }
+          const int vr = quarter * 32 + lane, key = t0 + vr;
           if (half == 0 && (key >= held_end || (in_gap && key >= gap0 && key < gap1))) {
 #pragma unroll
             for (int s = 0; s < kSub; ++s) {
-              uint4* vrow = reinterpret_cast<uint4*>(sV + buf * kTileBytes + s * kSubBytes + row * 128);
+              uint4* vrow = reinterpret_cast<uint4*>(sV + buf * kTileBytes + s * kSubBytes + vr * 128);
 #pragma unroll
               for (int c = 0; c < 8; ++c) vrow[c] = make_uint4(0u, 0u, 0u, 0u);
             }
             fence_async_smem();
           }
         }
-        if (__builtin_expect(quarter * 32 >= rows, 0)) {  // none of this warp's rows exists: what it leaves in P reaches no other row
+        if (__builtin_expect(row0 >= rows, 0)) {  // none of this warp's rows exists: what it leaves in P reaches no other row
           tc_fence_before();
           mbar_arrive(bar(iP + (int)buf));
           continue;
         }
-        const int c0 = t0 + half * kHalf;  // key of this thread's first column
-        // Bit i: this thread's column i is seen.
-        unsigned long long seen = ~0ull;
+        // What a row sees of the tile, from this thread's first column on.  Prompts: the last column.  Trees: seen[r][c], a bit for each of the
+        // columns from 64 c on.
         const bool masked = t0 + kBN > clear || in_gap;
+        int last[2];
+        unsigned long long seen[2][2];
         if (__builtin_expect(masked, 0)) {
-          if constexpr (TREE) {
-            const int d0 = c0 - clear;
-            if (d0 > -kHalf && row < rows) {
-              const unsigned long long* words = p.mask_row(x.it, row);
-              auto word = [&](int w) { return w < p.words ? words[w] : 0ull; };
-              if (d0 < 0) {
-                seen = (word(0) << -d0) | ((1ull << -d0) - 1ull);
-              } else {
-                const int w = d0 >> 6, s = d0 & 63;
-                seen = word(w) >> s;
-                if (s) seen |= word(w + 1) << (64 - s);
+          if constexpr (!TREE) {
+            // (what Q holds behind the last row is anything; its scores stay as they are)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) last[r] = row_of[r] < rows ? min(x.it.last0 + row_of[r], x.it.key1 - 1) - t0 - col : kBN;
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+              const int c0 = t0 + c * 64;
+              unsigned long long both = ~0ull;  // what neither row sees is cleared
+              const int a = max(gap0 - c0, 0), b = min(gap1 - c0, 64);  // the gap's columns
+              if (in_gap && a < b) both &= ~((b < 64 ? (1ull << b) - 1ull : ~0ull) & ~((1ull << a) - 1ull));
+              const int left = x.it.key1 - c0;
+              if (left < 64) both = left > 0 ? both & ((1ull << left) - 1ull) : 0ull;
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                unsigned long long bits = ~0ull;
+                const int d0 = c0 - clear;
+                if (d0 > -64 && row_of[r] < rows) {
+                  const unsigned long long* words = p.mask_row(x.it, row_of[r]);
+                  auto word = [&](int w) { return w < p.words ? words[w] : 0ull; };
+                  if (d0 < 0) {
+                    bits = (word(0) << -d0) | ((1ull << -d0) - 1ull);
+                  } else {
+                    const int w = d0 >> 6, s = d0 & 63;
+                    bits = word(w) >> s;
+                    if (s) bits |= word(w + 1) << (64 - s);
+                  }
+                }
+                bits = (bits & both) >> col;
+                if (c == 0) seen[r][0] = bits;
+                else seen[r][1] = bits;
               }
             }
-            if (in_gap) {
-              const int a = max(gap0 - c0, 0), b = min(gap1 - c0, kHalf);  // columns [a, b)
-              if (a < b) seen &= ~((b < 64 ? (1ull << b) - 1ull : ~0ull) & ~((1ull << a) - 1ull));
-            }
-            const int left = x.it.key1 - c0;
-            if (left < kHalf) seen = left > 0 ? seen & ((1ull << left) - 1ull) : 0ull;
-          } else {
-            const int n_seen = row < rows ? min(x.it.last0 + row, x.it.key1 - 1) - c0 + 1 : kHalf;
-            if (n_seen < kHalf) seen = n_seen > 0 ? (1ull << n_seen) - 1ull : 0ull;
           }
         }
-        // 32 scores at a time, in loops that stay loops: with all 64 in registers at once, and the code for them, the softmax warps waited for
-        // instructions: 40 prompts of 17 to 1000, 12 heads of 64, 110 us so, 102 in this form; 512 of 128 172 and 161; 8 of 4096, 16 of 128, 618 and 631)
+        // 64 columns at a time, in loops that stay loops: with all of a tile's scores in registers at once, and the code for them, the softmax
+        // warps waited for instructions (40 prompts of 17 to 1000, 12 heads of 64, 110 us so, 102 in this form)
         auto scores = [&](int c, float (&sv)[32]) {
-          tmem_ld32(lane_addr + buf * 128 + half * kHalf + c * 32, sv);
+          rows16_ld(lane_addr + buf * 128 + c * 64, sv);
           if (__builtin_expect(masked, 0)) {
-            const uint32_t bits = c ? (uint32_t)(seen >> 32) : (uint32_t)seen;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) sv[i] = (bits >> i) & 1u ? sv[i] : -INFINITY;
+            for (int r = 0; r < 2; ++r) {
+              const int end = TREE ? 0 : last[r] - c * 64;
+              const unsigned long long bits = !TREE ? 0ull : c ? seen[r][1] : seen[r][0];
+              const uint32_t w[2] = {(uint32_t)bits, (uint32_t)(bits >> 32)};
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const bool sees = TREE ? ((w[i >> 2] >> (8 * (i & 3) + e)) & 1u) != 0u : 8 * i + e <= end;
+                  sv[4 * i + 2 * r + e] = sees ? sv[4 * i + 2 * r + e] : -INFINITY;
+                }
+            }
           }
         };
-        // One sweep turns this thread's scores into probabilities against a reference (log2 domain), writes them as packed bf16 and
-        // returns their sum, and the largest exponent met.
-        auto sweep = [&](float ref, float& top) -> float {
-          const uint64_t scale2 = pack2(scale_log2, scale_log2), negm2 = pack2(-ref, -ref);
+        // One sweep turns this thread's scores into probabilities against references (log2 domain), writes them as packed bf16 and gives
+        // their sums, and the largest exponents met, of its two rows.
+        float sum[2], top[2];
+        auto sweep = [&](float ref0, float ref1) {
+          const uint64_t scale2 = pack2(scale_log2, scale_log2), neg2[2] = {pack2(-ref0, -ref0), pack2(-ref1, -ref1)};
           uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
           float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-          for (int c = 0; c < kHalf / 32; ++c) {
+          for (int c = 0; c < 2; ++c) {
             float sv[32];
             scores(c, sv);
             uint32_t packed[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float x0, x1;
-              unpack2(fma2(pack2(sv[i], sv[i + 1]), scale2, negm2), x0, x1);
-              tops[(i >> 1) & 3] = max3(tops[(i >> 1) & 3], x0, x1);
-              const float p0 = ex2(x0), p1 = ex2(x1);  // -inf -> 0
-              rs2[(i >> 1) & 3] = add2(rs2[(i >> 1) & 3], pack2(p0, p1));
-              const __nv_bfloat162 pk = __floats2bfloat162_rn(p0, p1);
-              packed[i >> 1] = *reinterpret_cast<const uint32_t*>(&pk);
+            for (int i = 0; i < 8; ++i) {
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const int k = 2 * r + (i & 1);
+                float x0, x1;
+                unpack2(fma2(pack2(sv[4 * i + 2 * r], sv[4 * i + 2 * r + 1]), scale2, neg2[r]), x0, x1);
+                tops[k] = max3(tops[k], x0, x1);
+                const float p0 = ex2(x0), p1 = ex2(x1);  // -inf -> 0
+                rs2[k] = add2(rs2[k], pack2(p0, p1));
+                const __nv_bfloat162 pk = __floats2bfloat162_rn(p0, p1);
+                packed[2 * i + r] = *reinterpret_cast<const uint32_t*>(&pk);
+              }
             }
-            tmem_st16(lane_addr + kPCol + buf * 64 + half * (kHalf / 2) + c * 16, packed);
+            rows16_st_pairs(lane_addr + kPCol + buf * 64 + c * 32, packed);
           }
-          float ra, rb, rc, rd;
-          unpack2(add2(rs2[0], rs2[1]), ra, rb);
-          unpack2(add2(rs2[2], rs2[3]), rc, rd);
-          top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-          return (ra + rb) + (rc + rd);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float a, b;
+            unpack2(add2(rs2[2 * r], rs2[2 * r + 1]), a, b);
+            sum[r] = a + b;
+            top[r] = fmaxf(tops[2 * r], tops[2 * r + 1]);
+          }
         };
-        // From an item's second tile on the running maximum is almost always still good (it has to be within 2^8 of the true one), so the
-        // probabilities are taken against it at once and the tile's maximum is found on the way; m is the same in both threads of a row and
-        // so is the decision, and the votes are the same in both of its warps.
-        bool xok = true, settled = false;
-        float mx2, sum = 0.f, top;
-        const bool fast = __all_sync(0xffffffffu, m != -INFINITY);
-        if (__builtin_expect(fast, 1)) {
-          sum = sweep(m, top);
-          mx2 = fmaxf(top, exchange(top, xok)) + m;  // exponents were taken against m
+        auto quad_max = [](float v) {
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+          return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+        };
+        // The running maximum is almost always good enough (it has to be within 2^8 of the true one), so the probabilities are taken against it at
+        // once and the tile's maximum is found on the way.  In an item's first tile the largest of the first 8 scores stands in for it.
+        if (__builtin_expect(!__all_sync(0xffffffffu, m[0] != -INFINITY && m[1] != -INFINITY), 0)) {
+          float v[4];
+          rows16_ld(lane_addr + buf * 128, v);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const bool sees0 = !masked || (TREE ? (seen[r][0] & 1ull) != 0ull : 0 <= last[r]), sees1 = !masked || (TREE ? (seen[r][0] & 2ull) != 0ull : 1 <= last[r]);
+            const float first = quad_max(fmaxf(sees0 ? v[2 * r] : -INFINITY, sees1 ? v[2 * r + 1] : -INFINITY)) * scale_log2;
+            if (m[r] == -INFINITY) m[r] = first;  // (nothing has been added to the row: no product to rescale)
+          }
+        }
+        bool settled = false;
+        float mx2[2];
+        if (__builtin_expect(__all_sync(0xffffffffu, m[0] != -INFINITY && m[1] != -INFINITY), 1)) {
+          sweep(m[0], m[1]);
+          settled = !__any_sync(0xffffffffu, fmaxf(top[0], top[1]) > 8.f);
+          if (settled) {
+            l[0] += sum[0];
+            l[1] += sum[1];
+          } else {
+            mx2[0] = quad_max(top[0]) + m[0];  // exponents were taken against m
+            mx2[1] = quad_max(top[1]) + m[1];
+          }
         } else {
-          float mine = -INFINITY;
+          mx2[0] = mx2[1] = -INFINITY;
 #pragma unroll 1
-          for (int c = 0; c < kHalf / 32; ++c) {
-            float sv[32], mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int c = 0; c < 2; ++c) {
+            float sv[32];
             scores(c, sv);
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
+            for (int r = 0; r < 2; ++r) {
+              float a = -INFINITY, b = -INFINITY;
 #pragma unroll
-              for (int u = 0; u < 4; ++u) mxs[u] = max3(mxs[u], sv[i + 2 * u], sv[i + 2 * u + 1]);
+              for (int i = 0; i < 8; i += 2) {
+                a = max3(a, sv[4 * i + 2 * r], sv[4 * i + 2 * r + 1]);
+                b = max3(b, sv[4 * i + 4 + 2 * r], sv[4 * i + 4 + 2 * r + 1]);
+              }
+              mx2[r] = max3(mx2[r], a, b);
             }
-            mine = fmaxf(mine, fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])));
           }
-          mx2 = fmaxf(mine, exchange(mine, xok)) * scale_log2;
-        }
-        if (!__all_sync(0xffffffffu, xok)) {
-          fail = true;
-          break;
-        }
-        if (fast && !__any_sync(0xffffffffu, mx2 > m + 8.f)) {
-          l += sum;
-          settled = true;
+          mx2[0] = quad_max(mx2[0]) * scale_log2;
+          mx2[1] = quad_max(mx2[1]) * scale_log2;
         }
         if (__builtin_expect(!settled, 0)) {
-          float alpha = 1.f;
-          if (mx2 > m + 8.f || m == -INFINITY) {
-            alpha = m == -INFINITY ? 0.f : ex2(m - mx2);
-            m = mx2;
-          }
-          if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-            // O may only be touched when no product into it is in flight: that of the tile before must be done (this tile's waits for this row)
+          float alpha[2] = {1.f, 1.f};
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            if (mx2[r] > m[r] + 8.f || m[r] == -INFINITY) {
+              alpha[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - mx2[r]);
+              m[r] = mx2[r];
+            }
+          if (j > 0 && __any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+            // O may only be touched when no product into it is in flight: that of the tile before must be done (this tile's waits for these rows)
             if (!__all_sync(0xffffffffu, wait_or_abort(bar(iO + (int)(buf ^ 1u)), ((g - 1) >> 1) & 1u, abort_flag))) {
               fail = true;
               break;
             }
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D / 64; ++c) {
-              float v[32];
-              tmem_ld32(lane_addr + kOCol + half * (D / 2) + c * 32, v);
+            for (int c = 0; c < D / 32; ++c) {
+              float v[16];
+              rows16_ld(lane_addr + kOCol + c * 32, v);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] *= alpha;
-              tmem_st32(lane_addr + kOCol + half * (D / 2) + c * 32, v);
+              for (int i = 0; i < 16; ++i) v[i] *= alpha[(i >> 1) & 1];
+              rows16_st(lane_addr + kOCol + c * 32, v);
             }
           }
-          l = l * alpha + sweep(m == -INFINITY ? 0.f : m, top);
+          sweep(m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]);
+          l[0] = l[0] * alpha[0] + sum[0];
+          l[1] = l[1] * alpha[1] + sum[1];
         }
         tc_wait_st();
         tc_fence_before();
@@ -718,8 +788,15 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         fail = true;
         break;
       }
-      sums[(slot * 3 + half) * kBM + row] = l;
-      if (half == 0) sums[(slot * 3 + 2) * kBM + row] = m;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float t = l[r] + __shfl_xor_sync(0xffffffffu, l[r], 1);
+        t += __shfl_xor_sync(0xffffffffu, t, 2);
+        if ((lane & 3) == 0) {
+          sums[slot * 2 * kBM + row_of[r]] = t;
+          sums[(slot * 2 + 1) * kBM + row_of[r]] = m[r];
+        }
+      }
       mbar_arrive(bar(iL + slot));
       ++items;
     }
@@ -744,7 +821,7 @@ static int ragged_tc_go(const TcMaps& maps, const P& p, long long items, int d_h
     set_error("ragged attention: too many rows");
     return DGPT_E_ARG;
   }
-  size_t smem = (size_t)6 * (D / 64) * kBN * 128 + 48 * 8 + 4 * kBM * 8 + 6 * kBM * 4 + kRtRing * 64 + 4 * 4096 + TreeProblem::kSorted * 4 + 1024;
+  size_t smem = (size_t)6 * (D / 64) * kBN * 128 + 48 * 8 + 4 * kBM * 4 + kRtRing * 64 + 4 * 4096 + TreeProblem::kSorted * 4 + 1024;
   if (smem < 120 * 1024) smem = 120 * 1024;  // one CTA owns an SM: it takes all 512 TMEM columns
   auto kernel = ragged_tc_kernel<D, P, TREE>;
   cudaError_t e = cudaSuccess;
