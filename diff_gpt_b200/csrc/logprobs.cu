@@ -26,6 +26,7 @@ constexpr int kLpMost = 32;       // most top tokens
 constexpr int kLpStream = 256;    // threads that stream a row; a warp more finishes it
 constexpr int kLpCtas = 4;        // of an SM
 constexpr float kLpBig = 1073741824.f;  // 2^30: M is kept within it
+constexpr float kLpCold = 1.17549435e-38f;  // lowest temperature, the smallest normal number: its reciprocal, and that times log2(e), are finite
 constexpr float kLpFar = -1e4f;  // an exponent whose power is 0: keeps 0 times infinity out of the sums
 constexpr int kLpFound = 512;     // tokens found above the bound that are ranked at once
 
@@ -557,7 +558,7 @@ extern "C" int dgpt_token_logprobs(const void* logits, int64_t logits_row_stride
                                    int32_t* status, void* stream) {
   DGPT_REQUIRE(R >= 0 && V > 0 && V <= 0x7fffff00, "token_logprobs: bad sizes");
   DGPT_REQUIRE(top_k >= 0 && top_k <= kLpMost && top_k <= V, "token_logprobs: top_k must be 0 to %d and at most the vocabulary, got %d", kLpMost, top_k);
-  DGPT_REQUIRE(temperature > 0.f && temperature < INFINITY, "token_logprobs: the temperature must be positive and finite");
+  DGPT_REQUIRE(temperature >= kLpCold && temperature < INFINITY, "token_logprobs: the temperature must be finite and at least %g", (double)kLpCold);
   DGPT_REQUIRE(R <= 0x0fffffff, "token_logprobs: too many rows");
   if (dtype != DGPT_F32 && dtype != DGPT_BF16) {
     set_error("token_logprobs: unknown dtype %d", dtype);

@@ -12,6 +12,7 @@ extern "C" int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_h
                                 const int32_t* key_starts, int32_t n_seq, int32_t n_rows, int32_t n_keys, int32_t H, int32_t G, int32_t D,
                                 float scale, int32_t dtype, int32_t impl, int32_t* status, void* stream) {
   DGPT_REQUIRE(n_seq >= 0 && n_rows >= 0 && n_keys >= 0 && H > 0 && G > 0 && H % G == 0, "fmha_packed: bad sizes");
+  DGPT_REQUIRE(n_rows <= kRgMost && n_keys <= kRgMost, "fmha_packed: too many rows");
   DGPT_REQUIRE(key_starts || n_keys == n_rows, "fmha_packed: without starts of their own the keys are as many as the queries");
   DGPT_REQUIRE(scale > 0.f, "fmha_packed: the scale must be positive");
   DGPT_REQUIRE(impl >= 0 && impl <= 2, "fmha_packed: impl must be 0 (choose), 1 (CUDA cores) or 2 (tensor cores)");
@@ -64,7 +65,7 @@ extern "C" int32_t dgpt_tree_attn_splits(int32_t B, int32_t T, int32_t H, int32_
     tiles = rows <= 16 ? 1 : (rows + 63) / 64;
     ctas = 2 * 148;
   }
-  const long long items = (long long)B * G * tiles, fit = ctas / items, most = (max_keys + 255) / 256;
+  const long long items = (long long)B * G * tiles, fit = ctas / items, most = ((long long)max_keys + 255) / 256;
   const long long n = fit < most ? fit : most;
   return (int32_t)(n < 1 ? 1 : n > 256 ? 256 : n);
 }

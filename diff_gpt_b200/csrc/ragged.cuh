@@ -11,6 +11,9 @@
 
 namespace dgpt {
 
+// Rows and keys are counted in 32 bits, with room behind the last one for a tile.
+constexpr long long kRgMost = 0x7fffff00ll;
+
 // One tile of up to BM rows against keys [key0, key1) of a sequence.
 struct RaggedItem {
   int rows;        // rows of the tile that exist
@@ -147,9 +150,10 @@ struct TreeProblem {
   int* status;
 
   __host__ __device__ long long items() const { return (long long)B * G * tiles * n_splits; }  // below 2^31 (the entry point sees to it)
+  __device__ long long room() const { return min((long long)(kv.page_table ? kv.max_pages : 1) * kv.page_tokens, kRgMost); }
   // Keys [0, keys) of a sequence, of which the last `nodes` are drafts.  What does not fit the layout is left out.
   __device__ void lengths(int s, int& context, int& nodes) const {
-    const long long room = (long long)(kv.page_table ? kv.max_pages : 1) * kv.page_tokens;
+    const long long room = this->room();
     context = (int)min((long long)max(ctx[s], 0), room);
     nodes = n_nodes ? min(max(n_nodes[s], 0), T) : T;
     nodes = (int)min((long long)nodes, room - context);
@@ -226,10 +230,9 @@ struct TreeProblem {
   // The first CTA looks at all lengths.
   __device__ void check(int block, int thread, int threads) const {
     if (block != 0 || status == nullptr) return;
-    const long long room = (long long)(kv.page_table ? kv.max_pages : 1) * kv.page_tokens;
     for (int s = thread; s < B; s += threads) {
       const int n = n_nodes ? n_nodes[s] : T;
-      bool bad = ctx[s] < 0 || n < 0 || n > T || (long long)ctx[s] + n > room;
+      bool bad = ctx[s] < 0 || n < 0 || n > T || (long long)ctx[s] + n > room();
       if (gap_start) bad |= gap_start[s] < 0 || gap_end[s] < gap_start[s] || gap_end[s] > ctx[s];
       if (bad) atomicOr(status, 1);
     }

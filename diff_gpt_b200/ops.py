@@ -1132,6 +1132,15 @@ def _here(*ts: torch.Tensor | None) -> None:
             raise RuntimeError(f"tensors must be on the current device (cuda:{at}), got one on {t.device}")
 
 
+def _stored(name: str, kv: KvLayout, dtype: torch.dtype) -> None:
+    """A cache of another type or device would be read outside its storage."""
+    held = getattr(kv, "_keep", ())
+    _here(*held)
+    for t in held[:2]:
+        if t.dtype is not dtype:
+            raise TypeError(f"{name}: a cache of {t.dtype} where {dtype} is expected")
+
+
 def _i32(name: str, t: torch.Tensor | None, shape: tuple[int, ...]) -> None:
     if t is not None and (t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
@@ -1241,6 +1250,7 @@ def tree_attn(
     least `tree_attn_workspace_bytes` (None: allocated here).
     """
     _here(q, ctx_len, ancestors, out, n_nodes, gap_start, gap_end, workspace, status)
+    _stored("tree_attn", kv, q.dtype)
     shape = ancestors.shape
     if len(shape) not in (2, 3) or ancestors.dtype is not torch.int64 or not ancestors.is_contiguous():
         raise ValueError("tree_attn: ancestors must be a contiguous int64 tensor [B, T, W]")
@@ -1274,7 +1284,8 @@ def tree_attn(
     check(
         lib.dgpt_tree_attn(
             q.data_ptr(), qs[0], C.byref(kv), token_stride or D, ctx_len.data_ptr(), _ptr(gap_start), _ptr(gap_end),
-            _ptr(n_nodes), ancestors.data_ptr(), words, out.data_ptr(), os_[0], _ptr(workspace), ws_bytes, n_splits, B, T, H, G, D, attn_scale(D) if scale is None else scale, code, impl, _ptr(status), _stream(),
+            _ptr(n_nodes), ancestors.data_ptr(), words, out.data_ptr(), os_[0], _ptr(workspace), ws_bytes, n_splits, B, T, H, G, D,
+            attn_scale(D) if scale is None else scale, code, impl, _ptr(status), _stream(),
         )
     )
 
@@ -1338,6 +1349,7 @@ def kv_keep(
     src_start[s] + path[s, i] held before the call, i < count[s].  kv: layer 0's storage; path: int32 [B, T], T up to 256; src_start, dst_start,
     count: int32 [B]; layer_stride, token_stride (0: D): elements."""
     _here(src_start, dst_start, path, count, status)
+    _stored("kv_keep", kv, dtype)
     shape = path.shape
     if len(shape) != 2:
         raise ValueError("kv_keep: path must be [B, T]")

@@ -616,10 +616,10 @@ int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_head_stride,
  * for nothing.  A draft that sees nothing gets zeros; rows from n_nodes[s] on are left as they are.
  * q, out: device [B * T, H * D], row s * T + t, with row strides that are multiples of 8; kv: keys and values of G heads, query head h
  * reads h / (H / G), consecutive tokens of a head kv_token_stride elements apart; slots behind a sequence's last draft and in the gap may
- * hold anything, the others finite numbers; a page number outside the pool stands for zeros.
+ * hold anything, the others finite numbers; a page number outside the pool (0 .. n_pages - 1, where the layout states n_pages) stands for zeros.
  * ancestors: device [B][T][words] with 64 * words >= T; T <= 256.  ctx_len, gap_start, gap_end, n_nodes: device int32 [B]; status bit 0 is
  * set where they do not fit T, the layout or one another (what does not fit is left out).
- * n_splits (1 to 256) splits each sequence's keys; workspace from the _bytes call (not needed for 1), 16-byte aligned.  _splits chooses a
+ * n_splits (1 to 256) splits each sequence's keys; workspace from the _bytes call (not needed for 1), 16-byte aligned, one call's at a time.  _splits chooses a
  * number for sequences of about max_keys keys; any number gives the same rows but for the order of their sums.
  * D, impl, status as in dgpt_fmha_packed. */
 int32_t dgpt_tree_attn_splits(int32_t B, int32_t T, int32_t H, int32_t G, int32_t D, int32_t max_keys, int32_t dtype);
@@ -635,7 +635,7 @@ int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv_layout* kv
  * A logit of -inf is a token that cannot come (probability 0, log probability -inf).  A row that holds a NaN or +inf, or nothing but -inf, has no
  * distribution: its numbers are NaN (its top ids are those of its largest logits, NaN behind all others).
  * logits: device [R, V] with row stride, rows on any boundary of their type; targets: device
- * int32 [R]; outputs: fp32 and int32.  A target outside [0, V) gives NaN for its logprob and sets bit 2 of *status (status may be NULL). */
+ * int32 [R]; temperature: from the smallest normal number on; outputs: fp32 and int32.  A target outside [0, V) gives NaN for its logprob and sets bit 2 of *status (status may be NULL). */
 int dgpt_token_logprobs(const void* logits, int64_t logits_row_stride, const int32_t* targets, float temperature, float* logprob,
                         float* entropy, int32_t* top_ids, float* top_logprobs, int32_t top_k, int32_t R, int32_t V, int32_t dtype,
                         int32_t* status, void* stream);
@@ -646,7 +646,7 @@ int dgpt_token_logprobs(const void* logits, int64_t logits_row_stride, const int
  * slots that others read or write.  kv: layer 0's storage (layer l's lies l * layer_stride elements behind it, through the same page
  * table); consecutive tokens of a head kv_token_stride elements apart; k_base == v_base: one storage, moved once.
  * path: device int32 [B, T], T <= 256; src_start, dst_start, count: device int32 [B].  A head's row is a multiple of 16 bytes.  A row whose
- * slots do not exist, or lie in a page outside the pool, is not moved and sets bit 0 of *status, as does a count outside 0 .. T. */
+ * slots do not exist, or lie in a page outside the pool (where the layout states n_pages), is not moved and sets bit 0 of *status, as does a count outside 0 .. T. */
 int dgpt_kv_keep(const dgpt_kv_layout* kv, int64_t kv_token_stride, const int32_t* src_start, const int32_t* dst_start,
                  const int32_t* path, const int32_t* count, int32_t n_layer, int64_t layer_stride, int32_t B, int32_t T, int32_t H,
                  int32_t D, int32_t dtype, int32_t* status, void* stream);

@@ -19,7 +19,7 @@ def packed(q=P, qr=256, qh=64, k=P, kr=128, kh=64, v=P, o=P, orow=256, starts=P,
 @pytest.mark.parametrize("wrong,code,word", [
     (dict(q=None), ARG, "NULL"), (dict(starts=None), ARG, "NULL"), (dict(k=None), ARG, "NULL"), (dict(q=P + 8), ARG, "aligned"), (dict(v=P + 2), ARG, "aligned"),
     (dict(qr=252), ARG, "strides"), (dict(qh=-64), ARG, "strides"), (dict(kh=32), ARG, "strides"), (dict(H=3), ARG, "sizes"), (dict(G=0), ARG, "sizes"),
-    (dict(N=-1), ARG, "sizes"), (dict(M=11), ARG, "starts of their own"), (dict(scale=0.0), ARG, "scale"), (dict(scale=float("nan")), ARG, "scale"),
+    (dict(N=-1), ARG, "sizes"), (dict(N=2**31 - 1, M=2**31 - 1), ARG, "rows"), (dict(M=11), ARG, "starts of their own"), (dict(scale=0.0), ARG, "scale"), (dict(scale=float("nan")), ARG, "scale"),
     (dict(impl=3), ARG, "impl"), (dict(dtype=2), UNSUPPORTED, "dtype"), (dict(D=48), UNSUPPORTED, "head_dim"), (dict(impl=2, dtype=0), UNSUPPORTED, "tensor"),
 ])
 def test_packed_refuses(wrong, code, word):
@@ -56,7 +56,7 @@ def logprobs(logits=P, stride=100, targets=P, T=1.0, out=P, ids=P, k=3, R=2, V=1
 
 @pytest.mark.parametrize("wrong,code,word", [
     (dict(logits=None), ARG, "NULL"), (dict(targets=None), ARG, "NULL"), (dict(ids=None), ARG, "NULL"), (dict(k=33), ARG, "top_k"), (dict(k=-1), ARG, "top_k"),
-    (dict(V=2, k=3), ARG, "top_k"), (dict(V=0), ARG, "sizes"), (dict(R=-1), ARG, "sizes"), (dict(T=0.0), ARG, "temperature"), (dict(T=float("inf")), ARG, "temperature"),
+    (dict(V=2, k=3), ARG, "top_k"), (dict(V=0), ARG, "sizes"), (dict(R=-1), ARG, "sizes"), (dict(T=0.0), ARG, "temperature"), (dict(T=1e-39), ARG, "temperature"), (dict(T=float("inf")), ARG, "temperature"),
     (dict(T=float("nan")), ARG, "temperature"), (dict(stride=99), ARG, "overlap"), (dict(logits=P + 1), ARG, "aligned"), (dict(dtype=3), UNSUPPORTED, "dtype"),
 ])
 def test_logprobs_refuses(wrong, code, word):
@@ -70,6 +70,7 @@ def keep(kv=None, ts=64, src=P, path=P, L=2, stride=1024, B=2, T=8, H=4, D=64, d
 @pytest.mark.parametrize("wrong,code,word", [
     (dict(src=None), ARG, "NULL"), (dict(path=None), ARG, "NULL"), (dict(T=257), ARG, "256"), (dict(L=0), ARG, "sizes"), (dict(D=4), ARG, "16 bytes"),
     (dict(ts=32), ARG, "strides"), (dict(stride=1001), ARG, "strides"), (dict(dtype=5), UNSUPPORTED, "dtype"), (dict(kv=layout(n_pages=-1)), ARG, "negative"),
+    (dict(kv=layout(head_stride=0)), ARG, "apart"), (dict(stride=0), ARG, "apart"),
 ])
 def test_keep_refuses(wrong, code, word):
     assert keep(**wrong) == code and word in _lib.last_error()
@@ -104,6 +105,17 @@ def test_the_wrappers_refuse_cpu_tensors():
         ops.token_logprobs(q.view(4, 128), torch.zeros(4, dtype=torch.int32))
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         ops.kv_keep(layout(), i, i, torch.zeros(2, 2, dtype=torch.int32), i, n_layer=1, layer_stride=0, H=1, D=8, dtype=torch.float32)
+
+
+def test_a_cache_of_another_type_or_place_is_refused(monkeypatch):
+    lay = layout()
+    lay._keep = (torch.zeros(8), torch.zeros(8), None)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ops._stored("tree_attn", lay, torch.float32)
+    monkeypatch.setattr(ops, "_here", lambda *ts: None)
+    ops._stored("tree_attn", lay, torch.float32)
+    with pytest.raises(TypeError, match="cache of torch.float32"):
+        ops._stored("tree_attn", lay, torch.bfloat16)
 
 
 def test_slots_of_packed_prompts_never_collide():

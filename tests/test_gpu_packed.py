@@ -121,6 +121,20 @@ def test_scales(scale, D, dtype, impl):
     run([500, 260], 2, 2, D, dtype, impl, scale=scale, seed=6)
 
 
+@pytest.mark.parametrize("impl", [0, 1])
+@pytest.mark.parametrize("D,dtype", [(32, BF), (64, BF), (128, BF), (16, F32)])
+def test_heads_before_rows(D, dtype, impl):
+    """A head's rows side by side, as a cache lays them out: the same numbers as with a row's heads side by side."""
+    from diff_gpt_b200 import ops
+
+    H, G, starts = 4, 2, torch.tensor([0, 130, 131, 131, 300], dtype=torch.int32, device="cuda")
+    q, k, v = (torch.randn(h, 300, D, device="cuda").to(dtype) for h in (H, G, G))
+    o, want, lse, want_lse = torch.empty_like(q), q.new_empty(300, H, D), torch.empty(300, H, device="cuda"), torch.empty(300, H, device="cuda")
+    ops.fmha_packed(*(x.transpose(0, 1) for x in (q, k, v)), starts, o.transpose(0, 1), lse=lse, impl=impl)
+    ops.fmha_packed(*(x.transpose(0, 1).contiguous() for x in (q, k, v)), starts, want, lse=want_lse, impl=impl)
+    assert torch.equal(o.transpose(0, 1), want) and torch.equal(lse, want_lse)
+
+
 @pytest.mark.parametrize("D,dtype", [(64, BF), (128, BF), (16, F32)])
 def test_rising_scores(D, dtype):
     """Scores that grow along the prompt: the running maximum moves in every tile."""
