@@ -7,7 +7,7 @@
 // probabilities whatever item they belong to, loads run ahead of those, and a warpgroup of its own takes a finished item's output out
 // of TMEM while the softmax threads are at the next one.
 //   warp 14          items
-//   warp 13          loader: TMA loads of Q, and of K and V tiles into rings of 3 and 2 slots (128-byte swizzle, one box per page and 64-wide
+//   warp 13          loader: TMA loads of Q, K and V tiles into two slots of each (128-byte swizzle, one box per page and 64-wide
 //                    half of the head); page numbers are fetched 32 at a time
 //   warp 12, lane 0  issuer: S_g = Q K_g^T into one of two score buffers, O += P_g V_g with P from TMEM.  P V of tile g goes before S of tile
 //                    g + 2, so that the arrival of those scores also says that P_g has been read
@@ -33,6 +33,7 @@ constexpr int kRtThreads = 512;
 // Registers per thread: the launch's, and a softmax and a helper thread's after the warpgroups have traded them (an output thread keeps the launch's).
 constexpr int kRtRegs = 128, kRtSoftmaxRegs = 152, kRtHelperRegs = 80;
 static_assert(2 * kRtSoftmaxRegs + kRtRegs + kRtHelperRegs == 4 * kRtRegs, "the warpgroups share what the launch has");
+constexpr int kRtLead = 3;                                                    // key tiles still to be loaded when the next item is asked for
 constexpr int kRtRing = 8;                                                    // items between the warp that finds them and the last role that reads them
 
 struct RtItem {
@@ -161,22 +162,24 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sV = smem + 4 * kTileBytes;  // Q | K0 K1 K2 | V0 V1 | barriers | row sums | items | output | order
+  uint8_t* sV = smem + 4 * kTileBytes;  // Q0 Q1 | K0 K1 | V0 V1 | barriers | row sums | items | output | order
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * kTileBytes);
-  constexpr int iQ = 0, iQF = 1, iK = 2, iKF = 5, iV = 8, iS = 10, iP = 12, iO = 14, iOF = 16, iL = 17, iLF = 19, iR = 21, iRF = iR + kRtRing,
+  constexpr int iQ = 0, iQF = 2, iK = 4, iKF = 6, iV = 8, iS = 10, iP = 12, iO = 14, iOF = 16, iL = 17, iLF = 19, iR = 21, iRF = iR + kRtRing,
                 iC = iRF + kRtRing, nBars = iC + 1;
-  static_assert(nBars <= 43, "barriers, an answer of 16 bytes and two words in 46 words");
+  static_assert(nBars <= 43, "barriers, an answer of 16 bytes and three words in 48 words");
   uint64_t* answer = bars + 44;  // 16-byte aligned
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 43);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile unsigned* loaded = reinterpret_cast<volatile unsigned*>(bars + 46);  // K tiles asked for
   float* sums = reinterpret_cast<float*>(bars + 48);        // [2 items][l | m][128 rows]
   uint8_t* ring = reinterpret_cast<uint8_t*>(sums + 2 * 2 * kBM);                                // [kRtRing] items
-  const uint32_t aQ = smem_u32(smem), aK = aQ + kTileBytes, aV = aQ + 4 * kTileBytes, bar0 = smem_u32(bars);
+  const uint32_t aQ = smem_u32(smem), aK = aQ + 2 * kTileBytes, aV = aQ + 4 * kTileBytes, bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     *abort_flag = 0;
+    *loaded = 0u;
     for (int i = 0; i < nBars; ++i)
       mbar_init(bar(i), (i == iP || i == iP + 1 || i == iL || i == iL + 1) ? 2 * kBM : (i == iOF || i == iLF || i == iLF + 1) ? kBM : i >= iRF && i < iC ? 14 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -185,7 +188,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
   if constexpr (TREE) {  // rows of Q that no load reaches: level scores keep their warp on the short path
     for (int i = p.rows_per_tile * 8 + tid; i < kBM * 8; i += kRtThreads)
 #pragma unroll
-      for (int s = 0; s < kSub; ++s) reinterpret_cast<uint4*>(smem + s * kSubBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int s = 0; s < 2 * kSub; ++s) reinterpret_cast<uint4*>(smem + s * kSubBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
     fence_async_smem();
   }
   if (warp == 0) {
@@ -298,27 +301,30 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       bool more = take_all(y, ahead);
       auto load_k = [&]() {
         if (kj == 0) {
-          if (items > 0) ok = wait(iQF, (items - 1) & 1u);  // the last S of the item before is done
+          const unsigned qs = items & 1u;
+          if (items >= 2) ok = wait(iQF + (int)qs, ((items - 2) >> 1) & 1u);  // the last S of the item before last is done
           if (!ok) return;
           if (lane == 0) {
+            const uint32_t full = bar(iQ + (int)qs), to = aQ + qs * kTileBytes;
             if constexpr (TREE) {
-              mbar_expect_tx(bar(iQ), (uint32_t)(p.rows_per_tile * 128 * kSub));
+              mbar_expect_tx(full, (uint32_t)(p.rows_per_tile * 128 * kSub));
 #pragma unroll
-              for (int s = 0; s < kSub; ++s) tma_load_4d(aQ + s * kSubBytes, &mq, bar(iQ), s * 64, y.it.h, y.it.row0 / p.group, y.it.seq);
+              for (int s = 0; s < kSub; ++s) tma_load_4d(to + s * kSubBytes, &mq, full, s * 64, y.it.h, y.it.row0 / p.group, y.it.seq);
             } else {
-              mbar_expect_tx(bar(iQ), kTileBytes);
+              mbar_expect_tx(full, kTileBytes);
 #pragma unroll
-              for (int s = 0; s < kSub; ++s) tma_load_4d(aQ + s * kSubBytes, &mq, bar(iQ), s * 64, y.it.h, y.it.row0, 0);
+              for (int s = 0; s < kSub; ++s) tma_load_4d(to + s * kSubBytes, &mq, full, s * 64, y.it.h, y.it.row0, 0);
             }
           }
           ++items;
         }
-        const unsigned ks = kn % 3u, ku = kn / 3u;
+        const unsigned ks = kn & 1u, ku = kn >> 1;
         if (ku > 0) ok = wait(iKF + (int)ks, (ku - 1) & 1u);
         if (!ok) return;
         if constexpr (TREE) find_pages(y, y.tile0 + kj);
         load_tile(&mk, aK + ks * kTileBytes, bar(iK + (int)ks), y, y.tile0 + kj, newer);
         ++kn;
+        if (lane == 0) *loaded = kn;
         if (++kj == y.n) {
           kj = 0;
           more = take_all(y, ahead);
@@ -340,8 +346,8 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       }
       if (!ok || *abort_flag) {  // something ran out of time: give the copies still in flight a bounded chance to land
         if (lane == 0 && p.status) atomicOr(p.status, 2);
-        if (items > 0) mbar_wait(bar(iQ), (items - 1) & 1u);
-        for (unsigned i = 0; i < 3u && i < kn; ++i) mbar_wait(bar(iK + (int)((kn - 1 - i) % 3u)), ((kn - 1 - i) / 3u) & 1u);
+        for (unsigned i = 0; i < 2u && i < items; ++i) mbar_wait(bar(iQ + (int)((items - 1 - i) & 1u)), ((items - 1 - i) >> 1) & 1u);
+        for (unsigned i = 0; i < 2u && i < kn; ++i) mbar_wait(bar(iK + (int)((kn - 1 - i) & 1u)), ((kn - 1 - i) >> 1) & 1u);
         for (unsigned i = 0; i < 2u && i < vn; ++i) mbar_wait(bar(iV + (int)((vn - 1 - i) & 1u)), ((vn - 1 - i) >> 1) & 1u);
       }
     } else if (warp == 12) {
@@ -354,21 +360,21 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         bool ok = true;
         auto take_one = [&](RtItem& z, unsigned& at) -> bool { return take(z, at++, ok); };
         bool more = take_one(y, ahead);
-        auto issue_s = [&]() {  // S(sg & 1) = Q K(sg % 3)^T
+        auto issue_s = [&]() {  // S(sg & 1) = Q K(sg & 1)^T
           if (sj == 0) {
-            ok = wait_or_abort(bar(iQ), items & 1u, abort_flag);
+            ok = wait_or_abort(bar(iQ + (int)(items & 1u)), (items >> 1) & 1u, abort_flag);
             ++items;
           }
-          const unsigned ks = sg % 3u, buf = sg & 1u;
-          ok = ok && wait_or_abort(bar(iK + (int)ks), (sg / 3u) & 1u, abort_flag);
+          const unsigned qs = (items - 1u) & 1u, buf = sg & 1u;
+          ok = ok && wait_or_abort(bar(iK + (int)buf), (sg >> 1) & 1u, abort_flag);
           if (!ok) return;
           tc_fence_after();
-          umma_ss_chain<D / 16>(tmem + buf * 128, dQK + (aQ >> 4), dQK + ((aK + ks * kTileBytes) >> 4), kIdescS, kSubBytes >> 4);
+          umma_ss_chain<D / 16>(tmem + buf * 128, dQK + ((aQ + qs * kTileBytes) >> 4), dQK + ((aK + buf * kTileBytes) >> 4), kIdescS, kSubBytes >> 4);
           umma_commit(bar(iS + (int)buf));
-          umma_commit(bar(iKF + (int)ks));
+          umma_commit(bar(iKF + (int)buf));
           ++sg;
           if (++sj == y.n) {
-            umma_commit(bar(iQF));  // Q may be overwritten
+            umma_commit(bar(iQF + (int)qs));  // Q may be overwritten
             sj = 0;
             more = take_one(y, ahead);
           }
@@ -399,31 +405,39 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       }
     } else if (warp == 14) {
       // ================= items =================
-      // An item is asked for when it will be wanted soon and not before, so that none waits behind a long one while another SM idles: beside
-      // the oldest unfinished item there is one more, or as many as make up three key tiles.  (No fewer: the issuer's score cursor is two
-      // tiles ahead of its products and waits for the next item before it goes on, the loader's K cursor one.  The items that they hold
-      // unfinished then have at most two tiles behind the oldest one's, so the next one is always on its way.  Items without a key never get here.)
+      // An item is asked for when it will be wanted soon and not before, so that none waits behind a long one while another SM idles: when no more
+      // than kRtLead key tiles are left to load.  (The issuer's score cursor and the loader's K cursor wait for the next item before they go on with what
+      // they have; both have passed the last tile's K by then, so the next item is always on its way.  Items without a key never get here.  48 trees
+      // of up to 32 drafts behind 300 to 4000 keys: the first SM done at 32, the last at 74 us with an item in store from the start; all of it 53 instead of 69.)
       std::conditional_t<TREE, TreeItems, PackedItems> items(p, reinterpret_cast<int*>(ring + kRtRing * 64 + 4 * 4096), lane);
       unsigned at = 0u, freed = 0u, asked = 0u, cta = blockIdx.x;  // items handed out, items finished
-      int ahead = 0;                                               // key tiles of those behind the oldest unfinished one
+      unsigned handed = 0u;                                        // key tiles of the items handed out
       bool ok = true, more = true;
-      auto make_room = [&](bool full_only) {
-        while (ok && at - freed >= (full_only ? (unsigned)kRtRing : 2u) && (full_only || ahead >= 3 || at - freed >= kRtRing)) {
+      auto push = [&]() {
+        if (at - freed >= (unsigned)kRtRing) {
           ok = __all_sync(0xffffffffu, wait_asleep(iRF + (int)(freed % kRtRing), (freed / kRtRing) & 1u)) != 0;
           ++freed;
-          if (ok && at > freed) ahead -= reinterpret_cast<const RtItem*>(ring + (freed % kRtRing) * 64)->n;
         }
-      };
-      auto push = [&]() {
-        make_room(true);
         if (!ok) return;
         if (lane == 0) {
           *reinterpret_cast<RtItem*>(ring + (at % kRtRing) * 64) = x;
           mbar_arrive(bar(iR + (int)(at % kRtRing)));
         }
         __syncwarp();
-        if (at > freed) ahead += x.n;
+        handed += (unsigned)x.n;
         ++at;
+      };
+      auto wanted = [&]() -> bool {  // whether the next item was wanted before the time ran out
+        const long long t0 = clock64();
+        while (handed - *loaded > (unsigned)kRtLead) {
+          if (*abort_flag) return false;
+          if (clock64() - t0 > kWaitLimitCycles) {
+            *abort_flag = 2;
+            return false;
+          }
+          __nanosleep(100);
+        }
+        return true;
       };
       while (ok && more) {
         if (items.get(cta, x.it, lane)) {
@@ -432,7 +446,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
           if (x.n > 0) push();
           else no_keys<P, TREE>(p, x.it, d_head, lane);
         }
-        make_room(false);
+        ok = __all_sync(0xffffffffu, wanted()) != 0;
         if (!ok) break;
         if (lane == 0) ask_for_cta(smem_u32(answer), bar(iC));
         if (!__all_sync(0xffffffffu, mbar_wait(bar(iC), asked & 1u))) {
