@@ -6,7 +6,7 @@
 // way, unless a row of a later round comes from a slot that an earlier round writes (it cannot where a path's rows only move down or away);
 // then 32 threads share a column, and read all of its rows before they write one.
 // (192 sequences, 12 layers, 12 heads of 64, 5 rows each: 95 us with 32 threads per column throughout, each finding its rows' places itself, 22 with
-// 16 rows in registers and two CTAs an SM, 14.6 so; reading and writing them takes 12.)
+// 16 rows in registers and two CTAs an SM, 14 to 15 so; reading and writing them takes 12.)
 #include "common.cuh"
 
 namespace dgpt {
@@ -20,8 +20,9 @@ struct KeepParams {
   int* status;
 };
 
-constexpr int kKeepCols = 256, kKeepRound = 8, kKeepMost = 256;
+constexpr int kKeepCols = 256, kKeepRound = 8, kKeepMost = 256;  // columns of a CTA, rows of a round, rows of a sequence
 
+// MOST: rows of a sequence.  (Up to 64: the shared path's rows then take fewer registers of everyone; 8 drafts of 192 sequences 9.8 us for 10.5.)
 template <int MOST>
 __global__ void __launch_bounds__(kKeepCols) kv_keep_kernel(const KeepParams p, const unsigned blocks_per_seq) {
   __shared__ long long from[MOST], to[MOST];  // bytes from a column's base, or -1
@@ -98,7 +99,7 @@ extern "C" int dgpt_kv_keep(const dgpt_kv_layout* kv, int64_t kv_token_stride, c
                             const int32_t* path, const int32_t* count, int32_t n_layer, int64_t layer_stride, int32_t B, int32_t T, int32_t H,
                             int32_t D, int32_t dtype, int32_t* status, void* stream) {
   DGPT_REQUIRE(B >= 0 && T >= 0 && n_layer > 0 && H > 0 && D > 0, "kv_keep: bad sizes");
-  DGPT_REQUIRE(T <= 256, "kv_keep: at most 256 rows per sequence, got %d", T);
+  DGPT_REQUIRE(T <= kKeepMost, "kv_keep: at most 256 rows per sequence, got %d", T);
   if (dtype != DGPT_F32 && dtype != DGPT_BF16) {
     set_error("kv_keep: unknown dtype %d", dtype);
     return DGPT_E_UNSUPPORTED;

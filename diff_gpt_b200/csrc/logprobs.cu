@@ -543,10 +543,14 @@ static int logprobs_go(const LpParams& p, int log_cluster, cudaStream_t st) {
 template <typename T>
 static int logprobs_launch(const LpParams& p, cudaStream_t st) {
   const int vecs = p.V / (Io<T>::kVec16 * kLpStream);  // of a thread, with one CTA a row
-  // one row's vectors over more CTAs while there are SMs without one and each thread keeps a vector
+  // One row's vectors over more CTAs while there are SMs for them and the row is long enough for what a cluster costs, its two barriers and with top
+  // tokens the lists that are joined.  (13 rows of bf16, top 5, us with 1, 2, 4 and 8 CTAs a row: V = 16384 5.8 6.4 6.7 8.2, 32768 7.3 7.1 7.0 8.3, 65536
+  // 10.1 8.9 7.7 8.9; without top tokens 4.0 4.2 4.0 3.8, 5.2 5.0 4.2 4.1, 7.7 6.3 5.0 4.4.)
   int log = 0;
-  while (log < 3 && ((long long)p.R << (log + 1)) <= 296 && vecs >= 2 << log) ++log;
-  return vecs >> log >= 4 ? logprobs_go<T, 4>(p, log, st) : logprobs_go<T, 1>(p, log, st);
+  while (log < (p.k > 0 ? 2 : 3) && ((long long)p.R << (log + 1)) <= 296 && vecs >= (p.k > 0 ? 16 : 12) << log) ++log;
+  // Four vectors a thread on their way, or one where rows are short and the last of a row would mostly be waited for in vain.  (4096 rows of bf16, top 5, us
+  // with four and one: V = 4096 36.6 29.6, 12288 47.6 42.2, 16384 49.1 50.5, 32768 72.1 79.6; one of 128000 fp32 19.1 26.3.)
+  return vecs >> log >= 8 ? logprobs_go<T, 4>(p, log, st) : logprobs_go<T, 1>(p, log, st);
 }
 
 }  // namespace dgpt

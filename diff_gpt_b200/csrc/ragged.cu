@@ -51,7 +51,9 @@ extern "C" int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_h
 }
 
 // One round of CTAs: a share is as long as its sequences allow.  The tensor-core kernel takes 128 rows an item and one CTA an SM, the other
-// 16 or 64 rows and two CTAs or more; a share below two tiles would wait for the second pass longer than it saves.
+// 16 or 64 rows and two CTAs or more; a share below two tiles would wait for the second pass longer than it saves, and so do shares beyond one
+// round, which write and read partial rows for nothing.  (bf16, us: 3 sequences of 40000 to 65000 keys, 64 drafts, 1 share 503, 6 as chosen 99, 8 134; 48 of 300 to
+// 4000, 1 as chosen 54, 2 75; 8 of them 47, 4 as chosen 24, 8 28; one draft behind 2000 keys 26, 8 as chosen 13.6.)
 extern "C" int32_t dgpt_tree_attn_splits(int32_t B, int32_t T, int32_t H, int32_t G, int32_t D, int32_t max_keys, int32_t dtype) {
   if (B <= 0 || T <= 0 || H <= 0 || G <= 0 || H % G != 0 || max_keys <= 0) return 1;
   const bool tensor = dtype == DGPT_BF16 && D >= 32;
