@@ -9,14 +9,15 @@
 // The top tokens come from the same pass.  A token's key is its logit, made an unsigned number of the same order, above the
 // complement of its index: keys differ, and ties go to the lower index.  Each thread knows the vector with its largest logit; the k-th
 // largest of 32 maxima over groups of threads is a key that at least k tokens reach, so the top k lie among the tokens that reach it:
-// a few dozen, all read by the few threads whose own maximum reaches it.  Those threads' vectors are read again (from L2, one in twenty or so of the row)
+// a few dozen.  A thread also keeps the largest logit of every fourth round; the rounds whose largest reaches the bound are read again (from L1 or L2, one
+// vector in thirty of the row; all rounds of such threads, one in eight, 93 us for 84 with 20 of 32001)
 // and the tokens found are ranked by counting.
 //
 // Eight warps of a CTA stream a row, a ninth finishes it (sums, top tokens, outputs) while they are at the next one; rows are handed over through
 // two buffers.  A cluster of 1 to 8 CTAs shares a row where rows are few; its first CTA joins the others' sums and lists through distributed shared memory.
 // What bounds it: one read of the logits, then the exponentials (16 a clock and SM: three quarters of a read's time in bf16) and the instructions
 // around them, which is why pairs share them (fma, add, max) and the next vectors are on their way while these are worked on.  4096 rows of
-// 32001 bf16 logits: 60 us without top tokens, 75 with 5, 93 with 20; their reading alone takes 40.5.  (A CTA of 256 threads per row whose every warp goes through
+// 32001 bf16 logits: 61 us without top tokens, 76 with 5, 84 with 20; their reading alone takes 40.5.  (A CTA of 256 threads per row whose every warp goes through
 // every phase: 132 with 20.)
 #include "common.cuh"
 
@@ -201,19 +202,17 @@ __device__ __forceinline__ void lp_rank(unsigned long long* keys, int n, unsigne
   if (lane < 8) keys[n + lane] = 0ull;  // up to whole rounds
   if (lane < k) best[lane] = 0ull;
   __syncwarp();
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    const unsigned long long a = i0 + lane < n ? keys[i0 + lane] : 0ull, b = i0 + 32 + lane < n ? keys[i0 + 32 + lane] : 0ull;
-    int over_a = 0, over_b = 0;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const unsigned long long a = i0 + lane < n ? keys[i0 + lane] : 0ull;
+    int over = 0;
     for (int j = 0; j < n; j += 8) {
 #pragma unroll
       for (int u = 0; u < 8; u += 2) {
         const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(keys + j + u);
-        over_a += (o.x > a) + (o.y > a);
-        over_b += (o.x > b) + (o.y > b);
+        over += (o.x > a) + (o.y > a);
       }
     }
-    if (a != 0ull && over_a < k) best[over_a] = a;
-    if (b != 0ull && over_b < k) best[over_b] = b;
+    if (a != 0ull && over < k) best[over] = a;
   }
   __syncwarp();
 }
@@ -226,11 +225,12 @@ __device__ __forceinline__ void lp_bar_arrive(int which) { asm volatile("bar.arr
 template <typename T, int UNROLL>
 __global__ void __launch_bounds__(kLpStream + 32, kLpCtas) token_logprobs_kernel(const LpParams p, const int log_cluster) {
   constexpr int VEC = Io<T>::kVec16, STREAM = kLpStream, WARPS = STREAM / 32;
+  constexpr int PARTS = UNROLL > 1 ? 4 : 1;  // of a thread's rounds, looked at again one by one (in short rows all together)
   constexpr int kFull = 1, kFree = 3;  // named barriers, one per buffer
   constexpr int kStream = 5;
   __shared__ unsigned long long lows[2][STREAM];                        // what the key of each streaming thread's largest logit is at least
   __shared__ __align__(16) unsigned long long groups[32];
-  __shared__ unsigned char owners[WARPS][32];
+  __shared__ unsigned char owners[WARPS][32 * PARTS];                   // threads and parts of their rounds
   __shared__ __align__(16) unsigned long long founds[2][kLpFound + 8];  // tokens that reach the bound
   __shared__ int mets[2];                                               // how many do (there may be more than there is room for)
   __shared__ unsigned long long limits[2];                              // the bound
@@ -281,6 +281,8 @@ __global__ void __launch_bounds__(kLpStream + 32, kLpCtas) token_logprobs_kernel
       const LpRow<T> row = row_of(r);
       const int v0 = part(row, rank), v1 = part(row, rank + 1);
       int top_vec = -1;
+      // Largest logits of rounds r, r + 4, ..: the upper halves of their numbers, the last round's lowest
+      uint32_t part_lo = 0xff80ff80u, part_hi = 0xff80ff80u;
       LpStat a = {-INFINITY, -kLpBig, 0.f, 0.f};
       auto meet = [&](float vm, int vec) {
         if (vm > a.m || (top_vec < 0 && vm == vm)) {  // the first of equal ones stays
@@ -341,7 +343,14 @@ __global__ void __launch_bounds__(kLpStream + 32, kLpCtas) token_logprobs_kernel
           for (int u = 1; u < UNROLL; ++u)
             if (base + u * STREAM >= v1) now[u] = make_uint4(row.kNothing, row.kNothing, row.kNothing, row.kNothing);
         }
-        if (lp_top(now, T{}) > a.m || top_vec < 0) {
+        const float round_top = lp_top(now, T{});
+        if (PARTS > 1 && p.k > 0) {
+          uint32_t most;  // (in its upper half)
+          asm("max.bf16x2 %0, %1, %2;" : "=r"(most) : "r"(part_hi), "r"(__float_as_uint(round_top)));
+          part_hi = __funnelshift_l(part_lo, part_hi, 16);
+          part_lo = (part_lo << 16) | (most >> 16);
+        }
+        if (round_top > a.m || top_vec < 0) {
 #pragma unroll
           for (int u = 0; u < UNROLL; ++u)
             if (u == 0 || base + u * STREAM < v1) meet(lp_top<1>({now[u]}, T{}), base + u * STREAM);
@@ -360,8 +369,6 @@ __global__ void __launch_bounds__(kLpStream + 32, kLpCtas) token_logprobs_kernel
       const int b = n & 1;
       if (n >= 2) lp_bar_sync<kFree>(b);  // the row before last has been read
       if (p.k > 0) {
-        // The key of this thread's largest logit lies between that of its vector's last element and that of its first.
-        const unsigned long long high = top_vec < 0 ? 0ull : lp_key(a.m, max(row.first(top_vec), 0));
         lows[b][tid] = top_vec < 0 ? 0ull : lp_key(a.m, min(row.first(top_vec) + VEC - 1, p.V - 1));
         asm volatile("bar.sync %0, %1;" ::"n"(kStream), "n"(STREAM) : "memory");
         if (warp == 0) {
@@ -382,14 +389,29 @@ __global__ void __launch_bounds__(kLpStream + 32, kLpCtas) token_logprobs_kernel
         const unsigned long long lim = limits[b];
         const float least = lp_value((uint32_t)(lim >> 32));
         if (edge) look(row, edge_vec, row.raw(edge_vec), lim, least, b);
-        const unsigned who = __ballot_sync(0xffffffffu, high >= lim), per = (unsigned)(v1 - v0 + STREAM - 1) / STREAM;
-        if (high >= lim) owners[warp][__popc(who & ((1u << lane) - 1u))] = (unsigned char)lane;
+        const uint32_t lim_half = (uint32_t)(lim >> 48);
+        const int rounds = (max(v1 - v0 - tid, 0) + STREAM * UNROLL - 1) / (STREAM * UNROLL);  // of this thread
+        unsigned some = 0u;
+        if constexpr (PARTS == 1) {
+          part_lo = __float_as_uint(a.m) >> 16;
+        }
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          const uint32_t half = ((i & 2 ? part_hi : part_lo) >> (16 * (i & 1))) & 0xffffu;
+          const bool reaches = lp_order(__uint_as_float(half << 16)) >> 16 >= lim_half;
+          const unsigned who = __ballot_sync(0xffffffffu, reaches);
+          if (reaches) owners[warp][some + __popc(who & ((1u << lane) - 1u))] = (unsigned char)(lane | ((rounds - 1 - i) & (PARTS - 1)) << 5);
+          some += __popc(who);
+        }
         __syncwarp();
-        const unsigned todo = __popc(who) * per;  // vectors of the warp's threads whose largest logit may reach it
+        const unsigned per = (unsigned)((v1 - v0 + PARTS * STREAM * UNROLL - 1) / (PARTS * STREAM * UNROLL)) * UNROLL;  // vectors of a part
+        const unsigned todo = some * per;
+        auto vector_of = [&](unsigned i) -> int {
+          const unsigned o = i / per, j = i - o * per, owner = owners[warp][o];
+          return v0 + warp * 32 + (int)(owner & 31u) + (int)((owner >> 5) * UNROLL + j / UNROLL * (PARTS * UNROLL) + j % UNROLL) * STREAM;
+        };
         for (unsigned i = lane; i < todo; i += 64u) {
-          const unsigned o0 = i / per, i1 = i + 32u, o1 = i1 / per;
-          const int vec0 = v0 + warp * 32 + owners[warp][o0] + (int)((i - o0 * per) * STREAM);
-          const int vec1 = i1 < todo ? v0 + warp * 32 + owners[warp][o1] + (int)((i1 - o1 * per) * STREAM) : v1;
+          const int vec0 = vector_of(i), vec1 = i + 32u < todo ? vector_of(i + 32u) : v1;
           const uint4 x0 = row.inner(min(vec0, v1 - 1)), x1 = row.inner(min(vec1, v1 - 1));
           if (vec0 < v1) look(row, vec0, x0, lim, least, b);
           if (vec1 < v1) look(row, vec1, x1, lim, least, b);
