@@ -16,7 +16,7 @@
 //                    redone.  (Two threads per row in different warps, each with half of a tile's columns and its maximum handed over through
 //                    shared memory: 8 x 16 heads of 128 x 4096 631 us, so 588; of 64 614 and 520; 40 mixed prompts 102 and 95.)
 //   warps 8-11       output: row sums from shared memory, O from TMEM (a row per thread), rows through shared memory so that a row's bytes leave together
-// What bounds it is the softmax: 8 x 16 heads of 128 x 4096 causal 583 to 595 us = 930 TFLOP/s, 0.56 of the measured product rate, with the tensor pipe and the
+// What bounds it is the softmax: 8 x 16 heads of 128 x 4096 causal 575 us = 956 TFLOP/s, 0.57 of the measured product rate, with the tensor pipe and the
 // exponentials each busy 41 to 45 % of the time; long caches 1.03 us a tile of 128 x 128, prompts of 17 to 1000 tokens 1.7 (starts and masked ends).
 // (Two CTAs an SM for heads of 64, each with one score buffer, its softmax threads storing the output: 512 prompts of 128 143 us instead of 161, 40 mixed
 // ones 106 instead of 102, 8 of 4096 597 instead of 615; not kept.)
@@ -626,7 +626,9 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         const bool masked = t0 + kBN > clear || in_gap;
         int last[2];
         unsigned long long seen[2][2];
+        int halves = 2;  // of the tile that one of this warp's rows sees something of (8 x 16 heads of 128 x 4096 590 us with all of it, 575 so)
         if (__builtin_expect(masked, 0)) {
+          if ((TREE ? x.it.key1 - 1 : min(x.it.last0 + row0 + 15, x.it.key1 - 1)) - t0 < 64) halves = 1;
           if constexpr (!TREE) {
             // (what Q holds behind the last row is anything; its scores stay as they are)
 #pragma unroll
@@ -691,9 +693,15 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
           float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
           for (int c = 0; c < 2; ++c) {
+            uint32_t packed[16];
+            if (__builtin_expect(c >= halves, 0)) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) packed[i] = 0u;
+              rows16_st_pairs(lane_addr + kPCol + buf * 64 + c * 32, packed);
+              break;
+            }
             float sv[32];
             scores(c, sv);
-            uint32_t packed[16];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
 #pragma unroll
