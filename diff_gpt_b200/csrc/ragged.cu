@@ -50,24 +50,28 @@ extern "C" int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_h
   return packed_simt(p, D, dtype, static_cast<cudaStream_t>(stream));
 }
 
-// One round of CTAs: a share is as long as its sequences allow.  The tensor-core kernel takes 128 rows an item and one CTA an SM, the other
-// 16 or 64 rows and two CTAs or more; a share below two tiles would wait for the second pass longer than it saves, and so do shares beyond one
-// round, which write and read partial rows for nothing.  (bf16, us: 3 sequences of 40000 to 65000 keys, 64 drafts, 1 share 503, 6 as chosen 99, 8 134; 48 of 300 to
-// 4000, 1 as chosen 54, 2 75; 8 of them 47, 4 as chosen 24, 8 28; one draft behind 2000 keys 26, 8 as chosen 13.6.)
+// One round of CTAs: a share is as long as its sequences allow.  The tensor-core kernel takes 128 rows an item and one CTA an SM; shares of its below two tiles
+// of 128 keys, or beyond one round, write, read and join partial rows for nothing.  On the CUDA cores a tile of 64 keys takes so long that tiles of 16 rows are worth
+// a share each (four CTAs an SM), and tiles of 64 rows two (two CTAs an SM); up to 128 keys the second pass costs what it saves.
+// (us, bf16: 3 sequences of 40000 to 65000 keys, 64 drafts, 1 share 495, 6 as chosen 99, 8 134; 48 of 300 to 4000, 1 as chosen 53, 2 75; 8 of them 46, 4 as chosen 24, 8
+// 28; one draft behind 2000 keys 26, 8 as chosen 13.4.  fp32, heads of 16: 24 sequences of 30 to 500 keys, 13 drafts, 1 share 14.5, 2 12.6, 6 as chosen 9.7; 2000 keys, 150
+// drafts, 1 101, 17 as chosen 16, 32 21; heads of 64: 1500 keys, one draft, 1 94, 6 20, 24 as chosen 9.3.)
 extern "C" int32_t dgpt_tree_attn_splits(int32_t B, int32_t T, int32_t H, int32_t G, int32_t D, int32_t max_keys, int32_t dtype) {
   if (B <= 0 || T <= 0 || H <= 0 || G <= 0 || H % G != 0 || max_keys <= 0) return 1;
   const bool tensor = dtype == DGPT_BF16 && D >= 32;
   const long long group = H / G, rows = T * group;
-  long long tiles, ctas;
+  long long tiles, ctas, least;
   if (tensor) {
     const long long nodes = group < 128 ? 128 / group : 1;
     tiles = (T + nodes - 1) / nodes;
     ctas = 148;
+    least = 256;
   } else {
     tiles = rows <= 16 ? 1 : (rows + 63) / 64;
-    ctas = 2 * 148;
+    ctas = (rows <= 16 ? 4 : 2) * 148;
+    least = rows <= 16 ? 64 : 128;
   }
-  const long long items = (long long)B * G * tiles, fit = ctas / items, most = ((long long)max_keys + 255) / 256;
+  const long long items = (long long)B * G * tiles, fit = ctas / items, most = max_keys <= 128 ? 1 : ((long long)max_keys + least - 1) / least;
   const long long n = fit < most ? fit : most;
   return (int32_t)(n < 1 ? 1 : n > 256 ? 256 : n);
 }

@@ -6,7 +6,7 @@
 // and over (rows, columns) of the output, each with BM / 16 rows, so that a number fetched from shared memory feeds several products.
 // fp32 products have no tensor-core form that keeps 24 bits; the floor is the FMA rate.  What bounds it: reads of shared memory and the softmax's shuffles
 // between the products (8 prompts of 700, 8 heads of 64, 183 us, 54 at the FMA rate), and for small ones the chain of a CTA's few steps (32 of 20 to 140, 4
-// heads of 16, 15 us, with tiles of 16 rows no less).  Trees of up to 16 rows take tiles of 16: 24 trees of 13 drafts behind 30 to 500 keys 12.2 us, with 64 rows 20.4.
+// heads of 16, 15 us, with tiles of 16 rows no less).  Trees of up to 16 rows take tiles of 16: 24 trees of 13 drafts behind 30 to 500 keys in two shares 12.2 us, with 64 rows 20.4.
 #include "ragged.cuh"
 
 namespace dgpt {
@@ -274,9 +274,9 @@ int tree_simt(const TreeProblem& full, int dtype, cudaStream_t st) {
 }
 
 // ---- partials of a tree's rows into one -------------------------------------------------------------------------
-// One warp per (row, head): y = sum_s 2^(lse_s - m) o_s / sum_s 2^(lse_s - m), with the running maximum m, four shares at a time.  Their loads, and
+// One warp per (row, head): y = sum_s 2^(lse_s - m) o_s / sum_s 2^(lse_s - m), with the running maximum m, STEP shares at a time.  Their loads, and
 // those of the lengths that say how many shares there are, do not wait for one another (what is read of shares that were not written counts for nothing).
-template <typename T>
+template <typename T, int STEP>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeProblem p) {
   dep_wait();
   const long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), n = (long long)p.B * p.T * p.H;
@@ -287,11 +287,11 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeProblem p) {
   const bool mine = lane * 4 < p.D;  // columns lane * 4 .. (D <= 128)
   int splits = p.n_splits;
   float acc[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f, m = -INFINITY;
-  for (int i0 = 0; i0 < splits; i0 += 4) {
-    float lse[4];
-    float4 v[4];
+  for (int i0 = 0; i0 < splits; i0 += STEP) {
+    float lse[STEP];
+    float4 v[STEP];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < STEP; ++u) {
       const long long slot = min(i0 + u, p.n_splits - 1) * n + at;
       lse[u] = p.part_lse[slot];
       v[u] = mine ? *reinterpret_cast<const float4*>(p.part_o + slot * p.D + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeProblem p) {
     }
     float top = m;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < STEP; ++u) {
       if (i0 + u >= splits) lse[u] = -INFINITY;
       top = fmaxf(top, lse[u]);
     }
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeProblem p) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) acc[c] *= f;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < STEP; ++u) {
       if (lse[u] == -INFINITY) continue;  // no key of this share is seen
       const float w = ex2(lse[u] - ref);
       total += w;
@@ -337,8 +337,10 @@ int tree_merge(const TreeProblem& full, int tile_keys, int dtype, cudaStream_t s
   p.tile_keys = tile_keys;
   const long long rows = (long long)p.B * p.T * p.H;
   const dim3 grid((unsigned)((rows + 7) / 8));
-  if (dtype == DGPT_F32) launch_few(true, tree_merge_kernel<float>, grid, dim3(256), 0, st, p);
-  else launch_few(true, tree_merge_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p);
+  // Eight shares at a time where there are more than four (one sequence of 30000 keys in 37: 25.9 us in fours, 24.5 so; 16 sequences in two: 31.2 and 33.0).
+  const bool many = p.n_splits > 4;
+  if (dtype == DGPT_F32) launch_few(true, many ? tree_merge_kernel<float, 8> : tree_merge_kernel<float, 4>, grid, dim3(256), 0, st, p);
+  else launch_few(true, many ? tree_merge_kernel<__nv_bfloat16, 8> : tree_merge_kernel<__nv_bfloat16, 4>, grid, dim3(256), 0, st, p);
   return launch_status("tree_attn");
 }
 

@@ -17,7 +17,7 @@
 //                    shared memory: 8 x 16 heads of 128 x 4096 631 us, so 588; of 64 614 and 520; 40 mixed prompts 102 and 95.)
 //   warps 8-11       output: row sums from shared memory, O from TMEM (a row per thread), rows through shared memory so that a row's bytes leave together
 // What bounds it is the softmax: 8 x 16 heads of 128 x 4096 causal 575 us = 956 TFLOP/s, 0.57 of the measured product rate, with the tensor pipe and the
-// exponentials each busy 41 to 45 % of the time; long caches 1.03 us a tile of 128 x 128, prompts of 17 to 1000 tokens 1.7 (starts and masked ends).
+// exponentials each busy 41 to 45 % of the time; long caches 1.35 us a tile of 128 x 128, prompts of 17 to 1000 tokens 1.7 (starts and masked ends).
 // (Two CTAs an SM for heads of 64, each with one score buffer, its softmax threads storing the output: 512 prompts of 128 143 us instead of 161, 40 mixed
 // ones 106 instead of 102, 8 of 4096 597 instead of 615; not kept.)
 // TMEM columns: S0 [0,128)  S1 [128,256)  P0 [256,320)  P1 [320,384)  O [384, 384 + D).
