@@ -26,6 +26,9 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
   constexpr int RM = BM / 16;                  // rows per thread
   constexpr int KC = kRgBN / 16;               // score columns per thread
   constexpr int CO = D >= 16 ? D / 16 : 1;     // output columns per thread
+  // Of which these lie side by side, so that 16 threads read 16 neighbouring pieces of a value's row (heads of 128, 8 drafts behind 500 keys: 78 us with all of a
+  // thread's columns side by side, 61 so).
+  constexpr int CV = CO < 4 ? CO : 4;
   constexpr int VEC = Io<T>::kVec16, VPR = D / VEC;
   constexpr int PITCH = D + 4, PPITCH = kRgBN + 4;
   extern __shared__ __align__(16) float sm[];
@@ -35,6 +38,7 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
   float* Ps = Vs + kRgBN * PITCH;      // [BM][PPITCH]
 
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  auto column = [&](int c) { return c / CV * 16 * CV + tx * CV + c % CV; };
   p.check((int)blockIdx.x, tid, kRgThreads);
   RaggedItem it;
   if constexpr (TREE) {
@@ -158,7 +162,7 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
       for (int c = 0; c < CO; ++c) acc[i][c] *= f;
     }
     __syncthreads();
-    // output: rows ty * RM + i, columns tx * CO + c
+    // output: rows ty * RM + i, columns column(c)
     if (D >= 16 || tx * CO < D) {
 #pragma unroll 4
       for (int j = 0; j < kRgBN; j += 4) {
@@ -167,9 +171,14 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
         for (int i = 0; i < RM; ++i) a[i] = *reinterpret_cast<const float4*>(&Ps[(ty * RM + i) * PPITCH + j]);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          float b[CO];
+          alignas(16) float b[CO];
 #pragma unroll
-          for (int c = 0; c < CO; ++c) b[c] = Vs[(j + x) * PITCH + tx * CO + c];
+          for (int c = 0; c < CO; c += CV) {
+            const float* from = &Vs[(j + x) * PITCH + column(c)];
+            if constexpr (CV == 4) *reinterpret_cast<float4*>(&b[c]) = *reinterpret_cast<const float4*>(from);
+            else if constexpr (CV == 2) *reinterpret_cast<float2*>(&b[c]) = *reinterpret_cast<const float2*>(from);
+            else b[c] = *from;
+          }
 #pragma unroll
           for (int i = 0; i < RM; ++i) {
             const float w = x == 0 ? a[i].x : x == 1 ? a[i].y : x == 2 ? a[i].z : a[i].w;
@@ -194,21 +203,21 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
         const long long at = ((long long)it.split * p.B * p.T + row) * p.H + h;
         if (D >= 16 || tx * CO < D) {
 #pragma unroll
-          for (int c = 0; c < CO; ++c) p.part_o[at * D + tx * CO + c] = any ? acc[i][c] * inv : 0.f;
+          for (int c = 0; c < CO; ++c) p.part_o[at * D + column(c)] = any ? acc[i][c] * inv : 0.f;
         }
         if (tx == 0) p.part_lse[at] = any ? m[i] + log2f(l[i]) : -INFINITY;
         continue;
       }
       if (D >= 16 || tx * CO < D) {
-        T* o = static_cast<T*>(p.o) + row * p.o_rs + (long long)h * D + tx * CO;
+        T* o = static_cast<T*>(p.o) + row * p.o_rs + (long long)h * D;
 #pragma unroll
-        for (int c = 0; c < CO; ++c) Io<T>::st(o + c, any ? acc[i][c] * inv : 0.f);
+        for (int c = 0; c < CO; ++c) Io<T>::st(o + column(c), any ? acc[i][c] * inv : 0.f);
       }
     } else {
       if (D >= 16 || tx * CO < D) {
-        T* o = static_cast<T*>(p.o) + (long long)(it.row0 + r) * p.o_rs + (long long)it.h * p.o_hs + tx * CO;
+        T* o = static_cast<T*>(p.o) + (long long)(it.row0 + r) * p.o_rs + (long long)it.h * p.o_hs;
 #pragma unroll
-        for (int c = 0; c < CO; ++c) Io<T>::st(o + c, any ? acc[i][c] * inv : 0.f);
+        for (int c = 0; c < CO; ++c) Io<T>::st(o + column(c), any ? acc[i][c] * inv : 0.f);
       }
       if (tx == 0 && p.lse) p.lse[(long long)(it.row0 + r) * p.H + it.h] = any ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
     }
