@@ -36,6 +36,8 @@ constexpr int kRtThreads = 512;
 constexpr int kRtRegs = 128, kRtSoftmaxRegs = 152, kRtHelperRegs = 80;
 static_assert(2 * kRtSoftmaxRegs + kRtRegs + kRtHelperRegs == 4 * kRtRegs, "the warpgroups share what the launch has");
 constexpr int kRtLead = 3;                                                    // key tiles still to be loaded when the next item is asked for
+// Limit of the waits that may last a whole item, 3 x 10^9 keys here; the others, of a tile or two, run out first and raise the abort flag.
+constexpr long long kRtItemCycles = 16 * kWaitLimitCycles;
 constexpr int kRtRing = 8;                                                    // items between the warp that finds them and the last role that reads them
 
 struct RtItem {
@@ -211,7 +213,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
     const long long t0 = clock64();
     while (!mbar_try_wait(bar(b), parity)) {
       if (*abort_flag) return false;
-      if (clock64() - t0 > kWaitLimitCycles) {
+      if (clock64() - t0 > kRtItemCycles) {
         *abort_flag = 2;
         return false;
       }
@@ -434,7 +436,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         const long long t0 = clock64();
         while (handed - *loaded > (unsigned)kRtLead) {
           if (*abort_flag) return false;
-          if (clock64() - t0 > kWaitLimitCycles) {
+          if (clock64() - t0 > kRtItemCycles) {
             *abort_flag = 2;
             return false;
           }
