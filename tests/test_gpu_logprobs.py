@@ -66,6 +66,16 @@ def test_sizes(R, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("R,V,kind", [(200, 70001, "normal"), (200, 70001, "ties"), (160, 70001, "rising"), (160, 70001, "falling"), (160, 70001, "masked"), (700, 40003, "normal")])
+def test_rows_of_many_rounds(R, V, kind, dtype):
+    """Rows too many for clusters and too long for four rounds of loads, and several of them to a CTA."""
+    from diff_gpt_b200 import ops
+
+    logits, targets = make(R, V, dtype, 6, kind)
+    check(logits, targets, 1.0, 20, ops.token_logprobs(logits, targets, top_k=20))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("kind", ["ties", "level", "rising", "falling", "peaked", "masked", "three", "comb", "zeros", "lowest"])
 @pytest.mark.parametrize("R,V", [(2, 40), (3, 20000), (320, 6001), (1, 100000)])
 def test_distributions(R, V, kind, dtype):
