@@ -54,8 +54,8 @@ extern "C" int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_h
 // of 128 keys, or beyond one round, write, read and join partial rows for nothing.  On the CUDA cores a tile of 64 keys takes so long that tiles of 16 rows are worth
 // a share each (four CTAs an SM), and tiles of 64 rows two (two CTAs an SM); up to 128 keys the second pass costs what it saves.
 // (us, bf16: 3 sequences of 40000 to 65000 keys, 64 drafts, 1 share 495, 6 as chosen 99, 8 134; 48 of 300 to 4000, 1 as chosen 53, 2 75; 8 of them 46, 4 as chosen 24, 8
-// 28; one draft behind 2000 keys 26, 8 as chosen 13.4.  fp32, heads of 16: 24 sequences of 30 to 500 keys, 13 drafts, 1 share 14.5, 2 12.6, 6 as chosen 9.7; 2000 keys, 150
-// drafts, 1 101, 17 as chosen 16, 32 21; heads of 64: 1500 keys, one draft, 1 94, 6 20, 24 as chosen 9.3.)
+// 28; one draft behind 2000 keys 26, 8 as chosen 13.4.  fp32, heads of 16: 24 sequences of 30 to 500 keys, 13 drafts, 1 share 12.2, 2 11.0, 6 as chosen 9.5; 2000 keys, 150
+// drafts, 1 83, 17 as chosen 19, 24 15, 32 20; heads of 64: 1500 keys, one draft, 1 64, 6 15, 24 as chosen 8.5.)
 extern "C" int32_t dgpt_tree_attn_splits(int32_t B, int32_t T, int32_t H, int32_t G, int32_t D, int32_t max_keys, int32_t dtype) {
   if (B <= 0 || T <= 0 || H <= 0 || G <= 0 || H % G != 0 || max_keys <= 0) return 1;
   const bool tensor = dtype == DGPT_BF16 && D >= 32;

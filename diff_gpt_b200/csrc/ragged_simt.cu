@@ -2,11 +2,11 @@
 // tensor-core kernel cannot tile.
 //
 // A CTA of 256 threads owns a tile of BM rows and walks through its keys 64 at a time with the running maximum and sum of a softmax.
-// Q, K, V and the probabilities of a step lie in shared memory as fp32; the threads form a 16 x 16 grid over (rows, keys) of the scores
-// and over (rows, columns) of the output, each with BM / 16 rows, so that a number fetched from shared memory feeds several products.
+// Q, K, V and the probabilities of a step lie in shared memory as fp32; a row belongs to 16 or 32 threads of one warp, each with 4 or 2 rows, its share of
+// a step's scores and of the output's columns, so that a number fetched from shared memory feeds several products and no barrier stands between the two products.
 // fp32 products have no tensor-core form that keeps 24 bits; the floor is the FMA rate.  What bounds it: reads of shared memory and the softmax's shuffles
-// between the products (8 prompts of 700, 8 heads of 64, 183 us, 54 at the FMA rate), and for small ones the chain of a CTA's few steps (32 of 20 to 140, 4
-// heads of 16, 15 us, with tiles of 16 rows no less).  Trees of up to 16 rows take tiles of 16: 24 trees of 13 drafts behind 30 to 500 keys in two shares 12.2 us, with 64 rows 20.4.
+// between the products (8 prompts of 700, 8 heads of 64, 171 us, 54 at the FMA rate), and for small ones the chain of a CTA's few steps (32 of 20 to 140, 4
+// heads of 16, 14 us).  Trees of up to 16 rows take tiles of 16 (24 trees of 13 drafts behind 30 to 500 keys in two shares 12.2 us, with 64 rows 20.4).
 #include "ragged.cuh"
 
 namespace dgpt {
@@ -23,12 +23,14 @@ constexpr int kRgBN = 64;
 
 template <typename T, int D, int BM, class P, bool TREE>
 __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
-  constexpr int RM = BM / 16;                  // rows per thread
-  constexpr int KC = kRgBN / 16;               // score columns per thread
-  constexpr int CO = D >= 16 ? D / 16 : 1;     // output columns per thread
-  // Of which these lie side by side, so that 16 threads read 16 neighbouring pieces of a value's row (heads of 128, 8 drafts behind 500 keys: 78 us with all of a
-  // thread's columns side by side, 61 so).
-  constexpr int CV = CO < 4 ? CO : 4;
+  // Threads that share a row.  (16 and 32, us: tiles of 16 rows, heads of 64, 8 drafts behind 2000 keys 97 and 81, one behind 1500 75 and 64; tiles of 64, 8 prompts
+  // of 700 171 and 199, 32 of 80 with heads of 16 7.1 and 8.3.)
+  constexpr int LX = BM == 16 ? 32 : 16;
+  constexpr int RM = BM * LX / kRgThreads;     // rows per thread
+  constexpr int KC = kRgBN / LX;               // score columns per thread
+  constexpr int CO = D >= LX ? D / LX : 1;     // output columns per thread
+  constexpr int CV = CO < 4 ? CO : 4;          // of which lie side by side, so that a row's threads read neighbouring pieces of a value's row
+  constexpr int KG = D >= LX ? 1 : LX / D;     // threads that share a step's keys of an output column
   constexpr int VEC = Io<T>::kVec16, VPR = D / VEC;
   constexpr int PITCH = D + 4, PPITCH = kRgBN + 4;
   extern __shared__ __align__(16) float sm[];
@@ -37,8 +39,8 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
   float* Vs = Ks + kRgBN * PITCH;      // [64][PITCH]
   float* Ps = Vs + kRgBN * PITCH;      // [BM][PPITCH]
 
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  auto column = [&](int c) { return c / CV * 16 * CV + tx * CV + c % CV; };
+  const int tid = threadIdx.x, tx = tid % LX, row0 = tid / LX * RM, group = tx / (LX / KG);
+  auto column = [&](int c) { return c / CV * LX * CV + tx % (LX / KG) * CV + c % CV; };
   p.check((int)blockIdx.x, tid, kRgThreads);
   RaggedItem it;
   if constexpr (TREE) {
@@ -63,7 +65,7 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
 #pragma unroll
     for (int x = 0; x < VEC; x += 4) *reinterpret_cast<float4*>(&Qs[r * PITCH + c * VEC + x]) = make_float4(t[x], t[x + 1], t[x + 2], t[x + 3]);
   }
-  float m[RM], l[RM], acc[RM][CO];
+  float m[RM], l[RM], acc[RM][CO];  // l: of this thread's keys
 #pragma unroll
   for (int i = 0; i < RM; ++i) {
     m[i] = -INFINITY;
@@ -111,7 +113,8 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
     }
     __syncthreads();
     if (j0 + kRgBN < it.key1) fetch(j0 + kRgBN);
-    // scores: rows ty * RM + i, keys tx + 16 j
+    if (tid / 32 * 32 / LX * RM >= it.rows) continue;  // none of this warp's rows exists
+    // scores: rows row0 + i, keys tx + LX j
     float s[RM][KC];
 #pragma unroll
     for (int i = 0; i < RM; ++i)
@@ -121,77 +124,86 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
     for (int d = 0; d < D; d += 4) {
       float4 a[RM], b[KC];
 #pragma unroll
-      for (int i = 0; i < RM; ++i) a[i] = *reinterpret_cast<const float4*>(&Qs[(ty * RM + i) * PITCH + d]);
+      for (int i = 0; i < RM; ++i) a[i] = *reinterpret_cast<const float4*>(&Qs[(row0 + i) * PITCH + d]);
 #pragma unroll
-      for (int j = 0; j < KC; ++j) b[j] = *reinterpret_cast<const float4*>(&Ks[(tx + 16 * j) * PITCH + d]);
+      for (int j = 0; j < KC; ++j) b[j] = *reinterpret_cast<const float4*>(&Ks[(tx + LX * j) * PITCH + d]);
 #pragma unroll
       for (int i = 0; i < RM; ++i)
 #pragma unroll
         for (int j = 0; j < KC; ++j) s[i][j] = fmaf(a[i].w, b[j].w, fmaf(a[i].z, b[j].z, fmaf(a[i].y, b[j].y, fmaf(a[i].x, b[j].x, s[i][j]))));
     }
     const bool masked = j0 + kRgBN > it.clear || j0 + kRgBN > it.key1 || (j0 < it.gap1 && j0 + kRgBN > it.gap0);
+    if (masked) {
 #pragma unroll
-    for (int i = 0; i < RM; ++i) {
-      const int r = ty * RM + i;
-      if (masked) {
+      for (int i = 0; i < RM; ++i)
 #pragma unroll
         for (int j = 0; j < KC; ++j) {
-          const int key = j0 + tx + 16 * j;
-          if (r >= it.rows || key >= it.key1 || !p.sees(it, r, key)) s[i][j] = -INFINITY;
+          const int key = j0 + tx + LX * j;
+          if (row0 + i >= it.rows || key >= it.key1 || !p.sees(it, row0 + i, key)) s[i][j] = -INFINITY;
         }
-      }
-      float top = s[i][0];
+    }
+    float top[RM];
 #pragma unroll
-      for (int j = 1; j < KC; ++j) top = fmaxf(top, s[i][j]);
+    for (int i = 0; i < RM; ++i) {
+      top[i] = s[i][0];
 #pragma unroll
-      for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const float mn = fmaxf(m[i], top), ref = mn == -INFINITY ? 0.f : mn;
+      for (int j = 1; j < KC; ++j) top[i] = fmaxf(top[i], s[i][j]);
+    }
+#pragma unroll
+    for (int x = LX / 2; x > 0; x >>= 1)
+#pragma unroll
+      for (int i = 0; i < RM; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], x));
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      const float mn = fmaxf(m[i], top[i]), ref = mn == -INFINITY ? 0.f : mn;
       const float f = ex2(m[i] - ref);  // m = -inf: 0
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
         const float e = ex2(s[i][j] - ref);
         sum += e;
-        Ps[r * PPITCH + tx + 16 * j] = e;
+        Ps[(row0 + i) * PPITCH + tx + LX * j] = e;
       }
-#pragma unroll
-      for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
       m[i] = mn;
-      l[i] = l[i] * f + sum;
+      l[i] = fmaf(l[i], f, sum);
 #pragma unroll
       for (int c = 0; c < CO; ++c) acc[i][c] *= f;
     }
-    __syncthreads();
-    // output: rows ty * RM + i, columns column(c)
-    if (D >= 16 || tx * CO < D) {
-#pragma unroll 4
-      for (int j = 0; j < kRgBN; j += 4) {
-        float4 a[RM];
+    __syncwarp();
+    // output: the same rows (a row's threads are of one warp), columns column(c), every KG-th four keys
+#pragma unroll 2
+    for (int j = group * 4; j < kRgBN; j += 4 * KG) {
+      float4 w[RM];
 #pragma unroll
-        for (int i = 0; i < RM; ++i) a[i] = *reinterpret_cast<const float4*>(&Ps[(ty * RM + i) * PPITCH + j]);
+      for (int i = 0; i < RM; ++i) w[i] = *reinterpret_cast<const float4*>(&Ps[(row0 + i) * PPITCH + j]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          alignas(16) float b[CO];
+      for (int x = 0; x < 4; ++x) {
+        alignas(16) float b[CO];
 #pragma unroll
-          for (int c = 0; c < CO; c += CV) {
-            const float* from = &Vs[(j + x) * PITCH + column(c)];
-            if constexpr (CV == 4) *reinterpret_cast<float4*>(&b[c]) = *reinterpret_cast<const float4*>(from);
-            else if constexpr (CV == 2) *reinterpret_cast<float2*>(&b[c]) = *reinterpret_cast<const float2*>(from);
-            else b[c] = *from;
-          }
+        for (int c = 0; c < CO; c += CV) {
+          const float* from = &Vs[(j + x) * PITCH + column(c)];
+          if constexpr (CV == 4) *reinterpret_cast<float4*>(&b[c]) = *reinterpret_cast<const float4*>(from);
+          else if constexpr (CV == 2) *reinterpret_cast<float2*>(&b[c]) = *reinterpret_cast<const float2*>(from);
+          else b[c] = *from;
+        }
 #pragma unroll
-          for (int i = 0; i < RM; ++i) {
-            const float w = x == 0 ? a[i].x : x == 1 ? a[i].y : x == 2 ? a[i].z : a[i].w;
+        for (int i = 0; i < RM; ++i) {
+          const float e = x == 0 ? w[i].x : x == 1 ? w[i].y : x == 2 ? w[i].z : w[i].w;
 #pragma unroll
-            for (int c = 0; c < CO; ++c) acc[i][c] = fmaf(w, b[c], acc[i][c]);
-          }
+          for (int c = 0; c < CO; ++c) acc[i][c] = fmaf(e, b[c], acc[i][c]);
         }
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < RM; ++i) {
-    const int r = ty * RM + i;
+    const int r = row0 + i;
+#pragma unroll
+    for (int x = LX / 2; x > 0; x >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+#pragma unroll
+    for (int x = LX / KG; x < LX; x <<= 1)
+#pragma unroll
+      for (int c = 0; c < CO; ++c) acc[i][c] += __shfl_xor_sync(0xffffffffu, acc[i][c], x);
     if (r >= it.rows) continue;
     // !(l <= 0): a row with a key that is not a number keeps saying so
     const bool any = !(l[i] <= 0.f);
@@ -201,20 +213,20 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
       const int h = p.head(it, r);
       if (p.n_splits > 1) {
         const long long at = ((long long)it.split * p.B * p.T + row) * p.H + h;
-        if (D >= 16 || tx * CO < D) {
+        if (group == 0) {
 #pragma unroll
           for (int c = 0; c < CO; ++c) p.part_o[at * D + column(c)] = any ? acc[i][c] * inv : 0.f;
         }
         if (tx == 0) p.part_lse[at] = any ? m[i] + log2f(l[i]) : -INFINITY;
         continue;
       }
-      if (D >= 16 || tx * CO < D) {
+      if (group == 0) {
         T* o = static_cast<T*>(p.o) + row * p.o_rs + (long long)h * D;
 #pragma unroll
         for (int c = 0; c < CO; ++c) Io<T>::st(o + column(c), any ? acc[i][c] * inv : 0.f);
       }
     } else {
-      if (D >= 16 || tx * CO < D) {
+      if (group == 0) {
         T* o = static_cast<T*>(p.o) + (long long)(it.row0 + r) * p.o_rs + (long long)it.h * p.o_hs;
 #pragma unroll
         for (int c = 0; c < CO; ++c) Io<T>::st(o + column(c), any ? acc[i][c] * inv : 0.f);
