@@ -111,6 +111,7 @@ extern "C" int dgpt_kv_keep(const dgpt_kv_layout* kv, int64_t kv_token_stride, c
   if (int e = validate_kv(kv, D)) return e;
   DGPT_REQUIRE(kv_token_stride >= D && kv_token_stride % 8 == 0 && layer_stride % 8 == 0, "kv_keep: strides must be multiples of 8 elements");
   DGPT_REQUIRE(kv->n_pages >= 0, "kv_keep: pages must not be negative");
+  DGPT_REQUIRE(kv->page_table || kv->n_pages == 0 || B <= kv->n_pages, "kv_keep: %d sequences in a cache of %lld", B, (long long)kv->n_pages);
   DGPT_REQUIRE((H == 1 || kv->head_stride >= D) && (n_layer == 1 || layer_stride != 0), "kv_keep: heads and layers must lie apart");
   KeepParams p;
   p.kv = make_view(kv);

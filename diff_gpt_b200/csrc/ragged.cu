@@ -103,6 +103,7 @@ extern "C" int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv
   DGPT_REQUIRE(q && ctx_len && ancestors && out, "tree_attn: NULL pointer");
   DGPT_REQUIRE((gap_start == nullptr) == (gap_end == nullptr), "tree_attn: a gap has a start and an end");
   if (int e = validate_kv(kv, D)) return e;
+  DGPT_REQUIRE(kv->page_table || kv->n_pages <= 0 || B <= kv->n_pages, "tree_attn: %d sequences in a cache of %lld", B, (long long)kv->n_pages);
   DGPT_REQUIRE(aligned16(q) && aligned16(out), "tree_attn: pointers must be 16-byte aligned");
   DGPT_REQUIRE(q_row_stride >= (int64_t)H * D && out_row_stride >= (int64_t)H * D && q_row_stride % 8 == 0 && out_row_stride % 8 == 0,
                "tree_attn: row strides must be multiples of 8 elements that hold a row");

@@ -94,9 +94,9 @@ class KVCache:
             self.kv_shape = self.kv_cache.shape
 
     def layer_layout(self, layer: int) -> ops.KvLayout:
-        _, _, _, H, T, D = self.kv_cache.shape
+        _, _, B, H, T, D = self.kv_cache.shape
         c = self.kv_cache
-        return ops.kv_layout(c[layer, 0], c[layer, 1], page_stride=H * T * D, head_stride=T * D, page_tokens=T)
+        return ops.kv_layout(c[layer, 0], c[layer, 1], page_stride=H * T * D, head_stride=T * D, page_tokens=T, n_pages=B)
 
 
 class PagedKVCache:

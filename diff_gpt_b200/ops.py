@@ -1141,6 +1141,31 @@ def _stored(name: str, kv: KvLayout, dtype: torch.dtype) -> None:
             raise TypeError(f"{name}: a cache of {t.dtype} where {dtype} is expected")
 
 
+def _covers(name: str, kv: KvLayout, B: int, heads: int, D: int, token_stride: int, n_layer: int = 1, layer_stride: int = 0) -> None:
+    """What a cache does not hold would be read, or written, in another sequence's place or outside its storage: as many sequences as the
+    call has, and of each all heads, tokens and layers.  (A layout made by hand, without its tensors, is taken at its word.)"""
+    held = getattr(kv, "_keep", None)
+    if held is None:
+        return
+    k, v, table = held
+    if table is None:
+        if 0 < kv.n_pages < B:
+            raise ValueError(f"{name}: {B} sequences in a cache of {kv.n_pages}")
+        pages = B
+    else:
+        if table.dtype is not torch.int32 or not table.is_contiguous() or table.numel() < B * kv.max_pages:
+            raise ValueError(f"{name}: the page table must be contiguous int32 with a row for each of {B} sequences, got {table.dtype} {tuple(table.shape)}")
+        pages = kv.n_pages or 1  # (0: the caller answers for the table's numbers)
+    if B < 1:
+        return
+    layers = (n_layer - 1) * layer_stride
+    last = (pages - 1) * kv.page_stride + (heads - 1) * kv.head_stride + (kv.page_tokens - 1) * (token_stride or D) + D + max(layers, 0)
+    for t in (k, v):
+        at = t.storage_offset()
+        if (at + last) * t.element_size() > t.untyped_storage().nbytes() or at + layers < 0:
+            raise ValueError(f"{name}: the layout reaches outside its tensors' storage ({B} sequences, {pages} pages, {heads} heads of {D}, {n_layer} layers)")
+
+
 def _i32(name: str, t: torch.Tensor | None, shape: tuple[int, ...]) -> None:
     if t is not None and (t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
@@ -1268,6 +1293,7 @@ def tree_attn(
     _i32("gap_start", gap_start, (B,))
     _i32("gap_end", gap_end, (B,))
     _i32("status", status, (1,))
+    _covers("tree_attn", kv, B, G, D, token_stride)
     code = dtype_code(q)
     if n_splits == 0:
         held = (kv.max_pages if kv.page_table else 1) * kv.page_tokens
@@ -1361,6 +1387,7 @@ def kv_keep(
     _i32("status", status, (1,))
     if dtype not in _DT:
         raise TypeError(f"unsupported dtype {dtype}: float32 and bfloat16 are built")
+    _covers("kv_keep", kv, B, H, D, token_stride, n_layer, layer_stride)
     check(
         lib.dgpt_kv_keep(
             C.byref(kv), token_stride or D, src_start.data_ptr(), dst_start.data_ptr(), path.data_ptr(), count.data_ptr(), n_layer,

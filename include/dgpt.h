@@ -53,7 +53,7 @@ typedef struct dgpt_kv_layout {
   const int32_t* page_table; /* device, [n_seq][max_pages], or NULL */
   int32_t page_tokens;
   int32_t max_pages;
-  int64_t n_pages;           /* pages addressable from the bases when a page table is used (0 = not stated) */
+  int64_t n_pages;           /* pages addressable from the bases when a page table is used, else sequences (0 = not stated) */
 } dgpt_kv_layout;
 
 /* Text of the last error raised on this host thread; returns its length. */
@@ -616,7 +616,7 @@ int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_head_stride,
  * for nothing.  A draft that sees nothing gets zeros; rows from n_nodes[s] on are left as they are.
  * q, out: device [B * T, H * D], row s * T + t, with row strides that are multiples of 8; kv: keys and values of G heads, query head h
  * reads h / (H / G), consecutive tokens of a head kv_token_stride elements apart; slots behind a sequence's last draft and in the gap may
- * hold anything, the others finite numbers; a page number outside the pool (0 .. n_pages - 1, where the layout states n_pages) stands for zeros.
+ * hold anything, the others finite numbers; a page table has a row for each of the B sequences, a dense layout at least B sequences; a page number outside the pool (0 .. n_pages - 1, where the layout states n_pages) stands for zeros.
  * ancestors: device [B][T][words] with 64 * words >= T; T <= 256.  ctx_len, gap_start, gap_end, n_nodes: device int32 [B]; status bit 0 is
  * set where they do not fit T, the layout or one another (what does not fit is left out).
  * n_splits (1 to 256) splits each sequence's keys; workspace from the _bytes call (not needed for 1), 16-byte aligned, one call's at a time.  _splits chooses a
@@ -644,7 +644,8 @@ int dgpt_token_logprobs(const void* logits, int64_t logits_row_stride, const int
  *   slot dst_start[s] + i  <-  slot src_start[s] + path[s][i],   i < count[s]
  * All rows of a sequence are read before the first is written, so source and target may overlap; sequences must not write
  * slots that others read or write.  kv: layer 0's storage (layer l's lies l * layer_stride elements behind it, through the same page
- * table); consecutive tokens of a head kv_token_stride elements apart; k_base == v_base: one storage, moved once.
+ * table, which has a row for each of the B sequences; a dense layout has at least B); consecutive tokens of a head kv_token_stride elements
+ * apart; k_base == v_base: one storage, moved once.
  * path: device int32 [B, T], T <= 256; src_start, dst_start, count: device int32 [B].  A head's row is a multiple of 16 bytes.  A row whose
  * slots do not exist, or lie in a page outside the pool (where the layout states n_pages), is not moved and sets bit 0 of *status, as does a count outside 0 .. T. */
 int dgpt_kv_keep(const dgpt_kv_layout* kv, int64_t kv_token_stride, const int32_t* src_start, const int32_t* dst_start,
