@@ -4,7 +4,8 @@
 // carries s = sum 2^x and w = sum x 2^x; then lse = (M + log2 s) ln 2 and entropy = (log2 s - w / s) ln 2, and when M moves by d = old - new,
 // s <- s 2^d and w <- (w + d s) 2^d.  How M was rounded cancels out, unless it is so large that the rounding itself outgrows an exponent (logits of
 // the type's lowest value throughout, temperatures next to 0): M is kept within 2^30, and a row whose maximum lies beyond is summed once more as
-// (logit - m) c, two roundings that need no M.
+// (logit / 2 - m / 2) 2 c, two roundings that need no M (halves, since the difference of two fp32 numbers may have none).  So is every row at a temperature
+// above 1.4e20: -inf is raised to -1e30 in the sums, which is nothing only while 1e30 c is far above 2^30.
 //
 // The top tokens come from the same pass.  A token's key is its logit, made an unsigned number of the same order, above the
 // complement of its index: keys differ, and ties go to the lower index.  Each thread knows the vector with its largest logit; the k-th
@@ -28,6 +29,7 @@ constexpr int kLpStream = 256;    // threads that stream a row; a warp more fini
 constexpr int kLpCtas = 4;        // of an SM
 constexpr float kLpBig = 1073741824.f;  // 2^30: M is kept within it
 constexpr float kLpCold = 1.17549435e-38f;  // lowest temperature, the smallest normal number: its reciprocal, and that times log2(e), are finite
+constexpr float kLpHot = 1e-20f;  // least c of the sums in one pass: 1e30 c is then 1e10, so what was raised to -1e30 has the power 0 against every M
 constexpr float kLpFar = -1e4f;  // an exponent whose power is 0: keeps 0 times infinity out of the sums
 constexpr int kLpFound = 512;     // tokens found above the bound that are ranked at once
 
@@ -114,7 +116,7 @@ struct LpParams {
   float *logprob, *entropy, *top_logprobs;
   int* top_ids;
   int R, V, k;
-  float c, inv_t;  // log2(e) / temperature, 1 / temperature
+  float c, c2, inv2;  // log2(e), 2 log2(e) and 2, each / temperature
   int* status;
 };
 
@@ -505,9 +507,9 @@ __global__ void __launch_bounds__(kLpStream + 32, kLpCtas) token_logprobs_kernel
       __syncwarp();
       if (lane < p.k) top = best[lane];
     }
-    // A row beyond M's range: once more, by this warp alone.
+    // A row beyond M's range, or at a temperature beyond that of one pass: once more, by this warp alone.
     const float m = a.m;
-    const bool far = m < INFINITY && m > -INFINITY && (!(fabsf(m * p.c) < kLpBig) || p.c > 1e7f);
+    const bool far = m < INFINITY && m > -INFINITY && (!(fabsf(m * p.c) < kLpBig) || p.c > 1e7f || p.c < kLpHot);
     if (far) {
       float s = 0.f, w = 0.f;
       for (int vec = lane; vec < row.n; vec += 32) {
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(kLpStream + 32, kLpCtas) token_logprobs_kernel
         unpack16<T>(row.raw(vec), x);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float y = (x[i] - m) * p.c, e = lp_exp2(y);
+          const float y = fmaf(x[i], 0.5f, -0.5f * m) * p.c2, e = lp_exp2(y);
           s += e;
           w = fmaf(e, fmaxf(y, kLpFar), w);
         }
@@ -525,11 +527,11 @@ __global__ void __launch_bounds__(kLpStream + 32, kLpCtas) token_logprobs_kernel
     }
     const float log_s = log2f(a.s);
     // nothing but -inf, or something that is not a number or +inf: no distribution
-    const bool none = !(a.s > 0.f) || !(m < INFINITY);
+    const bool none = !(a.s > 0.f) || !(m < INFINITY) || m == -INFINITY;
     const float nan = __int_as_float(0x7fc00000);
     auto logprob = [&](float z) {
       if (none) return nan;
-      if (far || z * p.c < -1e30f) return fmaf(z - m, p.inv_t, -log_s * kLn2);
+      if (far || z * p.c < -1e30f) return fmaf(fmaf(z, 0.5f, -0.5f * m), p.inv2, -log_s * kLn2);
       return (fmaf(z, p.c, -a.M) - log_s) * kLn2;
     };
     if (lane == 0) {
@@ -594,7 +596,7 @@ extern "C" int dgpt_token_logprobs(const void* logits, int64_t logits_row_stride
   DGPT_REQUIRE(logits && targets && logprob && entropy && (top_k == 0 || (top_ids && top_logprobs)), "token_logprobs: NULL pointer");
   DGPT_REQUIRE(logits_row_stride >= V || R == 1, "token_logprobs: rows overlap");
   DGPT_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (dtype == DGPT_F32 ? 4 : 2) == 0, "token_logprobs: logits are not aligned to their type");
-  LpParams p = {logits, R == 1 ? (int64_t)V : logits_row_stride, targets, logprob, entropy, top_logprobs, top_ids, R, V, top_k, kLog2e / temperature, 1.f / temperature, status};
+  LpParams p = {logits, R == 1 ? (int64_t)V : logits_row_stride, targets, logprob, entropy, top_logprobs, top_ids, R, V, top_k, kLog2e / temperature, 2.f * kLog2e / temperature, 2.f / temperature, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == DGPT_F32 ? logprobs_launch<float>(p, st) : logprobs_launch<__nv_bfloat16>(p, st);
 }

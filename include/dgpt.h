@@ -635,7 +635,7 @@ int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv_layout* kv
  * A logit of -inf is a token that cannot come (probability 0, log probability -inf).  A row that holds a NaN or +inf, or nothing but -inf, has no
  * distribution: its numbers are NaN (its top ids are those of its largest logits, NaN behind all others).
  * logits: device [R, V] with row stride, rows on any boundary of their type; targets: device
- * int32 [R]; temperature: from the smallest normal number on; outputs: fp32 and int32.  A target outside [0, V) gives NaN for its logprob and sets bit 2 of *status (status may be NULL). */
+ * int32 [R]; temperature: from the smallest normal number to the largest; outputs: fp32 and int32.  A target outside [0, V) gives NaN for its logprob and sets bit 2 of *status (status may be NULL). */
 int dgpt_token_logprobs(const void* logits, int64_t logits_row_stride, const int32_t* targets, float temperature, float* logprob,
                         float* entropy, int32_t* top_ids, float* top_logprobs, int32_t top_k, int32_t R, int32_t V, int32_t dtype,
                         int32_t* status, void* stream);
