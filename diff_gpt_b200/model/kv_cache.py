@@ -105,6 +105,7 @@ class PagedKVCache:
     pool            (n_layer, n_pages, 2, n_head, page_tokens, head_dim)
     prefix_table    (n_series, prefix_pages)            int32  -> prompt pages of a series
     row_table       (n_rows, prefix_pages + own_pages)  int32  -> same prompt pages, then the row's own run
+    keep_table      the pages that accepted drafts may move between: row_table, without the prompt's where rows share them
     Rows are series-major: row = series * rows_per_series + trajectory.
     A row's generated token g sits at logical slot prefix_pages * page_tokens + g.
     """
@@ -143,9 +144,13 @@ class PagedKVCache:
         own = n_series * self.prefix_pages + torch.arange(self.n_rows * self.own_pages, dtype=torch.int32).view(
             self.n_rows, self.own_pages
         )
-        row = torch.cat([pre.repeat_interleave(rows_per_series, dim=0), own], dim=1)
+        prompts = pre.repeat_interleave(rows_per_series, dim=0)
         self.prefix_table = pre.contiguous().to(device)
-        self.row_table = row.contiguous().to(device)
+        if rows_per_series == 1:
+            self.row_table = self.keep_table = torch.cat([prompts, own], dim=1).to(device)
+        else:
+            both = [torch.cat([p, own], dim=1) for p in (prompts, torch.full_like(prompts, -1))]
+            self.row_table, self.keep_table = torch.stack(both).to(device).unbind()
         self.suffix_slot0 = self.prefix_pages * pt
 
     @property
@@ -179,8 +184,8 @@ class PagedKVCache:
     def keep_drafts(self, src_start: torch.Tensor, dst_start: torch.Tensor, path: torch.Tensor, count: torch.Tensor,
                     status: torch.Tensor | None = None) -> None:
         """What drafts path[r, :count[r]] of every row hold in slots from src_start[r] on moves to the slots from dst_start[r] on, in all
-        layers.  Slots are a row's own (those of its table); the shared prompt's are not written."""
-        ops.kv_keep(self.row_layout(0), src_start, dst_start, path, count, n_layer=self.n_layer, layer_stride=self.pool.stride(0),
+        layers.  A slot in a prompt that rows share does not exist here: what would move from or to it stays, and sets bit 0 of `status`."""
+        ops.kv_keep(self._layout(0, self.keep_table), src_start, dst_start, path, count, n_layer=self.n_layer, layer_stride=self.pool.stride(0),
                     H=self.n_head, D=self.head_dim, dtype=self.pool.dtype, status=status)
 
 

@@ -124,3 +124,12 @@ def test_paged_caches_keep_as_many_rows_as_they_have(no_gpu):
     with pytest.raises(ValueError, match="page table"):
         call_tree(c.prefix_layout(0), 4)  # one row a series
     assert no_gpu == ["kv_keep"]
+
+
+def test_the_pages_that_kept_drafts_may_move_between():
+    """A row's own alone where a prompt is shared; all of them where the prompt is the row's."""
+    for rows in (1, 3):
+        c = PagedKVCache(L, G, D, n_series=2, rows_per_series=rows, prefix_len=70, max_new=130, dtype=torch.float32, device="cpu")
+        assert c.keep_table.dtype == torch.int32 and c.keep_table.is_contiguous() and c.row_table.is_contiguous()
+        assert torch.equal(c.keep_table[:, 2:], c.row_table[:, 2:])
+        assert torch.equal(c.keep_table[:, :2], c.row_table[:, :2] if rows == 1 else torch.full((6, 2), -1, dtype=torch.int32))
