@@ -149,6 +149,7 @@ PROTOTYPES = {
         [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32,
          _i32, _p, _p],
     ),
+    "dgpt_packed_wait_probe": (C.c_int, [_i64, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _p]),
     "dgpt_tree_attn_splits": (_i32, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "dgpt_tree_attn_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32]),
     "dgpt_tree_attn": (

@@ -41,6 +41,7 @@ extern "C" int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_h
   p.n_seq = n_seq; p.n_rows = n_rows; p.n_keys = n_keys; p.H = H; p.G = G;
   p.scale_log2 = scale * kLog2e;
   p.status = status;
+  p.wait_limit = 0;
   const bool tensor = packed_tc_supported(p, D, dtype);
   if (tensor && impl != 1) return packed_tc(p, D, static_cast<cudaStream_t>(stream));
   if (impl == 2) {
@@ -48,6 +49,27 @@ extern "C" int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_h
     return DGPT_E_UNSUPPORTED;
   }
   return packed_simt(p, D, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dgpt_packed_wait_probe(int64_t limit_cycles, const void* x, void* o, const int32_t* seq_starts, int32_t n_seq, int32_t n_rows, int32_t H,
+                                      int32_t D, int32_t* status, void* stream) {
+  DGPT_REQUIRE(limit_cycles > 0 && limit_cycles <= 2000000000ll, "packed_wait_probe: limit must be in (0, 2e9] cycles");
+  DGPT_REQUIRE(x && o && seq_starts && status && aligned16(x) && aligned16(o), "packed_wait_probe: NULL or unaligned pointer");
+  DGPT_REQUIRE(n_seq > 0 && n_rows > 0 && n_rows <= 1 << 20 && H > 0, "packed_wait_probe: bad sizes");
+  PackedProblem p = {};
+  p.q = p.k = p.v = x;
+  p.o = o;
+  p.q_rs = p.k_rs = p.v_rs = p.o_rs = (long long)H * D;
+  p.q_hs = p.k_hs = p.v_hs = p.o_hs = D;
+  p.q_starts = p.k_starts = seq_starts;
+  p.n_seq = n_seq; p.n_rows = p.n_keys = n_rows; p.H = p.G = H;
+  p.scale_log2 = kLog2e / (float)D;
+  p.status = status;
+  if (!packed_tc_supported(p, D, DGPT_BF16)) {
+    set_error("packed_wait_probe: the tensor-core kernel does not cover head_dim %d", D);
+    return DGPT_E_UNSUPPORTED;
+  }
+  return packed_tc(p, D, static_cast<cudaStream_t>(stream), limit_cycles);
 }
 
 // One round of CTAs: a share is as long as its sequences allow.  The tensor-core kernel takes 128 rows an item and one CTA an SM; shares of its below two tiles
@@ -136,6 +158,7 @@ extern "C" int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv
   p.rows_per_tile = p.tiles = p.tile_keys = 0;
   p.scale_log2 = scale * kLog2e;
   p.status = status;
+  p.wait_limit = 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool tensor = tree_tc_supported(p, dtype);
   if (impl == 2 && !tensor) {

@@ -45,6 +45,7 @@ struct PackedProblem {
   int n_seq, n_rows, n_keys, H, G;
   float scale_log2;
   int* status;
+  long long wait_limit;  // of the tensor-core kernel's waits, clock cycles
 
   __host__ __device__ long long slots(int bm) const { return (long long)n_rows / bm + n_seq; }
   // A start is taken into the tensor's rows: wrong numbers give wrong rows, never an access outside.
@@ -148,6 +149,7 @@ struct TreeProblem {
   int tile_keys;  // keys of a tile, as the pass that joins the splits counts them
   float scale_log2;
   int* status;
+  long long wait_limit;  // of the tensor-core kernel's waits, clock cycles
 
   __host__ __device__ long long items() const { return (long long)B * G * tiles * n_splits; }  // below 2^31 (the entry point sees to it)
   __device__ long long room() const { return min((long long)(kv.page_table ? kv.max_pages : 1) * kv.page_tokens, kRgMost); }
@@ -244,7 +246,7 @@ int packed_simt(const PackedProblem& p, int D, int dtype, cudaStream_t st);
 int tree_simt(const TreeProblem& p, int dtype, cudaStream_t st);
 // ragged_tc.cu: bf16, head_dim 32, 64 or 128
 bool packed_tc_supported(const PackedProblem& p, int D, int dtype);
-int packed_tc(const PackedProblem& p, int D, cudaStream_t st);
+int packed_tc(const PackedProblem& p, int D, cudaStream_t st, long long wait_limit = 0);  // limit 0: the library's
 bool tree_tc_supported(const TreeProblem& p, int dtype);
 int tree_tc(const TreeProblem& p, cudaStream_t st);
 // n_splits partials of every row into one (ragged_simt.cu)

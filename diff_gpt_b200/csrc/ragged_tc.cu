@@ -22,7 +22,8 @@
 // ones 106 instead of 102, 8 of 4096 597 instead of 615; not kept.)
 // TMEM columns: S0 [0,128)  S1 [128,256)  P0 [256,320)  P1 [320,384)  O [384, 384 + D).
 // No cluster launch and no multicast.  Every wait is bounded in clock cycles; one that runs out raises the CTA's abort flag, on which the other
-// roles stop too, sets bit 1 of the status word, and the CTA drains its copies, frees its TMEM and returns.
+// roles stop too, and sets bit 1 of the status word.  However the CTA ends, copies and products that were issued are waited for (with a limit) before it frees its
+// TMEM and returns.
 #include <type_traits>
 
 #include "ragged.cuh"
@@ -36,8 +37,8 @@ constexpr int kRtThreads = 512;
 constexpr int kRtRegs = 128, kRtSoftmaxRegs = 152, kRtHelperRegs = 80;
 static_assert(2 * kRtSoftmaxRegs + kRtRegs + kRtHelperRegs == 4 * kRtRegs, "the warpgroups share what the launch has");
 constexpr int kRtLead = 3;                                                    // key tiles still to be loaded when the next item is asked for
-// Limit of the waits that may last a whole item, 3 x 10^9 keys here; the others, of a tile or two, run out first and raise the abort flag.
-constexpr long long kRtItemCycles = 16 * kWaitLimitCycles;
+// Limit of the waits that may last a whole item, 3 x 10^9 keys here, in limits of the others, which last a tile or two, run out first and raise the abort flag.
+constexpr int kRtItemWaits = 16;
 constexpr int kRtRing = 8;                                                    // items between the warp that finds them and the last role that reads them
 
 struct RtItem {
@@ -170,7 +171,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
   uint8_t* sV = smem + 4 * kTileBytes;  // Q0 Q1 | K0 K1 | V0 V1 | barriers | row sums | items | output | order
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * kTileBytes);
   constexpr int iQ = 0, iQF = 2, iK = 4, iKF = 6, iV = 8, iS = 10, iP = 12, iO = 14, iOF = 16, iL = 17, iLF = 19, iR = 21, iRF = iR + kRtRing,
-                iC = iRF + kRtRing, nBars = iC + 1;
+                iC = iRF + kRtRing, iD = iC + 1, nBars = iD + 1;
   static_assert(nBars <= 43, "barriers, an answer of 16 bytes and three words in 48 words");
   uint64_t* answer = bars + 44;  // 16-byte aligned
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 43);
@@ -207,13 +208,14 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
   RtItem x;
   // A role's place in the ring.  `take` waits for the next item and reads it (every lane that calls gets it); false at the end or after a
   // wait that ran out (`ok` tells).  A slot is free when the loader, the issuer and every softmax and output warp have said `done`.
+  auto wait_tile = [&](int b, unsigned parity) { return wait_or_abort(bar(b), parity, abort_flag, 2, p.wait_limit); };
   // (Output and item warps wait for thousands of cycles at a time: they sleep between looks, so that their polling takes no issue slots from
   // the softmax warps that share their schedulers.)
   auto wait_asleep = [&](int b, unsigned parity) -> bool {
     const long long t0 = clock64();
     while (!mbar_try_wait(bar(b), parity)) {
       if (*abort_flag) return false;
-      if (clock64() - t0 > kRtItemCycles) {
+      if (clock64() - t0 > kRtItemWaits * p.wait_limit) {
         *abort_flag = 2;
         return false;
       }
@@ -223,7 +225,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
   };
   unsigned taken = 0u;
   auto take = [&](RtItem& y, unsigned at, bool& ok) -> bool {
-    ok = wait_or_abort(bar(iR + (int)(at % kRtRing)), (at / kRtRing) & 1u, abort_flag);
+    ok = wait_tile(iR + (int)(at % kRtRing), (at / kRtRing) & 1u);
     if (!ok) return false;
     y = *reinterpret_cast<const RtItem*>(ring + (at % kRtRing) * 64);
     return y.n >= 0;
@@ -241,7 +243,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       }
       unsigned items = 0u, kn = 0u, vn = 0u;  // loads issued: Q, K tiles, V tiles
       bool ok = true;
-      auto wait = [&](int b, unsigned parity) { return __all_sync(0xffffffffu, wait_or_abort(bar(b), parity, abort_flag)) != 0; };
+      auto wait = [&](int b, unsigned parity) { return __all_sync(0xffffffffu, wait_tile(b, parity)) != 0; };
       // tree: this lane holds the numbers of pages page0 + lane and page0 + 32 + lane of sequence page_seq, the latter on their way while the
       // former are used, and those of page `lane` of the last two K tiles, of which one is the next V tile
       int page0 = 0, page_seq = -1, page_id = 0, page_next = 0, newer = 0, older = 0;
@@ -349,12 +351,12 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         __syncwarp();
         if (lane == 0) done(taken - 1);
       }
-      if (!ok || *abort_flag) {  // something ran out of time: give the copies still in flight a bounded chance to land
-        if (lane == 0 && p.status) atomicOr(p.status, 2);
-        for (unsigned i = 0; i < 2u && i < items; ++i) mbar_wait(bar(iQ + (int)((items - 1 - i) & 1u)), ((items - 1 - i) >> 1) & 1u);
-        for (unsigned i = 0; i < 2u && i < kn; ++i) mbar_wait(bar(iK + (int)((kn - 1 - i) & 1u)), ((kn - 1 - i) >> 1) & 1u);
-        for (unsigned i = 0; i < 2u && i < vn; ++i) mbar_wait(bar(iV + (int)((vn - 1 - i) & 1u)), ((vn - 1 - i) >> 1) & 1u);
-      }
+      if ((!ok || *abort_flag) && lane == 0 && p.status) atomicOr(p.status, 2);
+      // Copies still in flight write shared memory.  (Another role may give up after the last of them was asked for, so they are waited for in any case; at a
+      // usual end the products have.)
+      for (unsigned i = 0; i < 2u && i < items; ++i) mbar_wait(bar(iQ + (int)((items - 1 - i) & 1u)), ((items - 1 - i) >> 1) & 1u);
+      for (unsigned i = 0; i < 2u && i < kn; ++i) mbar_wait(bar(iK + (int)((kn - 1 - i) & 1u)), ((kn - 1 - i) >> 1) & 1u);
+      for (unsigned i = 0; i < 2u && i < vn; ++i) mbar_wait(bar(iV + (int)((vn - 1 - i) & 1u)), ((vn - 1 - i) >> 1) & 1u);
     } else if (warp == 12) {
       // ================= MMA issuer (one lane) =================
       if (lane == 0) {
@@ -367,11 +369,11 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         bool more = take_one(y, ahead);
         auto issue_s = [&]() {  // S(sg & 1) = Q K(sg & 1)^T
           if (sj == 0) {
-            ok = wait_or_abort(bar(iQ + (int)(items & 1u)), (items >> 1) & 1u, abort_flag);
+            ok = wait_tile(iQ + (int)(items & 1u), (items >> 1) & 1u);
             ++items;
           }
           const unsigned qs = (items - 1u) & 1u, buf = sg & 1u;
-          ok = ok && wait_or_abort(bar(iK + (int)buf), (sg >> 1) & 1u, abort_flag);
+          ok = ok && wait_tile(iK + (int)buf, (sg >> 1) & 1u);
           if (!ok) return;
           tc_fence_after();
           umma_ss_chain<D / 16>(tmem + buf * 128, dQK + ((aQ + qs * kTileBytes) >> 4), dQK + ((aK + buf * kTileBytes) >> 4), kIdescS, kSubBytes >> 4);
@@ -390,9 +392,9 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
           for (int j = 0; ok && j < x.n; ++j, ++g) {
             const unsigned buf = g & 1u, ph = (g >> 1) & 1u;
             // P_g is complete when every row has arrived; by then every row has also consumed S_g
-            ok = wait_or_abort(bar(iP + (int)buf), ph, abort_flag) && wait_or_abort(bar(iV + (int)buf), ph, abort_flag);
+            ok = wait_tile(iP + (int)buf, ph) && wait_tile(iV + (int)buf, ph);
             if (ok && j == 0) {
-              if (outs > 0) ok = wait_or_abort(bar(iOF), (outs - 1) & 1u, abort_flag);  // O of the item before has been read
+              if (outs > 0) ok = wait_tile(iOF, (outs - 1) & 1u);  // O of the item before has been read
               ++outs;
             }
             if (!ok) break;
@@ -406,6 +408,11 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         if (!ok) {
           if (!*abort_flag) *abort_flag = 2;
           if (p.status) atomicOr(p.status, 2);
+        }
+        // Products still in flight read shared memory, write TMEM and arrive on barriers.  (At a usual end they are done: the output warps have waited for them.)
+        if (sg > 0u) {
+          umma_commit(bar(iD));
+          if (!mbar_wait(bar(iD), 0u) && p.status) atomicOr(p.status, 2);
         }
       }
     } else if (warp == 14) {
@@ -436,7 +443,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         const long long t0 = clock64();
         while (handed - *loaded > (unsigned)kRtLead) {
           if (*abort_flag) return false;
-          if (clock64() - t0 > kRtItemCycles) {
+          if (clock64() - t0 > kRtItemWaits * p.wait_limit) {
             *abort_flag = 2;
             return false;
           }
@@ -513,7 +520,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       const float l = sums[slot * 2 * kBM + row], m = sums[(slot * 2 + 1) * kBM + row];
       mbar_arrive(bar(iLF + slot));
       const unsigned last = g + (unsigned)x.n - 1u;
-      ok = __all_sync(0xffffffffu, wait_or_abort(bar(iO + (int)(last & 1u)), (last >> 1) & 1u, abort_flag)) != 0;
+      ok = __all_sync(0xffffffffu, wait_tile(iO + (int)(last & 1u), (last >> 1) & 1u)) != 0;
       if (!ok) break;
       tc_fence_after();
       g += (unsigned)x.n;
@@ -596,14 +603,14 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       for (int j = 0; j < n; ++j, ++g, t0 += kBN) {
         const unsigned buf = g & 1u, ph = (g >> 1) & 1u;
         // exits are taken by whole warps (the vote makes the decision uniform), never by single lanes
-        if (!__all_sync(0xffffffffu, wait_or_abort(bar(iS + (int)buf), ph, abort_flag))) {
+        if (!__all_sync(0xffffffffu, wait_tile(iS + (int)buf, ph))) {
           fail = true;
           break;
         }
         tc_fence_after();
         const bool in_gap = TREE && t0 < gap1 && t0 + kBN > gap0;
         if (__builtin_expect(t0 + kBN > held_end || in_gap, 0)) {  // clear those rows so that 0 * x stays 0
-          if (!__all_sync(0xffffffffu, wait_or_abort(bar(iV + (int)buf), ph, abort_flag))) {
+          if (!__all_sync(0xffffffffu, wait_tile(iV + (int)buf, ph))) {
             fail = true;
             break;
           }
@@ -786,7 +793,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
             }
           if (j > 0 && __any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
             // O may only be touched when no product into it is in flight: that of the tile before must be done (this tile's waits for these rows)
-            if (!__all_sync(0xffffffffu, wait_or_abort(bar(iO + (int)(buf ^ 1u)), ((g - 1) >> 1) & 1u, abort_flag))) {
+            if (!__all_sync(0xffffffffu, wait_tile(iO + (int)(buf ^ 1u), ((g - 1) >> 1) & 1u))) {
               fail = true;
               break;
             }
@@ -811,7 +818,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       if (fail) break;
       // the item's sums go to the output threads
       const int slot = (int)(items & 1u);
-      if (items >= 2 && !__all_sync(0xffffffffu, wait_or_abort(bar(iLF + slot), ((items - 2) >> 1) & 1u, abort_flag))) {
+      if (items >= 2 && !__all_sync(0xffffffffu, wait_tile(iLF + slot, ((items - 2) >> 1) & 1u))) {
         fail = true;
         break;
       }
@@ -827,7 +834,10 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       mbar_arrive(bar(iL + slot));
       ++items;
     }
-    if (fail && p.status) atomicOr(p.status, 2);
+    if (fail) {
+      tc_wait_st();  // probabilities of a tile that was given up
+      if (p.status) atomicOr(p.status, 2);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -877,8 +887,10 @@ static bool tc_type(int D, int dtype) {
 
 bool packed_tc_supported(const PackedProblem& p, int D, int dtype) { return p.n_keys > 0 && tc_type(D, dtype); }
 
-int packed_tc(const PackedProblem& p, int D, cudaStream_t st) {
+int packed_tc(const PackedProblem& full, int D, cudaStream_t st, long long wait_limit) {
   using namespace tc;
+  PackedProblem p = full;
+  p.wait_limit = wait_limit > 0 ? wait_limit : kWaitLimitCycles;
   TcMaps maps;
   const cuuint32_t box[4] = {64, 1, (cuuint32_t)kBM, 1};
   auto map = [&](CUtensorMap* m, const void* base, int heads, int rows, long long rs, long long hs) {
@@ -905,6 +917,7 @@ bool tree_tc_supported(const TreeProblem& p, int dtype) {
 int tree_tc(const TreeProblem& full, cudaStream_t st) {
   using namespace tc;
   TreeProblem p = full;
+  p.wait_limit = kWaitLimitCycles;
   const int nodes = kBM / p.group < p.T ? kBM / p.group : p.T;  // drafts of a tile, with all heads of a group
   p.rows_per_tile = nodes * p.group;
   p.tiles = (p.T + nodes - 1) / nodes;

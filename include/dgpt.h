@@ -609,6 +609,12 @@ int dgpt_fmha_packed(const void* q, int64_t q_row_stride, int64_t q_head_stride,
                      const int32_t* key_starts, int32_t n_seq, int32_t n_rows, int32_t n_keys, int32_t H, int32_t G, int32_t D,
                      float scale, int32_t dtype, int32_t impl, int32_t* status, void* stream);
 
+/* The tensor-core kernel of dgpt_fmha_packed with waits of at most limit_cycles clock cycles (up to 2e9; sixteen times that for those that may last a
+ * prompt's whole tile): where one runs out the kernel waits for what it has issued, sets bit 1 of *status and returns, and o is unspecified.
+ * x: bf16 [n_rows, H, D], queries, keys and values at once; o likewise; D = 32, 64 or 128. */
+int dgpt_packed_wait_probe(int64_t limit_cycles, const void* x, void* o, const int32_t* seq_starts, int32_t n_seq, int32_t n_rows, int32_t H,
+                           int32_t D, int32_t* status, void* stream);
+
 /* Attention of a tree of drafted tokens over a cache.  Sequence s has its cached tokens in slots 0 .. ctx_len[s] - 1, but for a gap
  * gap_start[s] .. gap_end[s] - 1 of slots that hold nothing (what a shared prompt leaves free of its last page; both NULL: none), and
  * n_nodes[s] drafts (NULL: T) in the slots behind them.  Draft t sees every cached token, and draft j of its own sequence where
