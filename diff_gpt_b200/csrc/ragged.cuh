@@ -114,9 +114,9 @@ struct PackedProblem {
   __device__ const T* v_row(const RaggedItem& it, int j) const {
     return static_cast<const T*>(v) + (long long)(it.kbase + j) * v_rs + (long long)it.g * v_hs;
   }
-  // The first CTA looks at all starts.
-  __device__ void check(int block, int thread, int threads) const {
-    if (block != 0 || status == nullptr) return;
+  // Whoever has the launch's first item looks at all starts.
+  __device__ void check(bool first, int thread, int threads) const {
+    if (!first || status == nullptr) return;
     bool bad = false;
     for (int s = thread; s <= n_seq; s += threads) {
       const int a = q_starts[s], b = k_starts[s];
@@ -229,9 +229,9 @@ struct TreeProblem {
     if (pg < 0 || (kv.n_pages > 0 && pg >= kv.n_pages)) return -1;
     return pg * kv.page_stride + (long long)it.g * kv.head_stride + (long long)in * kv.token_stride;
   }
-  // The first CTA looks at all lengths.
-  __device__ void check(int block, int thread, int threads) const {
-    if (block != 0 || status == nullptr) return;
+  // Whoever has the launch's first item looks at all lengths.
+  __device__ void check(bool first, int thread, int threads) const {
+    if (!first || status == nullptr) return;
     for (int s = thread; s < B; s += threads) {
       const int n = n_nodes ? n_nodes[s] : T;
       bool bad = ctx[s] < 0 || n < 0 || n > T || (long long)ctx[s] + n > room();

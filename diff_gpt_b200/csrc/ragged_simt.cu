@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(kRgThreads) ragged_simt_kernel(const P p) {
 
   const int tid = threadIdx.x, tx = tid % LX, row0 = tid / LX * RM, group = tx / (LX / KG);
   auto column = [&](int c) { return c / CV * LX * CV + tx % (LX / KG) * CV + c % CV; };
-  p.check((int)blockIdx.x, tid, kRgThreads);
+  p.check(blockIdx.x == 0, tid, kRgThreads);
   RaggedItem it;
   if constexpr (TREE) {
     if (!p.item(blockIdx.x, kRgBN, it) || (p.n_splits > 1 && it.key0 >= it.key1)) return;

@@ -424,7 +424,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
       std::conditional_t<TREE, TreeItems, PackedItems> items(p, reinterpret_cast<int*>(ring + kRtRing * 64 + 4 * 4096), lane);
       unsigned at = 0u, freed = 0u, asked = 0u, cta = blockIdx.x;  // items handed out, items finished
       unsigned handed = 0u;                                        // key tiles of the items handed out
-      bool ok = true, more = true;
+      bool ok = true, more = true, first = false;  // first: item 0 is this CTA's
       auto push = [&]() {
         if (at - freed >= (unsigned)kRtRing) {
           ok = __all_sync(0xffffffffu, wait_asleep(iRF + (int)(freed % kRtRing), (freed / kRtRing) & 1u)) != 0;
@@ -452,6 +452,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         return true;
       };
       while (ok && more) {
+        first = first || cta == 0u;
         if (items.get(cta, x.it, lane)) {
           x.tile0 = x.it.key0 / kBN;
           x.n = (x.it.key1 - x.it.key0 + kBN - 1) / kBN;
@@ -476,7 +477,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         push();
       }
       if (!ok && lane == 0 && p.status) atomicOr(p.status, 2);
-      p.check((int)blockIdx.x, lane, 32);
+      p.check(first, lane, 32);  // (CTA 0 itself may never be launched, its number being another's)
     }
   } else if (warp >= 8) {
     // ================= output =================
