@@ -847,46 +847,45 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
 
 }  // namespace tc
 
+constexpr size_t ragged_smem(int D) {
+  const size_t smem = (size_t)6 * (D / 64) * tc::kBN * 128 + 48 * 8 + 4 * tc::kBM * 4 + tc::kRtRing * 64 + 4 * 4096 + TreeProblem::kSorted * 4 + 1024;
+  return smem < 120 * 1024 ? 120 * 1024 : smem;  // one CTA owns an SM: it takes all 512 TMEM columns
+}
+
+// Whether the kernel can run on the current device: setmaxnreg would wait for registers that a launch with fewer a thread does not have.
+// (A compiler that gives it another number leaves the calls to the CUDA cores.)
+template <int D, class P, bool TREE>
+static bool ragged_tc_ready() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  static signed char known[64] = {};  // 1: yes, -1: no; both are a device's for good
+  if (known[dev] == 0) {
+    auto kernel = tc::ragged_tc_kernel<D, P, TREE>;
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) return false;
+    if (attr.numRegs == tc::kRtRegs && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ragged_smem(D)) != cudaSuccess) return false;
+    known[dev] = attr.numRegs == tc::kRtRegs ? 1 : -1;
+  }
+  return known[dev] > 0;
+}
+
 template <int D, class P, bool TREE>
 static int ragged_tc_go(const TcMaps& maps, const P& p, long long items, int d_head, cudaStream_t st) {
-  using namespace tc;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
-    set_error("ragged attention: cannot identify the current device");
-    return DGPT_E_CUDA;
-  }
   if (items > 0x7fffffffll) {
     set_error("ragged attention: too many rows");
     return DGPT_E_ARG;
   }
-  size_t smem = (size_t)6 * (D / 64) * kBN * 128 + 48 * 8 + 4 * kBM * 4 + kRtRing * 64 + 4 * 4096 + TreeProblem::kSorted * 4 + 1024;
-  if (smem < 120 * 1024) smem = 120 * 1024;  // one CTA owns an SM: it takes all 512 TMEM columns
-  auto kernel = ragged_tc_kernel<D, P, TREE>;
-  cudaError_t e = cudaSuccess;
-  static bool ready[64] = {};  // the attribute is a device's for good
-  if (!ready[dev]) {
-    cudaFuncAttributes attr;
-    e = cudaFuncGetAttributes(&attr, kernel);
-    if (e == cudaSuccess && attr.numRegs != kRtRegs) {  // setmaxnreg would wait for registers that the launch does not have
-      set_error("ragged attention: built with %d registers a thread instead of %d", attr.numRegs, kRtRegs);
-      return DGPT_E_UNSUPPORTED;
-    }
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    ready[dev] = e == cudaSuccess;
-  }
-  if (e != cudaSuccess) {
-    set_error("ragged attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-    return DGPT_E_CUDA;
-  }
-  kernel<<<(unsigned)items, kRtThreads, smem, st>>>(maps.q, maps.k, maps.v, p, d_head);
+  tc::ragged_tc_kernel<D, P, TREE><<<(unsigned)items, tc::kRtThreads, ragged_smem(D), st>>>(maps.q, maps.k, maps.v, p, d_head);
   return launch_status("ragged attention");
 }
 
+template <class P, bool TREE>
 static bool tc_type(int D, int dtype) {
-  return dtype == DGPT_BF16 && (D == 32 || D == 64 || D == 128) && tc::device_is_sm100() && tc::encode_fn() != nullptr;
+  return dtype == DGPT_BF16 && (D == 32 || D == 64 || D == 128) && tc::device_is_sm100() && tc::encode_fn() != nullptr &&
+         (D == 128 ? ragged_tc_ready<128, P, TREE>() : ragged_tc_ready<64, P, TREE>());
 }
 
-bool packed_tc_supported(const PackedProblem& p, int D, int dtype) { return p.n_keys > 0 && tc_type(D, dtype); }
+bool packed_tc_supported(const PackedProblem& p, int D, int dtype) { return p.n_keys > 0 && tc_type<PackedProblem, false>(D, dtype); }
 
 int packed_tc(const PackedProblem& full, int D, cudaStream_t st, long long wait_limit) {
   using namespace tc;
@@ -910,7 +909,7 @@ int packed_tc(const PackedProblem& full, int D, cudaStream_t st, long long wait_
 // run's tensor, and what the box covers past its end arrives as zeros.
 bool tree_tc_supported(const TreeProblem& p, int dtype) {
   const int pt = p.kv.page_tokens;
-  if (!tc_type(p.D, dtype) || p.group > tc::kBM) return false;
+  if (!tc_type<TreeProblem, true>(p.D, dtype) || p.group > tc::kBM) return false;
   if (p.kv.head_stride <= 0 || p.kv.page_stride <= 0) return false;
   return p.kv.page_table == nullptr || (pt >= tc::kBN ? pt % tc::kBN == 0 : pt >= 8 && tc::kBN % pt == 0);
 }
