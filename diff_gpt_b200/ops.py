@@ -1166,6 +1166,15 @@ def _covers(name: str, kv: KvLayout, B: int, heads: int, D: int, token_stride: i
             raise ValueError(f"{name}: the layout reaches outside its tensors' storage ({B} sequences, {pages} pages, {heads} heads of {D}, {n_layer} layers)")
 
 
+_MOST = 2**31 - 1
+
+
+def _counts(name: str, *n: int) -> None:
+    """The library takes counts in 32 bits; the bits above are cut off on the way to it."""
+    if max(n) > _MOST:
+        raise ValueError(f"{name}: more than {_MOST} rows or columns do not fit 32 bits, got {max(n)}")
+
+
 def _i32(name: str, t: torch.Tensor | None, shape: tuple[int, ...]) -> None:
     if t is not None and (t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
@@ -1198,6 +1207,7 @@ def fmha_packed(
     if k.dtype is not dtype or v.dtype is not dtype or o.dtype is not dtype:
         raise TypeError("fmha_packed: q, k, v and o must have one dtype")
     (N, H, D), (M, G, _) = qsh, ksh
+    _counts("fmha_packed", N, M, seq_starts.numel())
     qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), o.stride()
     if D > 1 and (qs[2] != 1 or ks[2] != 1 or vs[2] != 1 or os_[2] != 1):
         raise ValueError("fmha_packed: the elements of a head must lie side by side")
@@ -1281,6 +1291,7 @@ def tree_attn(
         raise ValueError("tree_attn: ancestors must be a contiguous int64 tensor [B, T, W]")
     B, T, words = shape if len(shape) == 3 else (*shape, 1)
     rows = (B * T, H * D)
+    _counts("tree_attn", B, T)
     if q.shape != rows or out.shape != rows or q.dtype is not out.dtype:
         raise ValueError(f"tree_attn: q {tuple(q.shape)} and out {tuple(out.shape)} must be {rows} of one dtype")
     qs, os_ = q.stride(), out.stride()
@@ -1297,7 +1308,7 @@ def tree_attn(
     code = dtype_code(q)
     if n_splits == 0:
         held = (kv.max_pages if kv.page_table else 1) * kv.page_tokens
-        n_splits, need = _tree_plan(B, T, H, G, D, min(max_keys, held) if max_keys > 0 else held, code)
+        n_splits, need = _tree_plan(B, T, H, G, D, min(max_keys, held, _MOST) if max_keys > 0 else min(held, _MOST), code)
     else:
         need = tree_attn_workspace_bytes(B, T, H, D, n_splits)
     ws_bytes = 0
@@ -1339,6 +1350,7 @@ def token_logprobs(
     if len(shape) != 2 or shape[1] < 1:
         raise ValueError("token_logprobs: logits must be [R, V]")
     R, V = shape
+    _counts("token_logprobs", R, V)
     stride, side = logits.stride()
     if side != 1 and V > 1:
         raise ValueError("token_logprobs: the elements of a row must lie side by side")
@@ -1380,6 +1392,7 @@ def kv_keep(
     if len(shape) != 2:
         raise ValueError("kv_keep: path must be [B, T]")
     B, T = shape
+    _counts("kv_keep", B, T)
     _i32("path", path, shape)
     _i32("src_start", src_start, (B,))
     _i32("dst_start", dst_start, (B,))
