@@ -1149,30 +1149,32 @@ def _covers(name: str, kv: KvLayout, B: int, heads: int, D: int, token_stride: i
         return
     k, v, table = held
     if table is None:
+        pages = B
         if 0 < kv.n_pages < B:
             raise ValueError(f"{name}: {B} sequences in a cache of {kv.n_pages}")
-        pages = B
     else:
+        pages = kv.n_pages or 1  # (0: the caller answers for the table's numbers)
         if table.dtype is not torch.int32 or not table.is_contiguous() or table.numel() < B * kv.max_pages:
             raise ValueError(f"{name}: the page table must be contiguous int32 with a row for each of {B} sequences, got {table.dtype} {tuple(table.shape)}")
-        pages = kv.n_pages or 1  # (0: the caller answers for the table's numbers)
     if B < 1:
         return
-    layers = (n_layer - 1) * layer_stride
-    last = (pages - 1) * kv.page_stride + (heads - 1) * kv.head_stride + (kv.page_tokens - 1) * (token_stride or D) + D + max(layers, 0)
-    for t in (k, v):
-        at = t.storage_offset()
-        if (at + last) * t.element_size() > t.untyped_storage().nbytes() or at + layers < 0:
-            raise ValueError(f"{name}: the layout reaches outside its tensors' storage ({B} sequences, {pages} pages, {heads} heads of {D}, {n_layer} layers)")
+    last = (pages - 1) * kv.page_stride + (heads - 1) * kv.head_stride + (kv.page_tokens - 1) * (token_stride or D) + D
+    first = 0
+    if n_layer > 1:
+        layers = (n_layer - 1) * layer_stride
+        first, last = min(layers, 0), last + max(layers, 0)
+    k_at, v_at = k.storage_offset(), v.storage_offset()
+    size = k.itemsize
+    if (k_at + last) * size > k.untyped_storage().nbytes() or (v_at + last) * size > v.untyped_storage().nbytes() or k_at + first < 0 or v_at + first < 0:
+        raise ValueError(f"{name}: the layout reaches outside its tensors' storage ({B} sequences, {pages} pages, {heads} heads of {D}, {n_layer} layers)")
 
 
 _MOST = 2**31 - 1
 
 
-def _counts(name: str, *n: int) -> None:
-    """The library takes counts in 32 bits; the bits above are cut off on the way to it."""
-    if max(n) > _MOST:
-        raise ValueError(f"{name}: more than {_MOST} rows or columns do not fit 32 bits, got {max(n)}")
+def _too_many(name: str, *n: int) -> ValueError:
+    """The library takes counts in 32 bits; the bits above would be cut off on the way to it."""
+    return ValueError(f"{name}: counts above {_MOST} do not fit 32 bits, got {max(n)}")
 
 
 def _i32(name: str, t: torch.Tensor | None, shape: tuple[int, ...]) -> None:
@@ -1207,7 +1209,8 @@ def fmha_packed(
     if k.dtype is not dtype or v.dtype is not dtype or o.dtype is not dtype:
         raise TypeError("fmha_packed: q, k, v and o must have one dtype")
     (N, H, D), (M, G, _) = qsh, ksh
-    _counts("fmha_packed", N, M, seq_starts.numel())
+    if N > _MOST or M > _MOST or seq_starts.numel() > _MOST:
+        raise _too_many("fmha_packed", N, M, seq_starts.numel())
     qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), o.stride()
     if D > 1 and (qs[2] != 1 or ks[2] != 1 or vs[2] != 1 or os_[2] != 1):
         raise ValueError("fmha_packed: the elements of a head must lie side by side")
@@ -1291,7 +1294,8 @@ def tree_attn(
         raise ValueError("tree_attn: ancestors must be a contiguous int64 tensor [B, T, W]")
     B, T, words = shape if len(shape) == 3 else (*shape, 1)
     rows = (B * T, H * D)
-    _counts("tree_attn", B, T)
+    if B > _MOST or T > _MOST:
+        raise _too_many("tree_attn", B, T)
     if q.shape != rows or out.shape != rows or q.dtype is not out.dtype:
         raise ValueError(f"tree_attn: q {tuple(q.shape)} and out {tuple(out.shape)} must be {rows} of one dtype")
     qs, os_ = q.stride(), out.stride()
@@ -1350,7 +1354,8 @@ def token_logprobs(
     if len(shape) != 2 or shape[1] < 1:
         raise ValueError("token_logprobs: logits must be [R, V]")
     R, V = shape
-    _counts("token_logprobs", R, V)
+    if R > _MOST or V > _MOST:
+        raise _too_many("token_logprobs", R, V)
     stride, side = logits.stride()
     if side != 1 and V > 1:
         raise ValueError("token_logprobs: the elements of a row must lie side by side")
@@ -1392,7 +1397,8 @@ def kv_keep(
     if len(shape) != 2:
         raise ValueError("kv_keep: path must be [B, T]")
     B, T = shape
-    _counts("kv_keep", B, T)
+    if B > _MOST or T > _MOST:
+        raise _too_many("kv_keep", B, T)
     _i32("path", path, shape)
     _i32("src_start", src_start, (B,))
     _i32("dst_start", dst_start, (B,))
