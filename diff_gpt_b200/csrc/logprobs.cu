@@ -72,16 +72,6 @@ struct LpStat {  // largest logit m, sums against M (lp_ref(m)); m = -inf: nothi
   float m, M, s, w;
 };
 __device__ __forceinline__ float lp_ref(float m, float c) { return fminf(fmaxf(m * c, -kLpBig), kLpBig); }
-__device__ __forceinline__ LpStat lp_join(const LpStat& a, const LpStat& b) {
-  LpStat r;
-  r.m = fmaxf(a.m, b.m);
-  r.M = fmaxf(a.M, b.M);
-  const float da = fmaxf(a.M - r.M, kLpFar), db = fmaxf(b.M - r.M, kLpFar);
-  const float fa = lp_exp2(da), fb = lp_exp2(db);
-  r.s = a.s * fa + b.s * fb;
-  r.w = (a.w + a.s * da) * fa + (b.w + b.s * db) * fb;
-  return r;
-}
 // All lanes' sums, the same in every lane: over to the largest maximum, then added.
 __device__ __forceinline__ LpStat lp_warp_join(const LpStat& a) {
   LpStat r;

@@ -77,7 +77,9 @@ extern "C" int dgpt_packed_wait_probe(int64_t limit_cycles, const void* x, void*
 // a share each (four CTAs an SM), and tiles of 64 rows two (two CTAs an SM); up to 128 keys the second pass costs what it saves.
 // (us, bf16: 3 sequences of 40000 to 65000 keys, 64 drafts, 1 share 495, 6 as chosen 99, 8 134; 48 of 300 to 4000, 1 as chosen 53, 2 75; 8 of them 46, 4 as chosen 24, 8
 // 28; one draft behind 2000 keys 26, 8 as chosen 13.4.  fp32, heads of 16: 24 sequences of 30 to 500 keys, 13 drafts, 1 share 12.2, 2 11.0, 6 as chosen 9.5; 2000 keys, 150
-// drafts, 1 83, 17 as chosen 19, 24 15, 32 20; heads of 64: 1500 keys, one draft, 1 64, 6 15, 24 as chosen 8.5.)
+// drafts, 1 83, 17 as chosen 19, 24 15, 32 20; heads of 64: 1500 keys, one draft, 1 64, 6 15, 24 as chosen 8.5.  Where the number of shares and of tiles just miss one
+// another the rule is up to a quarter behind the best number: 24 above, or 4 sequences of 800 keys, 40 drafts, heads of 32, 6 as chosen 13.1, 7 11.1; 64 of 1000, 4 drafts, heads of
+// 128, 2 as chosen 77, 4 69.  It sees sizes only: a bf16 layout that the tensor-core kernel does not cover gets its number all the same.)
 extern "C" int32_t dgpt_tree_attn_splits(int32_t B, int32_t T, int32_t H, int32_t G, int32_t D, int32_t max_keys, int32_t dtype) {
   if (B <= 0 || T <= 0 || H <= 0 || G <= 0 || H % G != 0 || max_keys <= 0) return 1;
   const bool tensor = dtype == DGPT_BF16 && D >= 32;

@@ -4,7 +4,7 @@
 //   o_r = sum_j p_rj v_j,   p_r = softmax_j(q_r . k_j * scale) over the keys that row r sees,
 // and differ in which rows lie side by side, where keys lie and which of them a row sees.  A problem struct answers these for the
 // kernels (ragged_simt.cu on the CUDA cores, ragged_tc.cu on the tensor cores): `item` turns a work item's number into the rows
-// and keys of one tile, `q_row`, `k_row`, `v_row` give addresses, `sees` the mask, `o_row` where a row's result goes.
+// and keys of one tile, `q_row`, `k_row`, `v_row` give addresses, `sees` the mask, `out_row` and `head` where a tree's row goes.
 #pragma once
 
 #include "common.cuh"

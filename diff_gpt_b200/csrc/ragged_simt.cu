@@ -4,9 +4,9 @@
 // A CTA of 256 threads owns a tile of BM rows and walks through its keys 64 at a time with the running maximum and sum of a softmax.
 // Q, K, V and the probabilities of a step lie in shared memory as fp32; a row belongs to 16 or 32 threads of one warp, each with 4 or 2 rows, its share of
 // a step's scores and of the output's columns, so that a number fetched from shared memory feeds several products and no barrier stands between the two products.
-// fp32 products have no tensor-core form that keeps 24 bits; the floor is the FMA rate.  What bounds it: reads of shared memory and the softmax's shuffles
+// fp32 products stay on the FMA units, whose rate is the floor (three bf16 parts per operand on the tensor cores would come close to 24 bits: not tried).  What bounds it: reads of shared memory and the softmax's shuffles
 // between the products (8 prompts of 700, 8 heads of 64, 171 us, 54 at the FMA rate), and for small ones the chain of a CTA's few steps (32 of 20 to 140, 4
-// heads of 16, 14 us).  Trees of up to 16 rows take tiles of 16 (24 trees of 13 drafts behind 30 to 500 keys in two shares 12.2 us, with 64 rows 20.4).
+// heads of 16, 14 us).  Trees of up to 16 rows take tiles of 16 (24 trees of 13 drafts behind 30 to 500 keys in one share 12.2 us, with 64 rows 18.2; in six, as chosen, 9.5 and 15.2).
 #include "ragged.cuh"
 
 namespace dgpt {

@@ -720,6 +720,8 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                 float x0, x1;
                 unpack2(fma2(pack2(sv[4 * i + 2 * r], sv[4 * i + 2 * r + 1]), scale2, neg2[r]), x0, x1);
                 tops[k] = max3(tops[k], x0, x1);
+                // Probabilities go to the second product in bf16, since kind::f16 multiplies numbers of one type and that is the values': off by 2^-8 of
+                // each at most, which averages out over a row's keys.  Their sum is taken before the rounding, in fp32.
                 const float p0 = ex2(x0), p1 = ex2(x1);  // -inf -> 0
                 rs2[k] = add2(rs2[k], pack2(p0, p1));
                 const __nv_bfloat162 pk = __floats2bfloat162_rn(p0, p1);

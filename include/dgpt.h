@@ -595,9 +595,9 @@ int dgpt_retention(const void* in, int64_t in_row_stride, int32_t q_col, int32_t
  *   o[i,h,:] = sum_j p_j v[j,g,:],  p = softmax_j(q[i,h,:] . k[j,g,:] * scale),  g = h / (H / G)
  * Sequence s has query rows seq_starts[s] .. seq_starts[s + 1] - 1 and key rows key_starts[s] .. key_starts[s + 1] - 1 (key_starts
  * NULL: the query rows').  Its last query sees all of its keys, each query before it one key less; a query that sees none gets
- * zeros.  Rows that belong to no sequence are neither read nor written, and no sequence's numbers reach another's output; within
+ * zeros.  Rows that belong to no sequence reach no output and are left as they are, and no sequence's numbers reach another's output; within
  * a sequence every key and value is a finite number.
- * q, o: element (i,h,d) at i*row_stride + h*head_stride + d; k, v likewise over G heads; pointers 16-byte aligned, strides multiples
+ * q, o: element (i,h,d) at i*row_stride + h*head_stride + d; k, v likewise over G heads; o overlaps none of the others; pointers 16-byte aligned, strides multiples
  * of 8 elements.  lse: fp32 [n_rows, H], the scores' log-sum-exp (-inf where no key is seen), or NULL.
  * seq_starts, key_starts: device int32 [n_seq + 1], not decreasing, within 0 .. n_rows (n_keys); status bit 0 is set where
  * they are not (rows are then wrong, but nothing outside the tensors is touched).
@@ -640,8 +640,8 @@ int dgpt_tree_attn(const void* q, int64_t q_row_stride, const dgpt_kv_layout* kv
  *   logprob[r] = log p[r][targets[r]],  entropy[r] = - sum_j p_j log p_j,  top_ids [R, top_k],  top_logprobs [R, top_k]
  * A logit of -inf is a token that cannot come (probability 0, log probability -inf).  A row that holds a NaN or +inf, or nothing but -inf, has no
  * distribution: its numbers are NaN (its top ids are those of its largest logits, NaN behind all others).
- * logits: device [R, V] with row stride, rows on any boundary of their type; targets: device
- * int32 [R]; temperature: from the smallest normal number to the largest; outputs: fp32 and int32.  A target outside [0, V) gives NaN for its logprob and sets bit 2 of *status (status may be NULL). */
+ * logits: device [R, V] with row stride, rows on any boundary of their type (the aligned 16 bytes that hold a row's first and last logit are read whole, up
+ * to 14 of them before or behind it; what lies there counts for nothing); targets: device int32 [R]; temperature: from the smallest normal number to the largest; outputs: fp32 and int32.  A target outside [0, V) gives NaN for its logprob and sets bit 2 of *status (status may be NULL). */
 int dgpt_token_logprobs(const void* logits, int64_t logits_row_stride, const int32_t* targets, float temperature, float* logprob,
                         float* entropy, int32_t* top_ids, float* top_logprobs, int32_t top_k, int32_t R, int32_t V, int32_t dtype,
                         int32_t* status, void* stream);
@@ -651,7 +651,7 @@ int dgpt_token_logprobs(const void* logits, int64_t logits_row_stride, const int
  * All rows of a sequence are read before the first is written, so source and target may overlap; sequences must not write
  * slots that others read or write.  kv: layer 0's storage (layer l's lies l * layer_stride elements behind it, through the same page
  * table, which has a row for each of the B sequences; a dense layout has at least B); consecutive tokens of a head kv_token_stride elements
- * apart; k_base == v_base: one storage, moved once.
+ * apart; k_base == v_base: one storage, moved once (otherwise keys and values do not overlap); no page stands twice in a sequence's row of the table.
  * path: device int32 [B, T], T <= 256; src_start, dst_start, count: device int32 [B].  A head's row is a multiple of 16 bytes.  A row whose
  * slots do not exist, or lie in a page outside the pool (where the layout states n_pages), is not moved and sets bit 0 of *status, as does a count outside 0 .. T. */
 int dgpt_kv_keep(const dgpt_kv_layout* kv, int64_t kv_token_stride, const int32_t* src_start, const int32_t* dst_start,
